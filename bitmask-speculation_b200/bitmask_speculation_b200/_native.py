@@ -38,7 +38,25 @@ EXPORTS = (
     "bms_masked_reduce_batch_noalloc",
     "bms_exchange_bytes", "bms_exchange_create", "bms_exchange_open", "bms_exchange_close", "bms_exchange_destroy",
     "bms_shard_partials_exchange", "bms_shard_merge_exchange",
+    "bms_filtered_sample_batch", "bms_page_plan", "bms_rotary_append", "bms_attention_workspace_bytes",
+    "bms_chunk_attention",
 )
+
+
+class Filter(ctypes.Structure):
+    """``bms_filter``: scalar sampling parameters, or per-row device arrays where given."""
+
+    _fields_ = [("temperature", ctypes.c_double), ("top_p", ctypes.c_double), ("min_p", ctypes.c_double),
+                ("top_k", ctypes.c_int64), ("temperatures", ctypes.c_void_p), ("top_ps", ctypes.c_void_p),
+                ("min_ps", ctypes.c_void_p), ("top_ks", ctypes.c_void_p)]
+
+
+class Cache(ctypes.Structure):
+    """``bms_paged_cache``: key and value pages and their strides in elements."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("pages", ctypes.c_int64), ("page_size", ctypes.c_int64),
+                ("kv_heads", ctypes.c_int64), ("dim", ctypes.c_int64), ("k_stride", ctypes.c_int64 * 3),
+                ("v_stride", ctypes.c_int64 * 3)]
 
 
 class IpcHandle(ctypes.Structure):
@@ -74,6 +92,10 @@ def _declare(lib) -> None:
         "bms_exchange_close": [i32, p],
         "bms_exchange_destroy": [i32, p],
         "bms_shard_partials_exchange": [p, i32, p, i64, i64, i64, i64, p, i32, i32, i64, ctypes.c_uint32, i32, p],
+        "bms_filtered_sample_batch": [p, i32, p, p, i64, i64, i64, p, p, p, p, p, i32, p],
+        "bms_page_plan": [p, p, p, i64, p, i64, p, i64, p, i64, i64, p, p, p, p, p, p, p, i32, p],
+        "bms_rotary_append": [p, p, p, i32, i64, i64, p, p, p, p, p, i64, p, p, p, p, p, i32, p],
+        "bms_chunk_attention": [p, i32, i64, i64, p, p, p, i64, i64, p, p, f64, i64, i64, p, p, p, p, i64, i32, p],
         "bms_shard_merge_exchange": [p, i32, i32, i64, ctypes.c_uint32, i64, p, p, p, i32, p],
     }
     for name, args in sig.items():
@@ -84,6 +106,8 @@ def _declare(lib) -> None:
     lib.bms_shard_granule_bytes.restype = i64
     lib.bms_workspace_bytes.argtypes = [i32]
     lib.bms_workspace_bytes.restype = i64
+    lib.bms_attention_workspace_bytes.argtypes = [i32, i64, i64, i64, i64]
+    lib.bms_attention_workspace_bytes.restype = i64
     lib.bms_exchange_bytes.argtypes = [i32, i64]
     lib.bms_exchange_bytes.restype = i64
 

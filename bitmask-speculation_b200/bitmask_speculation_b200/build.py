@@ -10,6 +10,7 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
@@ -18,8 +19,9 @@ INCLUDE = PACKAGE.parents[1] / "include"
 LIBRARY = PACKAGE / "_lib" / "libbms_b200.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
-NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
+NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
               "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr"]
+LINK_FLAGS = ["-shared", "-Xcompiler", "-fPIC"]
 
 
 def sources() -> list[Path]:
@@ -46,17 +48,26 @@ def stale() -> bool:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile ``csrc/bms_abi.cu`` into ``_lib/libbms_b200.so`` if stale."""
+    """Compile every ``csrc/*.cu`` (one nvcc each, side by side) into ``_lib/libbms_b200.so`` if stale."""
     if not force and not stale():
         return LIBRARY
     LIBRARY.parent.mkdir(parents=True, exist_ok=True)
     tmp = LIBRARY.with_suffix(f".{os.getpid()}.tmp")
-    cmd = [nvcc(), *ARCH_FLAGS, *NVCC_FLAGS, "-I", str(INCLUDE), "-o", str(tmp),
-           str(SOURCE_ROOT / "bms_abi.cu")]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-    subprocess.run(cmd, check=True)
-    os.replace(tmp, LIBRARY)
+    units = [p for p in sources() if p.suffix == ".cu"]
+    objects = [LIBRARY.parent / f"{p.stem}.{os.getpid()}.o" for p in units]
+
+    def compile_one(pair):
+        flags = [*(["-Xptxas=-v"] if verbose else []), *ARCH_FLAGS, *NVCC_FLAGS]
+        subprocess.run([nvcc(), *flags, "-I", str(INCLUDE), "-c", "-o", str(pair[1]), str(pair[0])], check=True)
+
+    try:
+        with ThreadPoolExecutor(len(units)) as pool:
+            list(pool.map(compile_one, zip(units, objects)))
+        subprocess.run([nvcc(), *ARCH_FLAGS, *LINK_FLAGS, "-o", str(tmp), *map(str, objects)], check=True)
+        os.replace(tmp, LIBRARY)
+    finally:
+        for o in objects:
+            o.unlink(missing_ok=True)
     return LIBRARY
 
 

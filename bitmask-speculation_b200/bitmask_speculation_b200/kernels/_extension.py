@@ -289,6 +289,96 @@ class NativeModule:
             tokens.data_ptr(), None, status.data_ptr(), None, s + 4 * rows, s + 8 * rows, s + 16 * rows,
             s + 20 * rows, mask_rows.data_ptr(), table.shape[0], None, 0, dev.index, _stream(dev)))
 
+    # -- filtered sampling and the paged cache (no reference counterpart) -----------
+    # Arguments were checked by kernels/cuda.py and paged.py; the C library checks every pointer.
+    def filtered_sample_batch(self, logits, mask, mask_rows, temperature, top_k, top_p, min_p, uniforms):
+        """``bms_filtered_sample_batch``: [tokens, kept counts, status] of a batch."""
+        import ctypes
+        torch = _torch()
+        rows, vocab = logits.shape
+        dev = logits.device
+        tokens = torch.empty(rows, dtype=torch.int64, device=dev)
+        kept = torch.empty(rows, dtype=torch.int64, device=dev)
+        status = torch.empty(rows, dtype=torch.int32, device=dev)
+        if rows:
+            f = _native.Filter()
+            for name, value in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p), ("top_k", top_k)):
+                if isinstance(value, torch.Tensor):
+                    setattr(f, name + "s", value.data_ptr())
+                else:
+                    setattr(f, name, value)
+            _native.check(self._lib.bms_filtered_sample_batch(
+                logits.data_ptr(), _dtype_code(logits), None if mask is None else mask.data_ptr(),
+                None if mask_rows is None else mask_rows.data_ptr(), 0 if mask is None else mask.shape[0], rows, vocab,
+                ctypes.byref(f), uniforms.data_ptr(), tokens.data_ptr(), kept.data_ptr(), status.data_ptr(), dev.index,
+                _stream(dev)))
+        return [tokens, kept, status]
+
+    def page_plan(self, past, new, held, table, free_pages, free_count, page_size, tokens):
+        """``bms_page_plan``: query_start, seq_lens, positions, slots, held, free_count, status."""
+        torch = _torch()
+        dev = past.device
+        seqs, width = table.shape
+        # One int32 block for all small outputs; views start on multiples of 4 elements.
+        sizes = (seqs + 1, seqs, tokens, seqs, 1, seqs)
+        at, offsets = 0, []
+        for n in sizes:
+            offsets.append(at)
+            at += (n + 3) // 4 * 4
+        block = torch.empty(at, dtype=torch.int32, device=dev)
+        query_start, seq_lens, positions, held_out, count_out, status = (block[o:o + n] for o, n in zip(offsets, sizes))
+        slots = torch.empty(tokens, dtype=torch.int64, device=dev)
+        base = block.data_ptr()
+        a = [base + 4 * o for o in offsets]
+        _native.check(self._lib.bms_page_plan(
+            past.data_ptr(), new.data_ptr(), held.data_ptr(), seqs, table.data_ptr(), width, free_pages.data_ptr(),
+            free_pages.shape[0], free_count.data_ptr(), page_size, tokens, a[0], a[1], a[2] if tokens else None,
+            slots.data_ptr() if tokens else None, a[3], a[4], a[5], dev.index, _stream(dev)))
+        return [query_start, seq_lens, positions, slots, held_out, count_out, status]
+
+    @staticmethod
+    def _cache(cache):
+        """The cache's ``bms_paged_cache`` (kept on the cache: its tensors do not change)."""
+        import ctypes
+        if cache._native is None:
+            k, v = cache.k, cache.v
+            strides = ctypes.c_int64 * 3
+            cache._native = _native.Cache(k.data_ptr(), v.data_ptr(), *k.shape, strides(*k.stride()[:3]), strides(*v.stride()[:3]))
+        return ctypes.byref(cache._native)
+
+    def rotary_append(self, q, k, v, cos, sin, positions, slots, out, cache, status):
+        import ctypes
+        n, heads, _ = q.shape
+        if n == 0:
+            return
+        pair = ctypes.c_int64 * 2
+        dev = q.device
+        _native.check(self._lib.bms_rotary_append(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), _dtype_code(q), n, heads, pair(*q.stride()[:2]), pair(*k.stride()[:2]),
+            pair(*v.stride()[:2]), cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(), slots.data_ptr(),
+            out.data_ptr(), self._cache(cache), None if status is None else status.data_ptr(), dev.index, _stream(dev)))
+
+    def chunk_attention(self, q, cache, table, seq_lens, query_start, scale, window, sinks, out):
+        """``bms_chunk_attention`` with scratch from the caching allocator (its own in every call and every
+        captured graph): [lse, status]."""
+        import ctypes
+        torch = _torch()
+        n, heads, dim = q.shape
+        seqs, width = table.shape
+        dev = q.device
+        lse = torch.empty((n, heads), dtype=torch.float32, device=dev)
+        status = torch.empty(seqs, dtype=torch.int32, device=dev)
+        nbytes = int(self._lib.bms_attention_workspace_bytes(dev.index, n, heads, seqs, dim))
+        if nbytes < 0:
+            raise RuntimeError(f"no workspace size for device {dev}")
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _native.check(self._lib.bms_chunk_attention(
+            q.data_ptr() if n else None, _dtype_code(q), n, heads, (ctypes.c_int64 * 2)(*q.stride()[:2]), self._cache(cache),
+            table.data_ptr(), seqs, width, seq_lens.data_ptr(), query_start.data_ptr(), scale, window, sinks,
+            out.data_ptr() if n else None, lse.data_ptr() if n else None, status.data_ptr(), ws.data_ptr(), nbytes, dev.index,
+            _stream(dev)))
+        return [lse, status]
+
 
 @lru_cache(maxsize=1)
 def load_extension() -> NativeModule:

@@ -103,3 +103,47 @@ def uniforms_input(uniforms, batch: int, device):
     if uniforms.device != device:
         raise ValueError("uniforms must be on the logits device")
     return uniforms
+
+
+def device_tensor(t, name: str, *, ndim: int, dtype=None, device=None, floating: bool = False):
+    """A strided CUDA tensor of ``ndim`` dimensions, of ``dtype`` (or any of the float types), on ``device``."""
+    import torch
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if floating and t.dtype not in _float_dtypes():
+        raise TypeError(f"{name} must be a float32, bfloat16 or float16 tensor")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} must be a {str(dtype).removeprefix('torch.')} tensor")
+    if t.layout != torch.strided or t.ndim != ndim:
+        raise ValueError(f"{name} must be a strided tensor of {ndim} dimensions")
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must be on CUDA; no implicit transfer")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} must be on the same CUDA device as the other inputs")
+    return t
+
+
+def index_tensor(t, name: str, *, ndim: int, device=None, dtype=None):
+    """A contiguous CUDA tensor of int32 (or the given integer type)."""
+    import torch
+    device_tensor(t, name, ndim=ndim, dtype=torch.int32 if dtype is None else dtype, device=device)
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t
+
+
+def filter_value(value, name: str, batch: int, device, *, low: float, high: float, low_open: bool = False, integer: bool = False):
+    """A filter parameter: a number in range, or a contiguous device tensor [batch] (float32; int32 for counts),
+    whose rows are checked on the device."""
+    import torch
+    if isinstance(value, torch.Tensor):
+        dtype = torch.int32 if integer else torch.float32
+        index_tensor(value, name, ndim=1, device=device, dtype=dtype)
+        if value.shape[0] != batch:
+            raise ValueError(f"{name} must have one value per row")
+        return value
+    if isinstance(value, bool) or not isinstance(value, int if integer else (int, float)):
+        raise TypeError(f"{name} must be {'an integer' if integer else 'numeric'} or a tensor")
+    if not math.isfinite(value) or value > high or value < low or (low_open and value == low):
+        raise ValueError(f"{name} must be in {'(' if low_open else '['}{low}, {high}]")
+    return value

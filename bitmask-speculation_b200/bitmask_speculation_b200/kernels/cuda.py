@@ -3,7 +3,8 @@
 The functions a caller of the reference imports from kernels/cuda.py:7-69 --
 ``mask_count``, ``mask_density``, ``masked_argmax``, ``masked_sample`` and
 ``batched_masked_reduce`` -- with the same arguments, return types and errors,
-plus ``batched_masked_sample`` (one uniform per row).  Inputs must already be on
+plus ``batched_masked_sample`` (one uniform per row) and ``batched_filtered_sample``
+(temperature, top-k, top-p and min-p per row).  Inputs must already be on
 the GPU: nothing here copies, widens or moves a tensor, and a missing library is
 an error, never a CPU computation.
 """
@@ -13,7 +14,7 @@ from __future__ import annotations
 from dataclasses import dataclass
 
 from ._extension import load_extension
-from ._validation import (batched_selection_inputs, mask_input, selection_inputs,
+from ._validation import (batched_selection_inputs, filter_value, index_tensor, mask_input, selection_inputs,
                           temperature_input, uniforms_input)
 
 _MESSAGES = {
@@ -118,3 +119,72 @@ def batched_masked_sample(logits, mask, *, temperature: float, uniforms=None, ge
     uniforms_input(uniforms, batch, logits.device)
     tokens, counts, status = native.masked_sample_batch(logits, mask, temperature, uniforms)
     return BatchedMaskedReduction(tokens, counts, status)
+
+
+@dataclass(frozen=True, slots=True)
+class FilteredSample:
+    """Per-row results of ``batched_filtered_sample``: token (-1 on error), number of tokens the
+    filters kept (0 on error), status code.  ``check()`` reads the statuses back once and raises
+    ValueError listing failed rows."""
+
+    token_ids: object
+    kept_counts: object
+    status: object
+
+    def check(self) -> "FilteredSample":
+        errors = [(row, code) for row, code in enumerate(self.status.tolist()) if code]
+        if errors:
+            raise ValueError(f"invalid filtered rows (row, status): {errors}")
+        return self
+
+
+def batched_filtered_sample(logits, mask, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, uniforms=None,
+                            generator=None, mask_rows=None):
+    """Sample every row of a [B, V] batch from its filtered masked softmax; one float64 uniform per row
+    (drawn if not given).
+
+    A row's valid finite tokens are ordered by (logit descending, token ascending) and weigh
+    exp((x - max) / temperature).  Kept is the shortest of three prefixes of that order: the first
+    ``top_k`` tokens (0: off); of their mass, the tokens whose preceding mass is below ``top_p`` times it
+    (1: off); the tokens weighing at least ``min_p`` (0: off).  The result is the lowest kept token
+    whose running mass in token order exceeds the uniform times the kept mass.  ``temperature`` 0 is
+    the masked argmax.  Each parameter is a number or a [B] tensor on the device (float32; int32 for
+    ``top_k``), mixed as needed; a row whose value is out of range fails with status 10.
+
+    ``mask``: [B, ceil(V / 32)] int32 rows, or None (every token allowed); with ``mask_rows`` (int32
+    [B] on the device) ``mask`` is a table [R, ceil(V / 32)] and row r uses ``mask[mask_rows[r]]`` (status 8
+    for an index outside it).  The other statuses are the sampler's.  Weights and sums are float64:
+    equal inputs give equal tokens whatever the batch around them.  No host synchronization.
+    """
+    import torch
+    if mask is None:
+        if mask_rows is not None:
+            raise ValueError("mask_rows needs a mask table")
+        if not isinstance(logits, torch.Tensor) or logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            raise TypeError("logits must be a float32, bfloat16 or float16 tensor")
+        if logits.layout != torch.strided or logits.ndim != 2 or not logits.is_contiguous() or logits.shape[1] == 0:
+            raise ValueError("logits must be a contiguous [batch, vocab] tensor")
+        if logits.device.type != "cuda":
+            raise ValueError("logits must be on CUDA; no implicit transfer")
+        batch = logits.shape[0]
+    elif mask_rows is None:
+        batch, _ = batched_selection_inputs(logits, mask)
+    else:
+        if not isinstance(mask, torch.Tensor) or mask.ndim != 2 or mask.shape[0] == 0:
+            raise ValueError("mask must be a table [R, ceil(vocab_size / 32)]")
+        batched_selection_inputs(logits[:0], mask[:0])
+        batch = logits.shape[0]
+        if not logits.is_contiguous() or not mask.is_contiguous():
+            raise ValueError("batch inputs must be contiguous two-dimensional strided tensors")
+        if index_tensor(mask_rows, "mask_rows", ndim=1, device=logits.device).shape[0] != batch:
+            raise ValueError("mask_rows must have one index per row")
+    dev = logits.device
+    temperature = filter_value(temperature, "temperature", batch, dev, low=0.0, high=1.7976931348623157e308)
+    top_k = filter_value(top_k, "top_k", batch, dev, low=0, high=2 ** 63 - 1, integer=True)
+    top_p = filter_value(top_p, "top_p", batch, dev, low=0.0, high=1.0, low_open=True)
+    min_p = filter_value(min_p, "min_p", batch, dev, low=0.0, high=1.0)
+    native = load_extension()
+    if uniforms is None:
+        uniforms = torch.rand(batch, dtype=torch.float64, device=dev, generator=generator)
+    uniforms_input(uniforms, batch, dev)
+    return FilteredSample(*native.filtered_sample_batch(logits, mask, mask_rows, temperature, top_k, top_p, min_p, uniforms))

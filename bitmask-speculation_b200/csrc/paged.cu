@@ -1,0 +1,623 @@
+// Paged key/value cache: page planning, rotary append, and attention of a chunk of new tokens.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/bms_b200.h"
+#include "abi_common.cuh"
+
+namespace bms {
+namespace {
+
+constexpr int kMaxPlanSeqs = 8192;
+
+// Entry points may be called while the caller's stream is being captured: pointer queries are
+// allowed there in the relaxed mode only.
+struct RelaxedCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
+template <typename T>
+struct Convert;
+template <>
+struct Convert<float> {
+    static __device__ __forceinline__ float up(float x) { return x; }
+    static __device__ __forceinline__ float down(float x) { return x; }
+};
+template <>
+struct Convert<__nv_bfloat16> {
+    static __device__ __forceinline__ float up(__nv_bfloat16 x) { return __bfloat162float(x); }
+    static __device__ __forceinline__ __nv_bfloat16 down(float x) { return __float2bfloat16_rn(x); }
+};
+template <>
+struct Convert<__half> {
+    static __device__ __forceinline__ float up(__half x) { return __half2float(x); }
+    static __device__ __forceinline__ __half down(float x) { return __float2half_rn(x); }
+};
+
+// ---------------------------------------------------------------- page plan
+struct PlanParams {
+    const int32_t *past, *fresh, *held, *free_count;
+    int32_t *table, *free_pages;
+    int32_t *query_start, *seq_lens, *positions, *held_out, *free_count_out, *status;
+    int64_t* slots;
+    int32_t seqs, width, pages, page_size, tokens;
+};
+
+constexpr int kPlanThreads = 512;
+
+__device__ __forceinline__ int64_t warp_scan(int64_t v, int lane) {
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += up;
+    }
+    return v;
+}
+
+// Inclusive block scan of three values per thread; `carry` holds the running totals before the block.
+__device__ __forceinline__ void block_scan3(int64_t (&v)[3], int64_t (&carry)[3], int64_t (*warp_tot)[3]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int kWarps = kPlanThreads / 32;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) v[i] = warp_scan(v[i], lane);
+    __syncthreads();
+    if (lane == 31) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) warp_tot[warp][i] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        int64_t before = carry[i], all = carry[i];
+        for (int w = 0; w < kWarps; ++w) {
+            const int64_t t = warp_tot[w][i];
+            if (w < warp) before += t;
+            all += t;
+        }
+        v[i] += before;
+        carry[i] = all;
+    }
+}
+
+// Every CTA scans all sequences (new tokens, pages given back, pages taken; 12 bytes each, from L2)
+// into shared memory, then does its share: sequences s = blockIdx.x, blockIdx.x + gridDim.x, ... (table
+// entries, per-sequence outputs) and a contiguous range of tokens, each found by a binary search
+// over the starts.  One launch and no exchange between CTAs; the scan is repeated instead, which
+// costs about a microsecond at 1,024 sequences against a second launch.  Nothing a CTA writes is read by
+// another one: given-back pages are read from entries [need, held) of shrinking rows, taken ones
+// written to entries [held, need) of growing rows; the stack is read below free_count and written
+// from it on.
+__global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanParams p) {
+    extern __shared__ int32_t plan_smem[];
+    __shared__ int64_t warp_tot[kPlanThreads / 32][3];
+    int32_t* start = plan_smem;              // [seqs + 1] first token
+    int32_t* drop_at = start + p.seqs + 1;   // [seqs + 1] pages given back by earlier sequences
+    int32_t* grab_at = drop_at + p.seqs + 1; // [seqs] pages taken by earlier sequences, -1: failed
+    const int64_t page = p.page_size;
+    const int32_t count = min(max(*p.free_count, 0), p.pages);
+
+    int64_t carry[3] = {0, 0, 0};
+    if (threadIdx.x == 0) start[0] = drop_at[0] = 0;
+    for (int base = 0; base < p.seqs; base += kPlanThreads) {
+        const int s = base + threadIdx.x;
+        int64_t v[3] = {0, 0, 0};
+        int64_t past = 0, fresh = 0, held = 0;
+        if (s < p.seqs) {
+            past = p.past[s], fresh = p.fresh[s], held = p.held[s];
+            v[0] = fresh > 0 ? fresh : 0;
+        }
+        // Whether the step's token capacity holds the sequence depends on the starts: scan them first.
+        int64_t first[3] = {v[0], 0, 0}, c0[3] = {carry[0], 0, 0};
+        block_scan3(first, c0, warp_tot);
+        const bool good = s < p.seqs && past >= 0 && fresh >= 0 && held >= 0 && held <= p.width && past <= held * page &&
+                          past + fresh <= p.width * page && first[0] <= p.tokens;
+        const int64_t need = good ? (past + fresh + page - 1) / page : held;
+        v[0] = 0;
+        v[1] = held > need ? held - need : 0;
+        v[2] = need > held ? need - held : 0;
+        const int64_t grab = v[2];
+        int64_t c12[3] = {0, carry[1], carry[2]};
+        block_scan3(v, c12, warp_tot);
+        carry[0] = c0[0], carry[1] = c12[1], carry[2] = c12[2];
+        if (s < p.seqs) {
+            start[s + 1] = static_cast<int32_t>(min(first[0], static_cast<int64_t>(p.tokens)));
+            drop_at[s + 1] = static_cast<int32_t>(v[1]);
+            grab_at[s] = good ? static_cast<int32_t>(v[2] - grab) : -1;
+        }
+    }
+    __syncthreads();
+    const int32_t level = count + drop_at[p.seqs];  // pages that can be handed out
+
+    // A sequence's demand is met iff all demands up to its own fit: later ones cannot overtake it.
+    auto shape = [&](int s, int32_t& held, int32_t& need, bool& good, bool& enough) {
+        held = p.held[s];
+        good = grab_at[s] >= 0;
+        need = good ? static_cast<int32_t>((static_cast<int64_t>(p.past[s]) + p.fresh[s] + page - 1) / page) : held;
+        enough = need <= held || static_cast<int64_t>(grab_at[s]) + need - held <= level;
+        good = good && enough;
+    };
+    // Entry `pos` of the stack of free and given-back pages.
+    auto stack_page = [&](int32_t pos) {
+        if (pos < count) return p.free_pages[pos];
+        const int32_t j = pos - count;
+        int lo = 0, hi = p.seqs - 1;  // the sequence s with drop_at[s] <= j < drop_at[s + 1]
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (drop_at[mid + 1] > j) hi = mid;
+            else lo = mid + 1;
+        }
+        const int32_t need = static_cast<int32_t>((static_cast<int64_t>(p.past[lo]) + p.fresh[lo] + page - 1) / page);
+        return p.table[static_cast<int64_t>(lo) * p.width + need + (j - drop_at[lo])];
+    };
+
+    const int lane = threadIdx.x & 31;
+    const int warps = gridDim.x * (kPlanThreads / 32);
+    for (int s = blockIdx.x * (kPlanThreads / 32) + (threadIdx.x >> 5); s < p.seqs; s += warps) {
+        int32_t held, need;
+        bool good, enough;
+        shape(s, held, need, good, enough);
+        if (good) {
+            int32_t* row = p.table + static_cast<int64_t>(s) * p.width;
+            for (int32_t i = held + lane; i < need; i += 32) row[i] = stack_page(level - 1 - grab_at[s] - (i - held));
+        }
+        if (lane == 0) {
+            p.query_start[s + 1] = start[s + 1];
+            p.seq_lens[s] = good ? p.past[s] + p.fresh[s] : 0;
+            p.held_out[s] = good ? need : held;
+            p.status[s] = good ? BMS_STATUS_OK : (enough ? BMS_STATUS_BAD_LENGTH : BMS_STATUS_NO_PAGES);
+        }
+    }
+    // Pages left on the stack above the old free ones: given back and not taken.
+    int32_t taken = 0;
+    {
+        // The last sequence whose demand is met ends the taken range: demands are met in order.
+        int32_t most = 0;
+        for (int s = threadIdx.x; s < p.seqs; s += kPlanThreads) {
+            int32_t held, need;
+            bool good, enough;
+            shape(s, held, need, good, enough);
+            if (good && need > held) most = max(most, grab_at[s] + need - held);
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+        __syncthreads();
+        if (lane == 0) warp_tot[threadIdx.x >> 5][0] = most;
+        __syncthreads();
+        for (int w = 0; w < kPlanThreads / 32; ++w) taken = max(taken, static_cast<int32_t>(warp_tot[w][0]));
+    }
+    const int32_t left = min(level - taken, p.pages);
+    for (int32_t i = count + blockIdx.x * kPlanThreads + threadIdx.x; i < left; i += gridDim.x * kPlanThreads)
+        p.free_pages[i] = stack_page(i);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        p.query_start[0] = 0;
+        *p.free_count_out = left;
+    }
+
+    const int32_t total = start[p.seqs];
+    for (int32_t t = blockIdx.x * kPlanThreads + threadIdx.x; t < p.tokens; t += gridDim.x * kPlanThreads) {
+        int32_t position = -1;
+        int64_t slot = -1;
+        if (t < total) {
+            int lo = 0, hi = p.seqs - 1;  // the sequence s with start[s] <= t < start[s + 1]
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (start[mid + 1] > t) hi = mid;
+                else lo = mid + 1;
+            }
+            int32_t held, need;
+            bool good, enough;
+            shape(lo, held, need, good, enough);
+            if (good) {
+                position = p.past[lo] + (t - start[lo]);
+                const int32_t i = position / p.page_size;
+                const int32_t pg = i < held ? p.table[static_cast<int64_t>(lo) * p.width + i]
+                                            : stack_page(level - 1 - grab_at[lo] - (i - held));
+                if (pg >= 0 && pg < p.pages) slot = static_cast<int64_t>(pg) * p.page_size + position % p.page_size;
+            }
+        }
+        p.positions[t] = position;
+        p.slots[t] = slot;
+    }
+}
+
+// ---------------------------------------------------------------- rotary append
+struct AppendParams {
+    const void *q, *k, *v;
+    void *q_out, *k_cache, *v_cache;
+    const float *cos, *sin;
+    const int32_t* positions;
+    const int64_t* slots;
+    int32_t* status;
+    int64_t tokens, max_positions, total_slots;
+    int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
+    int64_t kc_page, kc_slot, kc_head, vc_page, vc_slot, vc_head;
+    int32_t heads, kv_heads, half, page_size;
+};
+
+template <typename T, int kVec>
+struct alignas(sizeof(T) * kVec) Pack {
+    T v[kVec];
+};
+
+// A thread owns kVec rotation pairs of one token (kVec elements of each half), keeps their cos and sin
+// in registers, and walks its share of the heads: query heads, then key/value heads (rotate and
+// write the key, copy the value).  Neighbouring threads take neighbouring vectors, so every head's
+// halves move as full lines.  Bound by HBM for long steps; blockIdx.y splits the heads so that short
+// steps still fill the GPU.
+template <typename T, int kVec>
+__global__ void __launch_bounds__(256) rotary_append_kernel(const AppendParams p) {
+    const int chunks = p.half / kVec;
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t t = id / chunks;
+    const int c = static_cast<int>(id % chunks) * kVec;
+    if (t >= p.tokens) return;
+    const int32_t position = p.positions[t];
+    const int64_t slot = p.slots[t];
+    const bool bad_position = position >= p.max_positions, bad_slot = slot >= p.total_slots;
+    if (p.status != nullptr && c == 0 && blockIdx.y == 0)
+        p.status[t] = bad_position ? BMS_STATUS_BAD_POSITION : bad_slot ? BMS_STATUS_BAD_PAGE : BMS_STATUS_OK;
+    if (position < 0 || bad_position || bad_slot) return;
+    float cs[kVec], sn[kVec];
+    const float* cr = p.cos + static_cast<int64_t>(position) * p.half + c;
+    const float* sr = p.sin + static_cast<int64_t>(position) * p.half + c;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) cs[i] = cr[i], sn[i] = sr[i];
+
+    using P = Pack<T, kVec>;
+    auto turn = [&](const T* src, T* dst) {
+        const P a = *reinterpret_cast<const P*>(src + c), b = *reinterpret_cast<const P*>(src + p.half + c);
+        P x, y;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+            const float u = Convert<T>::up(a.v[i]), w = Convert<T>::up(b.v[i]);
+            x.v[i] = Convert<T>::down(fmaf(u, cs[i], -w * sn[i]));
+            y.v[i] = Convert<T>::down(fmaf(u, sn[i], w * cs[i]));
+        }
+        *reinterpret_cast<P*>(dst + c) = x;
+        *reinterpret_cast<P*>(dst + p.half + c) = y;
+    };
+    const int all = p.heads + p.kv_heads;
+    const int64_t dim = 2 * static_cast<int64_t>(p.half);
+    const T* q = static_cast<const T*>(p.q) + t * p.q_tok;
+    T* q_out = static_cast<T*>(p.q_out) + t * p.heads * dim;
+    const int64_t pg = slot / p.page_size, off = slot % p.page_size;
+    for (int h = blockIdx.y; h < all; h += gridDim.y) {
+        if (h < p.heads) {
+            turn(q + h * p.q_head, q_out + h * dim);
+        } else if (slot >= 0) {
+            const int j = h - p.heads;
+            turn(static_cast<const T*>(p.k) + t * p.k_tok + j * p.k_head,
+                 static_cast<T*>(p.k_cache) + pg * p.kc_page + off * p.kc_slot + j * p.kc_head);
+            const T* src = static_cast<const T*>(p.v) + t * p.v_tok + j * p.v_head + c;
+            T* dst = static_cast<T*>(p.v_cache) + pg * p.vc_page + off * p.vc_slot + j * p.vc_head + c;
+            *reinterpret_cast<P*>(dst) = *reinterpret_cast<const P*>(src);
+            *reinterpret_cast<P*>(dst + p.half) = *reinterpret_cast<const P*>(src + p.half);
+        }
+    }
+}
+
+template <typename T>
+int launch_append(const AppendParams& p, int sms, cudaStream_t stream) {
+    constexpr int kVec = 16 / sizeof(T);
+    auto aligned = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
+    const int64_t strides[] = {p.q_tok, p.q_head, p.k_tok, p.k_head, p.v_tok, p.v_head, p.kc_page, p.kc_slot, p.kc_head, p.vc_page, p.vc_slot, p.vc_head};
+    bool wide = p.half % kVec == 0 && aligned(p.q) && aligned(p.k) && aligned(p.v) && aligned(p.q_out) && aligned(p.k_cache) && aligned(p.v_cache);
+    for (const int64_t s : strides) wide = wide && s % kVec == 0;
+    const int64_t threads = p.tokens * (p.half / (wide ? kVec : 1));
+    const int64_t blocks = (threads + 255) / 256;
+    if (blocks > 2147483647LL) return fail(BMS_ERROR_UNSUPPORTED, "too many tokens");
+    const int64_t fill = (16LL * sms + blocks - 1) / blocks;
+    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(std::clamp<int64_t>(fill, 1, std::min<int64_t>(p.heads + p.kv_heads, 65535))));
+    if (wide)
+        rotary_append_kernel<T, kVec><<<grid, 256, 0, stream>>>(p);
+    else
+        rotary_append_kernel<T, 1><<<grid, 256, 0, stream>>>(p);
+    BMS_CUDA(cudaGetLastError(), "rotary append launch");
+    return BMS_SUCCESS;
+}
+
+// ---------------------------------------------------------------- chunk attention
+struct AttendParams {
+    const void* q;
+    const void *k, *v;
+    void* out;
+    float* lse;
+    const int32_t *table, *seq_lens, *query_start;
+    int32_t* status;
+    int64_t tokens, q_tok, q_head;
+    int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;
+    int64_t pages, window, sinks;
+    int32_t seqs, width, page_size, heads, kv_heads, dim;
+    float scale;
+};
+
+// Status of each sequence's lengths.
+__global__ void __launch_bounds__(256) attend_check_kernel(const AttendParams p) {
+    for (int s = blockIdx.x * 256 + threadIdx.x; s < p.seqs; s += gridDim.x * 256) {
+        const int64_t a = p.query_start[s], b = p.query_start[s + 1], len = p.seq_lens[s];
+        const bool bad = a < 0 || b < a || b > p.tokens || len < b - a || len > static_cast<int64_t>(p.width) * p.page_size;
+        p.status[s] = bad ? BMS_STATUS_BAD_LENGTH : BMS_STATUS_OK;
+    }
+}
+
+// Zeroes the rows of failed sequences (those of a sequence whose row range is usable).
+template <typename T>
+__global__ void __launch_bounds__(256) attend_clear_kernel(const AttendParams p) {
+    const int s = blockIdx.x;
+    if (p.status[s] == BMS_STATUS_OK) return;
+    const int64_t a = max(p.query_start[s], 0), b = min(static_cast<int64_t>(p.query_start[s + 1]), p.tokens);
+    const int64_t row = static_cast<int64_t>(p.heads) * p.dim;
+    T* out = static_cast<T*>(p.out);
+    for (int64_t i = a * row + threadIdx.x; i < b * row; i += 256) out[i] = Convert<T>::down(0.f);
+    if (p.lse != nullptr)
+        for (int64_t i = a * p.heads + threadIdx.x; i < b * p.heads; i += 256) p.lse[i] = -INFINITY;
+}
+
+// One warp computes one row (token, head) with plain arithmetic: 32 keys at a time, one per lane, for
+// the scores, a running maximum and sum, then the lanes share the value row's elements.  Keys that
+// the row does not see are never loaded.
+template <typename T>
+__device__ void attend_row(const AttendParams& p, int s, int64_t token, int head, float* qs) {
+    const int lane = threadIdx.x & 31;
+    const int64_t n = p.query_start[s + 1] - p.query_start[s];
+    const int64_t pos = p.seq_lens[s] - n + (token - p.query_start[s]);
+    const int kvh = head / (p.heads / p.kv_heads);
+    const T* q = static_cast<const T*>(p.q) + token * p.q_tok + head * p.q_head;
+    __syncwarp();
+    for (int d = lane; d < p.dim; d += 32) qs[d] = Convert<T>::up(q[d]);
+    __syncwarp();
+    const int32_t* row = p.table + static_cast<int64_t>(s) * p.width;
+    const int64_t low = p.window > 0 ? max(pos + 1 - p.window, static_cast<int64_t>(0)) : 0;
+    const int64_t sinks = min(p.sinks, low);
+    const int64_t visible = sinks + (pos + 1 - low);
+    const float sc = p.scale * 1.4426950408889634f;
+    float m = -INFINITY, l = 0.f, acc[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+    bool bad = false;
+    for (int64_t j0 = 0; j0 < visible; j0 += 32) {
+        const int64_t i = j0 + lane;
+        const int64_t key = i < sinks ? i : low + (i - sinks);
+        float x = -INFINITY;
+        int64_t v_at = 0;
+        const bool live = i < visible;
+        if (live) {
+            const int32_t pg = row[key / p.page_size];
+            const int64_t off = key % p.page_size;
+            if (pg < 0 || pg >= p.pages) {
+                bad = true;
+            } else {
+                const T* kr = static_cast<const T*>(p.k) + pg * p.k_page + off * p.k_slot + kvh * p.k_head;
+                v_at = pg * p.v_page + off * p.v_slot + kvh * p.v_head;
+                float dot = 0.f;
+                for (int d = 0; d < p.dim; ++d) dot = fmaf(qs[d], Convert<T>::up(kr[d]), dot);
+                x = dot * sc;
+            }
+        }
+        if (__any_sync(0xffffffffu, bad)) break;
+        float mx = x;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+        const float mn = fmaxf(m, mx);
+        const float keep = m == -INFINITY ? 0.f : exp2f(m - mn);
+        const float w = live ? exp2f(x - mn) : 0.f;
+        float sum = w;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        l = l * keep + sum;
+        m = mn;
+#pragma unroll
+        for (int i8 = 0; i8 < 8; ++i8) acc[i8] *= keep;
+        const int live_keys = static_cast<int>(min(visible - j0, static_cast<int64_t>(32)));
+        for (int u = 0; u < live_keys; ++u) {
+            const float wu = __shfl_sync(0xffffffffu, w, u);
+            const T* vr = static_cast<const T*>(p.v) + __shfl_sync(0xffffffffu, v_at, u);
+#pragma unroll
+            for (int i8 = 0; i8 < 8; ++i8) {
+                const int d = lane + 32 * i8;
+                if (d < p.dim) acc[i8] = fmaf(wu, Convert<T>::up(vr[d]), acc[i8]);
+            }
+        }
+    }
+    if (__any_sync(0xffffffffu, bad)) {
+        if (lane == 0) atomicMax(&p.status[s], static_cast<int32_t>(BMS_STATUS_BAD_PAGE));
+        return;
+    }
+    T* out = static_cast<T*>(p.out) + (token * p.heads + head) * p.dim;
+#pragma unroll
+    for (int i8 = 0; i8 < 8; ++i8) {
+        const int d = lane + 32 * i8;
+        if (d < p.dim) out[d] = Convert<T>::down(acc[i8] / l);
+    }
+    if (lane == 0 && p.lse != nullptr) p.lse[token * p.heads + head] = m * 0.6931471805599453f + logf(l);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) attend_rows_kernel(const AttendParams p) {
+    __shared__ float qs[8][256];
+    const int64_t rows = p.tokens * p.heads;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); r < rows; r += static_cast<int64_t>(gridDim.x) * 8) {
+        const int64_t token = r / p.heads;
+        int lo = 0, hi = p.seqs;  // the last s with query_start[s] <= token
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (p.query_start[mid + 1] > token) hi = mid;
+            else lo = mid + 1;
+        }
+        if (lo >= p.seqs || p.query_start[lo] > token || p.status[lo] == BMS_STATUS_BAD_LENGTH) continue;
+        attend_row<T>(p, lo, token, static_cast<int>(r % p.heads), qs[threadIdx.x >> 5]);
+    }
+}
+
+template <typename T>
+int launch_attend(const AttendParams& p, int sms, cudaStream_t stream) {
+    attend_check_kernel<<<(p.seqs + 255) / 256, 256, 0, stream>>>(p);
+    const int64_t blocks = std::min<int64_t>((p.tokens * p.heads + 7) / 8, 16LL * sms);
+    if (blocks > 0) attend_rows_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p);
+    attend_clear_kernel<T><<<p.seqs, 256, 0, stream>>>(p);
+    BMS_CUDA(cudaGetLastError(), "chunk attention launch");
+    return BMS_SUCCESS;
+}
+
+int sm_count(int device, int& sms) {
+    static int table[kMaxDevices];
+    if (device >= kMaxDevices) return fail(BMS_ERROR_UNSUPPORTED, "device %d", device);
+    if (table[device] == 0) {
+        int n = 0;
+        BMS_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device), "sm count");
+        table[device] = n;
+    }
+    sms = table[device];
+    return BMS_SUCCESS;
+}
+
+int check_cache(const bms_paged_cache* c, int device, int size) {
+    if (c == nullptr) return fail(BMS_ERROR_INVALID_ARGUMENT, "cache must not be NULL");
+    if (c->pages <= 0 || c->page_size <= 0 || c->kv_heads <= 0 || c->dim <= 0 || c->pages > 2147483647LL || c->page_size > 65536 || c->kv_heads > 65535)
+        return fail(BMS_ERROR_INVALID_ARGUMENT, "invalid cache shape");
+    for (int i = 0; i < 3; ++i)
+        if (c->k_stride[i] < 0 || c->v_stride[i] < 0) return fail(BMS_ERROR_INVALID_ARGUMENT, "cache strides must not be negative");
+    BMS_CHECK(check_ptr(c->k, device, "cache k", size));
+    return check_ptr(c->v, device, "cache v", size);
+}
+
+int check_kind(int dtype) {
+    if (dtype != BMS_FLOAT32 && dtype != BMS_BFLOAT16 && dtype != BMS_FLOAT16)
+        return fail(BMS_ERROR_INVALID_ARGUMENT, "q, k and v must be float32, bfloat16 or float16 (dtype code %d)", dtype);
+    return BMS_SUCCESS;
+}
+
+}  // namespace
+}  // namespace bms
+
+using namespace bms;
+
+extern "C" {
+
+int bms_page_plan(const int32_t* past_lens, const int32_t* new_lens, const int32_t* held, int64_t seqs, int32_t* table, int64_t width,
+                  int32_t* free_pages, int64_t pages, const int32_t* free_count, int64_t page_size, int64_t tokens, int32_t* query_start,
+                  int32_t* seq_lens, int32_t* positions, int64_t* slots, int32_t* held_out, int32_t* free_count_out, int32_t* status,
+                  int32_t device, void* stream) {
+    if (seqs <= 0 || width <= 0 || pages <= 0 || page_size <= 0 || tokens < 0)
+        return fail(BMS_ERROR_INVALID_ARGUMENT, "seqs, width, pages and page_size must be positive and tokens not negative");
+    if (seqs > kMaxPlanSeqs) return fail(BMS_ERROR_UNSUPPORTED, "at most %d sequences per plan", kMaxPlanSeqs);
+    if (pages > 1073741823LL || page_size > 65536 || tokens > 1073741823LL || seqs * width > 1073741823LL || width * page_size > 2147483647LL)
+        return fail(BMS_ERROR_UNSUPPORTED, "pages, tokens or table beyond the 32-bit range");
+    RelaxedCapture relaxed;
+    BMS_CHECK(check_device(device));
+    const void* in[] = {past_lens, new_lens, held, free_count, table, free_pages};
+    const char* in_names[] = {"past_lens", "new_lens", "held", "free_count", "table", "free_pages"};
+    void* outs[] = {query_start, seq_lens, held_out, free_count_out, status, tokens ? positions : nullptr, tokens ? slots : nullptr};
+    const char* out_names[] = {"query_start", "seq_lens", "held_out", "free_count_out", "status", "positions", "slots"};
+    for (int i = 0; i < 6; ++i) BMS_CHECK(check_ptr(in[i], device, in_names[i], 4));
+    for (int i = 0; i < (tokens ? 7 : 5); ++i) {
+        BMS_CHECK(check_ptr(outs[i], device, out_names[i], i == 6 ? 8 : 4));
+        for (const void* x : in)
+            if (x == outs[i]) return fail(BMS_ERROR_INVALID_ARGUMENT, "%s must not alias an input", out_names[i]);
+    }
+    DeviceGuard guard;
+    BMS_CUDA(guard.enter(device), "cudaSetDevice");
+    int sms = 0;
+    BMS_CHECK(sm_count(device, sms));
+    const size_t smem = (3 * static_cast<size_t>(seqs) + 2) * sizeof(int32_t);
+    BMS_CUDA(cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * (kMaxPlanSeqs + 1) * 4), "cudaFuncSetAttribute");
+    const int64_t blocks = std::clamp<int64_t>(std::max((tokens + kPlanThreads - 1) / kPlanThreads, (seqs * 32 + kPlanThreads - 1) / kPlanThreads), 1, sms);
+    const PlanParams p{past_lens, new_lens, held, free_count, table, free_pages, query_start, seq_lens, positions, held_out, free_count_out, status, slots,
+                       static_cast<int32_t>(seqs), static_cast<int32_t>(width), static_cast<int32_t>(pages), static_cast<int32_t>(page_size),
+                       static_cast<int32_t>(tokens)};
+    page_plan_kernel<<<static_cast<unsigned>(blocks), kPlanThreads, smem, static_cast<cudaStream_t>(stream)>>>(p);
+    BMS_CUDA(cudaGetLastError(), "page plan launch");
+    return BMS_SUCCESS;
+}
+
+int bms_rotary_append(const void* q, const void* k, const void* v, int32_t dtype, int64_t tokens, int64_t heads, const int64_t q_stride[2],
+                      const int64_t k_stride[2], const int64_t v_stride[2], const float* cos, const float* sin, int64_t max_positions,
+                      const int32_t* positions, const int64_t* slots, void* q_out, const bms_paged_cache* cache, int32_t* status, int32_t device,
+                      void* stream) {
+    BMS_CHECK(check_kind(dtype));
+    if (tokens < 0 || heads <= 0 || heads > 65535 || max_positions <= 0)
+        return fail(BMS_ERROR_INVALID_ARGUMENT, "tokens, heads and max_positions must be positive");
+    if (q_stride == nullptr || k_stride == nullptr || v_stride == nullptr) return fail(BMS_ERROR_INVALID_ARGUMENT, "strides must not be NULL");
+    const int size = dtype == BMS_FLOAT32 ? 4 : 2;
+    RelaxedCapture relaxed;
+    BMS_CHECK(check_device(device));
+    BMS_CHECK(check_cache(cache, device, size));
+    if (cache->dim % 2 != 0 || cache->dim > 65536) return fail(BMS_ERROR_INVALID_ARGUMENT, "dim must be even");
+    if (tokens == 0) return BMS_SUCCESS;
+    const void* ptrs[] = {q, k, v, q_out};
+    const char* names[] = {"q", "k", "v", "q_out"};
+    for (int i = 0; i < 4; ++i) BMS_CHECK(check_ptr(ptrs[i], device, names[i], size));
+    BMS_CHECK(check_ptr(cos, device, "cos", 4));
+    BMS_CHECK(check_ptr(sin, device, "sin", 4));
+    BMS_CHECK(check_ptr(positions, device, "positions", 4));
+    BMS_CHECK(check_ptr(slots, device, "slots", 8));
+    if (status != nullptr) BMS_CHECK(check_ptr(status, device, "status", 4));
+    DeviceGuard guard;
+    BMS_CUDA(guard.enter(device), "cudaSetDevice");
+    int sms = 0;
+    BMS_CHECK(sm_count(device, sms));
+    const AppendParams p{q, k, v, q_out, cache->k, cache->v, cos, sin, positions, slots, status, tokens, max_positions, cache->pages * cache->page_size,
+                         q_stride[0], q_stride[1], k_stride[0], k_stride[1], v_stride[0], v_stride[1], cache->k_stride[0], cache->k_stride[1],
+                         cache->k_stride[2], cache->v_stride[0], cache->v_stride[1], cache->v_stride[2], static_cast<int32_t>(heads),
+                         static_cast<int32_t>(cache->kv_heads), static_cast<int32_t>(cache->dim / 2), static_cast<int32_t>(cache->page_size)};
+    const auto st = static_cast<cudaStream_t>(stream);
+    if (dtype == BMS_FLOAT32) return launch_append<float>(p, sms, st);
+    if (dtype == BMS_BFLOAT16) return launch_append<__nv_bfloat16>(p, sms, st);
+    return launch_append<__half>(p, sms, st);
+}
+
+int64_t bms_attention_workspace_bytes(int32_t device, int64_t tokens, int64_t heads, int64_t seqs, int64_t dim) {
+    if (device < 0 || tokens < 0 || heads <= 0 || seqs <= 0 || dim <= 0) return -1;
+    return 256;
+}
+
+int bms_chunk_attention(const void* q, int32_t dtype, int64_t tokens, int64_t heads, const int64_t q_stride[2], const bms_paged_cache* cache,
+                        const int32_t* table, int64_t seqs, int64_t width, const int32_t* seq_lens, const int32_t* query_start, double scale,
+                        int64_t window, int64_t sinks, void* out, float* lse, int32_t* status, void* workspace, int64_t workspace_bytes,
+                        int32_t device, void* stream) {
+    BMS_CHECK(check_kind(dtype));
+    if (tokens < 0 || heads <= 0 || heads > 65535 || seqs <= 0 || width <= 0 || seqs > 1048576)
+        return fail(BMS_ERROR_INVALID_ARGUMENT, "tokens, heads, seqs and width must be positive");
+    if (window < 0 || sinks < 0) return fail(BMS_ERROR_INVALID_ARGUMENT, "window and sinks must not be negative");
+    if (!std::isfinite(scale) || std::fabs(scale) > 1e30) return fail(BMS_ERROR_INVALID_ARGUMENT, "scale must be finite");
+    if (q_stride == nullptr) return fail(BMS_ERROR_INVALID_ARGUMENT, "strides must not be NULL");
+    const int size = dtype == BMS_FLOAT32 ? 4 : 2;
+    RelaxedCapture relaxed;
+    BMS_CHECK(check_device(device));
+    BMS_CHECK(check_cache(cache, device, size));
+    if (cache->dim > 256) return fail(BMS_ERROR_UNSUPPORTED, "dim is at most 256");
+    if (heads % cache->kv_heads != 0) return fail(BMS_ERROR_INVALID_ARGUMENT, "heads must be a multiple of the cache's kv_heads");
+    if (tokens > 1073741823LL || width * cache->page_size > 2147483647LL) return fail(BMS_ERROR_UNSUPPORTED, "lengths beyond the 32-bit range");
+    BMS_CHECK(check_ptr(table, device, "table", 4));
+    BMS_CHECK(check_ptr(seq_lens, device, "seq_lens", 4));
+    BMS_CHECK(check_ptr(query_start, device, "query_start", 4));
+    BMS_CHECK(check_ptr(status, device, "status", 4));
+    if (tokens > 0) {
+        BMS_CHECK(check_ptr(q, device, "q", size));
+        BMS_CHECK(check_ptr(out, device, "out", size));
+        if (lse != nullptr) BMS_CHECK(check_ptr(lse, device, "lse", 4));
+    }
+    const int64_t need = bms_attention_workspace_bytes(device, tokens, heads, seqs, cache->dim);
+    BMS_CHECK(check_ptr(workspace, device, "workspace", 256));
+    if (workspace_bytes < need) return fail(BMS_ERROR_INVALID_ARGUMENT, "workspace needs %lld bytes", static_cast<long long>(need));
+    DeviceGuard guard;
+    BMS_CUDA(guard.enter(device), "cudaSetDevice");
+    int sms = 0;
+    BMS_CHECK(sm_count(device, sms));
+    const AttendParams p{q, cache->k, cache->v, out, lse, table, seq_lens, query_start, status, tokens, q_stride[0], q_stride[1],
+                         cache->k_stride[0], cache->k_stride[1], cache->k_stride[2], cache->v_stride[0], cache->v_stride[1], cache->v_stride[2],
+                         cache->pages, window, sinks, static_cast<int32_t>(seqs), static_cast<int32_t>(width), static_cast<int32_t>(cache->page_size),
+                         static_cast<int32_t>(heads), static_cast<int32_t>(cache->kv_heads), static_cast<int32_t>(cache->dim), static_cast<float>(scale)};
+    const auto st = static_cast<cudaStream_t>(stream);
+    if (dtype == BMS_FLOAT32) return launch_attend<float>(p, sms, st);
+    if (dtype == BMS_BFLOAT16) return launch_attend<__nv_bfloat16>(p, sms, st);
+    return launch_attend<__half>(p, sms, st);
+}
+
+}  // extern "C"

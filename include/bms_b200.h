@@ -57,7 +57,11 @@ enum {
     BMS_STATUS_POS_INF = 5,     /* a valid logit is +inf (sampler) */
     BMS_STATUS_BAD_LENGTH = 6,  /* verification: proposal count outside [0, K] */
     BMS_STATUS_TIMEOUT = 7,     /* a bounded device wait expired; row result undefined */
-    BMS_STATUS_BAD_MASK_ROW = 8 /* verification with a mask table: index outside the table */
+    BMS_STATUS_BAD_MASK_ROW = 8, /* verification with a mask table: index outside the table */
+    BMS_STATUS_NO_PAGES = 9,     /* page plan: the pool has too few pages for the sequence */
+    BMS_STATUS_BAD_PARAMETER = 10, /* filtered sampler: a row's temperature or filter is out of range */
+    BMS_STATUS_BAD_PAGE = 11,    /* paged cache: a page or slot index outside the cache */
+    BMS_STATUS_BAD_POSITION = 12 /* rotary append: a position outside the cos/sin tables */
 };
 
 /* Draft budget policy.  kind 0: decoding/scheduling.py:21-46 DensityPolicy
@@ -134,6 +138,30 @@ BMS_API int bms_masked_sample_batch(const void *logits, int32_t dtype, const int
                             int64_t vocab, double temperature, const double *uniforms,
                             int64_t *tokens, int64_t *counts, int32_t *status, void *workspace,
                             int64_t workspace_bytes, int32_t device, void *stream);
+
+/* Filters of bms_filtered_sample_batch: one value for every row, or, where an array is given (device,
+ * [rows]), one per row.  temperature is finite and not negative (0: masked argmax), top_k 0 is off,
+ * top_p is in (0, 1] (1: off), min_p in [0, 1] (0: off). */
+typedef struct bms_filter {
+    double temperature, top_p, min_p;
+    int64_t top_k;
+    const float *temperatures, *top_ps, *min_ps;
+    const int32_t *top_ks;
+} bms_filter;
+
+/* Masked sampling with temperature, top-k, top-p and min-p (no reference counterpart; the reference
+ * samples with a temperature only, csrc/sample.cu:116-132).  The valid finite tokens of a row in the
+ * order (logit descending, token ascending) have weights exp((x - max) / T); kept is the shortest of
+ * the first top_k tokens, those whose preceding mass is below top_p times the mass of the first top_k,
+ * and those with weight >= min_p.  tokens[r] is the lowest kept token whose running mass in token
+ * order exceeds uniforms[r] times the kept mass (float64 throughout), kept[r] their number; -1 and 0
+ * where status[r] is not 0 (10 for a row parameter out of range, else as the sampler's).  `masks` NULL allows every
+ * token; with `mask_rows` (int32 [rows]) row r uses row mask_rows[r] of a table of mask_table_rows
+ * rows (8 for an index outside it).  No workspace. */
+BMS_API int bms_filtered_sample_batch(const void *logits, int32_t dtype, const int32_t *masks, const int32_t *mask_rows,
+                                      int64_t mask_table_rows, int64_t rows, int64_t vocab, const bms_filter *filter,
+                                      const double *uniforms, int64_t *tokens, int64_t *kept, int32_t *status,
+                                      int32_t device, void *stream);
 
 /* Device form of grammar/density.py:23-53 (packed_mask_count / density) and
  * decoding/scheduling.py:40-46 (DensityPolicy.budget) for a [rows, words]
@@ -298,6 +326,71 @@ BMS_API int bms_shard_partials_exchange(const void *logits, int32_t dtype, const
 BMS_API int bms_shard_merge_exchange(void *const *areas, int32_t ranks, int32_t rank, int64_t rows_cap,
                                      uint32_t epoch, int64_t rows, int64_t *tokens, int64_t *counts,
                                      int32_t *status, int32_t device, void *stream);
+
+/* ---- Paged key/value cache (no reference counterpart: the reference recomputes or delegates the
+ * model forward, models/transformers.py:147-201).  A cache holds `pages` pages of `page_size` slots;
+ * slot j of page p is token slot p * page_size + j.  A sequence's block table row lists its pages in
+ * order, so its token t lives in page table[t / page_size], slot t % page_size. */
+typedef struct bms_paged_cache {
+    void *k, *v;        /* [pages, page_size, kv_heads, dim] of the entry point's dtype, dim contiguous */
+    int64_t pages, page_size, kv_heads, dim;
+    int64_t k_stride[3]; /* elements between pages, slots and heads */
+    int64_t v_stride[3];
+} bms_paged_cache;
+
+/* Brings the block tables of `seqs` sequences (at most 8,192) to the lengths of one step.  Sequence s
+ * keeps past_lens[s] tokens and gets new_lens[s] more; it holds held[s] pages of its table row
+ * ([seqs, width] int32).  It then holds exactly ceil((past + new) / page_size) pages: surplus pages
+ * are given back, lacking ones taken from the top of the stack of free pages (free_pages[0,
+ * *free_count), then the pages given back in this call in the order of sequences and entries; a take
+ * pops the last).  Outputs: query_start [seqs + 1] (prefix sums of new_lens, at most `tokens`),
+ * seq_lens [seqs] (past + new), per token of the packed step positions int32 and slots int64
+ * ([tokens]; -1 behind the last sequence and for failed ones), held_out, *free_count_out, and per
+ * sequence a status: 6 for lengths that are negative, do not fit the table row or `tokens`, or exceed
+ * the held pages; 9 when the pool runs out.  A failed sequence keeps its pages and gets seq_lens 0.
+ * `table` and `free_pages` are updated in place, only where no entry that the call reads lies:
+ * the same call again gives the same result.  No output may alias an input. */
+BMS_API int bms_page_plan(const int32_t *past_lens, const int32_t *new_lens, const int32_t *held, int64_t seqs,
+                          int32_t *table, int64_t width, int32_t *free_pages, int64_t pages,
+                          const int32_t *free_count, int64_t page_size, int64_t tokens, int32_t *query_start,
+                          int32_t *seq_lens, int32_t *positions, int64_t *slots, int32_t *held_out,
+                          int32_t *free_count_out, int32_t *status, int32_t device, void *stream);
+
+/* Rotates a step's queries and keys and writes keys and values into the cache.  q [tokens, heads,
+ * dim], k and v [tokens, kv_heads, dim] with the given token and head strides (elements; dim is
+ * contiguous and even).  With half = dim / 2, element i < half and i + half of a head at position p
+ * become a cos[p, i] - b sin[p, i] and a sin[p, i] + b cos[p, i]; cos and sin are float32
+ * [max_positions, half].  Sums in float32, rounded once.  q_out is contiguous [tokens, heads, dim];
+ * token t's key and value go to slot slots[t].  A token with slots[t] < 0 writes no key or value, one
+ * with positions[t] < 0 nothing at all.  `status` (int32 [tokens], may be NULL): 11 for a slot at or
+ * past the cache's end, 12 for a position at or past max_positions (such a token writes nothing).
+ * Slots of one call are distinct (plan_pages gives such slots); of equal ones either may win. */
+BMS_API int bms_rotary_append(const void *q, const void *k, const void *v, int32_t dtype, int64_t tokens, int64_t heads,
+                              const int64_t q_stride[2], const int64_t k_stride[2], const int64_t v_stride[2],
+                              const float *cos, const float *sin, int64_t max_positions, const int32_t *positions,
+                              const int64_t *slots, void *q_out, const bms_paged_cache *cache, int32_t *status,
+                              int32_t device, void *stream);
+
+/* Scratch bytes of bms_chunk_attention (-1 if invalid).  Plain scratch: nothing is kept in it between
+ * calls; calls that may overlap need different scratch. */
+BMS_API int64_t bms_attention_workspace_bytes(int32_t device, int64_t tokens, int64_t heads, int64_t seqs, int64_t dim);
+
+/* Attention of a chunk of new tokens over the paged cache that already holds them.  Sequence s owns
+ * the rows [query_start[s], query_start[s + 1]) of q ([tokens, heads, dim], token and head strides in
+ * elements) and has seq_lens[s] tokens in the cache, its own n rows the last of them: row i is at
+ * position p = seq_lens[s] - n + i and sees the keys j <= p, with window > 0 only those with p - j <
+ * window or j < sinks.  out [tokens, heads, dim] contiguous = softmax(scale q.k) v, lse (float32
+ * [tokens, heads], may be NULL) the natural log of the sum of exp(scale q.k).  heads is a multiple of
+ * kv_heads; head h reads key head h / (heads / kv_heads).  dim is at most 256.  Keys that a row does
+ * not see do not reach it, whatever their bits.  Per-sequence status: 6 for query_start out of order or beyond
+ * `tokens`, seq_lens below n or above the table row; 11 for a visible page outside the cache; the
+ * rows of a failed sequence are 0 with lse -inf.  Rows behind query_start[seqs] are left as they
+ * were. */
+BMS_API int bms_chunk_attention(const void *q, int32_t dtype, int64_t tokens, int64_t heads, const int64_t q_stride[2],
+                                const bms_paged_cache *cache, const int32_t *table, int64_t seqs, int64_t width,
+                                const int32_t *seq_lens, const int32_t *query_start, double scale, int64_t window,
+                                int64_t sinks, void *out, float *lse, int32_t *status, void *workspace,
+                                int64_t workspace_bytes, int32_t device, void *stream);
 
 /* Test hook: force the cluster size (1, 2, 4, 8 or 16) and the number of
  * clusters of the selection kernels' fixed schedule; 0 restores the automatic
