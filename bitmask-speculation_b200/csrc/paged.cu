@@ -346,17 +346,20 @@ __global__ void __launch_bounds__(256) attend_check_kernel(const AttendParams p)
     }
 }
 
-// Zeroes the rows of failed sequences (those of a sequence whose row range is usable).
+// Zeroes the rows of a failed sequence, as far as its row range is usable.
 template <typename T>
-__global__ void __launch_bounds__(256) attend_clear_kernel(const AttendParams p) {
-    const int s = blockIdx.x;
-    if (p.status[s] == BMS_STATUS_OK) return;
+__device__ void clear_rows(const AttendParams& p, int s) {
     const int64_t a = max(p.query_start[s], 0), b = min(static_cast<int64_t>(p.query_start[s + 1]), p.tokens);
     const int64_t row = static_cast<int64_t>(p.heads) * p.dim;
     T* out = static_cast<T*>(p.out);
-    for (int64_t i = a * row + threadIdx.x; i < b * row; i += 256) out[i] = Convert<T>::down(0.f);
+    for (int64_t i = a * row + threadIdx.x; i < b * row; i += blockDim.x) out[i] = Convert<T>::down(0.f);
     if (p.lse != nullptr)
-        for (int64_t i = a * p.heads + threadIdx.x; i < b * p.heads; i += 256) p.lse[i] = -INFINITY;
+        for (int64_t i = a * p.heads + threadIdx.x; i < b * p.heads; i += blockDim.x) p.lse[i] = -INFINITY;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) attend_clear_kernel(const AttendParams p) {
+    if (p.status[blockIdx.x] != BMS_STATUS_OK) clear_rows<T>(p, blockIdx.x);
 }
 
 // One warp computes one row (token, head) with plain arithmetic: 32 keys at a time, one per lane, for
@@ -453,6 +456,88 @@ __global__ void __launch_bounds__(256) attend_rows_kernel(const AttendParams p) 
         if (lo >= p.seqs || p.query_start[lo] > token || p.status[lo] == BMS_STATUS_BAD_LENGTH) continue;
         attend_row<T>(p, lo, token, static_cast<int>(r % p.heads), qs[threadIdx.x >> 5]);
     }
+}
+
+}  // namespace
+}  // namespace bms
+
+#include "attend.cuh"
+
+namespace bms {
+namespace {
+
+using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
+
+// The driver's tensor-map encoder, looked up once (the library links no driver stub).
+EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            f = nullptr;
+        }
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    return fn;
+}
+
+// Where the tile kernel takes a call: 16-bit types, dim 64 or 128, pages that divide or are divided by a tile's 128 keys
+// and hold whole 8-row swizzle groups, everything on 16-byte boundaries (TMA, 16-byte query loads and
+// result stores), at most 128 query heads per key head.  Other calls go row by row.
+bool tiles_fit(const AttendParams& p, int dtype) {
+    if (dtype == BMS_FLOAT32 || (p.dim != 64 && p.dim != 128) || p.page_size % 8 != 0) return false;
+    if (tc::kTile % p.page_size != 0 && p.page_size % tc::kTile != 0) return false;
+    if (tc::kTile / std::min(p.page_size, tc::kTile) > 16 || p.heads / p.kv_heads > tc::kTile || encode_tiled() == nullptr) return false;
+    for (const void* x : {p.q, p.k, p.v, static_cast<const void*>(p.out)})
+        if (reinterpret_cast<uintptr_t>(x) % 16 != 0) return false;
+    for (const int64_t s : {p.q_tok, p.q_head, p.k_page, p.k_slot, p.k_head, p.v_page, p.v_slot, p.v_head})
+        if (s % 8 != 0 || s >= (1LL << 38)) return false;
+    return true;
+}
+
+int page_map(CUtensorMap* map, const AttendParams& p, int dtype, const void* base, int64_t page, int64_t slot, int64_t head) {
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(p.dim), static_cast<cuuint64_t>(p.kv_heads), static_cast<cuuint64_t>(p.page_size),
+                                static_cast<cuuint64_t>(p.pages)};
+    // A dimension of one entry may have any stride: 16 bytes stand in for one of 0.
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(std::max<int64_t>(head * 2, 16)), static_cast<cuuint64_t>(std::max<int64_t>(slot * 2, 16)),
+                                   static_cast<cuuint64_t>(std::max<int64_t>(page * 2, 16))};
+    const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(std::min(p.page_size, tc::kTile)), 1};
+    const cuuint32_t steps[4] = {1, 1, 1, 1};
+    const CUresult rc = encode_tiled()(map, dtype == BMS_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                                       const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) return fail(BMS_ERROR_CUDA, "tensor map of the cache (driver error %d)", static_cast<int>(rc));
+    return BMS_SUCCESS;
+}
+
+int64_t tiles_workspace(int64_t ctas, int64_t dim) { return 256 + ctas * 2 * 256 * (dim + 1) * 4 + ((ctas * 4 + 255) / 256) * 256; }
+
+template <typename T, int D>
+int launch_tiles(const AttendParams& a, int dtype, int device, int sms, void* workspace, cudaStream_t stream) {
+    static bool ready[kMaxDevices];
+    auto kernel = tc::attend_tiles_kernel<T, D>;
+    if (!ready[device]) {
+        BMS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tc::Layout<D>::kSmem), "cudaFuncSetAttribute(smem)");
+        ready[device] = true;
+    }
+    CUtensorMap k_map, v_map;
+    BMS_CHECK(page_map(&k_map, a, dtype, a.k, a.k_page, a.k_slot, a.k_head));
+    BMS_CHECK(page_map(&v_map, a, dtype, a.v, a.v_page, a.v_slot, a.v_head));
+    tc::Params p{};
+    p.a = a;
+    p.flags = static_cast<int32_t*>(workspace);
+    unsigned char* rest = static_cast<unsigned char*>(workspace) + ((sms * 4 + 255) / 256) * 256;
+    p.parts = reinterpret_cast<float*>(rest);
+    p.part_lse = p.parts + static_cast<int64_t>(sms) * 2 * 256 * D;
+    p.scale2 = std::max(std::fabs(a.scale) * 1.4426950408889634f, 1e-30f);  // a factor of 0 would turn masked scores into NaN
+    p.negate = a.scale < 0.f ? 0x80008000u : 0u;
+    p.group = a.heads / a.kv_heads;
+    p.tile_tokens = tc::kTile / p.group;
+    kernel<<<sms, tc::kThreads, tc::Layout<D>::kSmem, stream>>>(k_map, v_map, p);
+    tc::attend_finish_kernel<T, D><<<sms, tc::kFinishThreads, 0, stream>>>(p);
+    BMS_CUDA(cudaGetLastError(), "chunk attention launch");
+    return BMS_SUCCESS;
 }
 
 template <typename T>
@@ -573,8 +658,9 @@ int bms_rotary_append(const void* q, const void* k, const void* v, int32_t dtype
 }
 
 int64_t bms_attention_workspace_bytes(int32_t device, int64_t tokens, int64_t heads, int64_t seqs, int64_t dim) {
-    if (device < 0 || tokens < 0 || heads <= 0 || seqs <= 0 || dim <= 0) return -1;
-    return 256;
+    int sms = 0;
+    if (device < 0 || tokens < 0 || heads <= 0 || seqs <= 0 || dim <= 0 || sm_count(device, sms) != BMS_SUCCESS) return -1;
+    return dim == 64 || dim == 128 ? tiles_workspace(sms, dim) : 256;
 }
 
 int bms_chunk_attention(const void* q, int32_t dtype, int64_t tokens, int64_t heads, const int64_t q_stride[2], const bms_paged_cache* cache,
@@ -616,8 +702,13 @@ int bms_chunk_attention(const void* q, int32_t dtype, int64_t tokens, int64_t he
                          static_cast<int32_t>(heads), static_cast<int32_t>(cache->kv_heads), static_cast<int32_t>(cache->dim), static_cast<float>(scale)};
     const auto st = static_cast<cudaStream_t>(stream);
     if (dtype == BMS_FLOAT32) return launch_attend<float>(p, sms, st);
-    if (dtype == BMS_BFLOAT16) return launch_attend<__nv_bfloat16>(p, sms, st);
-    return launch_attend<__half>(p, sms, st);
+    const bool bf16 = dtype == BMS_BFLOAT16;
+    if (tokens > 0 && tiles_fit(p, dtype)) {
+        if (p.dim == 64)
+            return bf16 ? launch_tiles<__nv_bfloat16, 64>(p, dtype, device, sms, workspace, st) : launch_tiles<__half, 64>(p, dtype, device, sms, workspace, st);
+        return bf16 ? launch_tiles<__nv_bfloat16, 128>(p, dtype, device, sms, workspace, st) : launch_tiles<__half, 128>(p, dtype, device, sms, workspace, st);
+    }
+    return bf16 ? launch_attend<__nv_bfloat16>(p, sms, st) : launch_attend<__half>(p, sms, st);
 }
 
 }  // extern "C"
