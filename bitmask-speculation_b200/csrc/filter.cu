@@ -7,18 +7,18 @@
 //
 // A cluster of C CTAs owns a row, each CTA a contiguous slice, each warp a contiguous span of it.  The
 // row is streamed from HBM once (maximum, counts, NaN); later passes hit L2, because only the rows in
-// flight are live there.  Order keys are 64-bit: ordered float bits, then the complement of the token, so that ties
-// are part of the key and every prefix is "key >= cut".
+// flight are live there.  A place in the order is a score and a token (`Place`); every filter ends at one.
 //
 // Passes.  The first one also gives a lower bound of the k-th largest score for free: G disjoint
 // groups of lanes each hold a token at or above the smallest of their maxima, so at least G tokens reach it.
-//  * Few tokens in play (k small, min-p alone, or a sparse mask): they are collected into shared
-//    memory, sorted, weighed and cut there; only they are ever exponentiated.
+//  * Few tokens in play (k small, min-p alone, or a sparse mask): one pass collects them in token order into
+//    shared memory (vectors whose maximum stays below the bound cost a handful of instructions), and
+//    one CTA orders, weighs, cuts and draws there; only these tokens are ever exponentiated.
 //  * Otherwise one counting pass over value bins estimates where the nucleus ends, one weighing pass
 //    sums the exact masses above and below a bracket of bins around that place and collects the
-//    bracket's tokens, whose sorted prefix gives the exact cut; if the estimate missed or a
-//    bracket overflows (runs of equal scores), the cut is bisected over the order keys instead.
-//    A last pass weighs the kept tokens by spans, and one CTA walks the span that holds u.
+//    bracket's tokens, whose sorted prefix gives the exact end; if the estimate missed, the exact masses place
+//    the next bracket, and if a bracket overflows (runs of equal scores) the end is bisected over the
+//    64-bit order keys instead.  The kept masses by spans give the span that holds u, which one CTA walks.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -27,10 +27,13 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <cstdlib>
 #include <cstring>
+#include <type_traits>
 
 #include "../../include/bms_b200.h"
 #include "abi_common.cuh"
+#include "ptx.cuh"
 
 namespace bms {
 namespace {
@@ -41,8 +44,14 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 16;
 constexpr int kCap = 4096;   // tokens that the list path holds
-constexpr int kBins = 8192;  // value bins of the counting pass
+constexpr int kSegment = 512;  // of them in one warp's span
+constexpr int kTable = 512;    // powers 2^(j / 512)
+constexpr int kBins = 4096;   // value bins of the counting pass
+// A warp's queue: 63 tokens left over and a round of one 16-byte vector per lane.
+template <typename T>
+constexpr int kQueue = 64 + 32 * 16 / static_cast<int>(sizeof(T));
 constexpr int kPerThread = kBins / kThreads;
+constexpr int kWide = kCap / kThreads;  // list entries per thread
 
 struct FilterParams {
     const void* logits;
@@ -62,7 +71,7 @@ struct FilterParams {
 struct RowStats {
     float max;               // maximum of the valid tokens
     float low[3];            // smallest maximum of the groups of 32, 8 and 1 lanes
-    uint32_t finite, flags;  // valid finite tokens; 1 NaN, 2 some valid token
+    uint32_t finite, flags;  // valid tokens; 1 NaN, 2 some valid token, 4 a valid -inf
 };
 
 __device__ __forceinline__ void merge(RowStats& a, const RowStats& o) {
@@ -73,35 +82,56 @@ __device__ __forceinline__ void merge(RowStats& a, const RowStats& o) {
     a.flags |= o.flags;
 }
 
+// A place in the order of a row's tokens, as an order key or in parts: tokens up to it are kept.
+struct Place {
+    float x;
+    uint32_t t;
+    __device__ __forceinline__ bool keeps(float y, uint32_t s) const { return y > x || (y == x && s <= t); }
+};
+
 struct MassCount {
     double mass;
     int64_t count;
 };
 
 struct Shared {
+    double top, rate, top_p, u;     // the row: maximum, 512 / (T ln 2), nucleus, uniform
+    float topf, floor_x;            // maximum; lowest score that min-p keeps
+    float width, bin_scale, bin_at; // value bins: their width, and a score's bin is bin_at - x * bin_scale
+    int32_t shift;                  // order bits that the scores' type leaves constant
+    int64_t k;                      // tokens that top-k keeps
+    uint64_t first_k;               // order key of the last of them
+    int32_t bounds[kWarps + 1];     // the warps' spans, in groups
+    int32_t b0, b1;                 // bracket of bins
+    alignas(16) unsigned char view[64];  // RowView
     union {
-        uint64_t list[kCap];
+        uint64_t list[kCap];   // order keys
         uint32_t bins[kBins];  // this CTA's counts, until every CTA has read them
     };
-    double weight[kCap];
-    uint32_t merged[kBins];
+    union {
+        struct {
+            uint32_t merged[kBins];  // the row's counts
+            uint32_t queue[kWarps][2 * kQueue<float>];
+        };
+        uint64_t segment[kWarps][kSegment];  // keys that a warp collected, until they are in the list
+        RowStats warp_stats[kWarps];
+    };
+    double exp_table[kTable];
     double spans[kMaxCluster * kWarps];
+    unsigned long long extra[kMaxCluster * kWarps];  // kept bracket tokens' mass by span, units of 2^-50
+    uint32_t warp_counts[kMaxCluster * kWarps];
     MassCount part[2][kMaxCluster];
     RowStats stats[kMaxCluster];
-    double warp_mass[kWarps];
-    int64_t warp_count[kWarps];
-    double exp_table[64];  // 2^(j / 64)
-    uint64_t cut;
+    double warp_mass[kWarps], warp_below[kWarps], step_mass[2][kWarps];
+    int64_t warp_count[kWarps], counts[kMaxCluster];
     double above[kMaxCluster], below[kMaxCluster];
+    double target, before;
+    uint64_t cut;
     uint32_t list_counts[kMaxCluster];
-    uint32_t list_count, list_base;
+    uint32_t list_count, bin_count, pick, last, passed;
     int32_t bin[3];
-    uint32_t bin_count;
-    float goal;
-    int32_t found, owner;
-    double before;
-    uint32_t pick;
-    int64_t token;
+    float goal, floor;
+    int32_t found, owner, token;
 };
 
 __device__ __forceinline__ uint32_t order_bits(float x) {
@@ -115,9 +145,45 @@ __device__ __forceinline__ uint64_t order_key(float x, uint32_t token) {
     return (static_cast<uint64_t>(order_bits(x)) << 32) | (0xffffffffu - token);
 }
 
+__device__ __forceinline__ Place place_of(uint64_t key) { return {order_value(static_cast<uint32_t>(key >> 32)), 0xffffffffu - static_cast<uint32_t>(key)}; }
+
 __device__ __forceinline__ float widen(float x) { return x; }
 __device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float widen(__half x) { return __half2float(x); }
+
+// Two 16-bit scores in a word.
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__nv_bfloat16> {
+    static constexpr uint32_t kInf = 0x7f807f80u;
+    static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) { return ptx::max_bf16x2(a, b); }
+    static __device__ __forceinline__ uint32_t max_nan(uint32_t a, uint32_t b) { return ptx::max_nan_bf16x2(a, b); }
+    static __device__ __forceinline__ uint32_t min(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("min.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ float lo(uint32_t u) { return __uint_as_float(u << 16); }
+    static __device__ __forceinline__ float hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+};
+template <>
+struct Pair<__half> {
+    static constexpr uint32_t kInf = 0x7c007c00u;
+    static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) { return ptx::max_f16x2(a, b); }
+    static __device__ __forceinline__ uint32_t max_nan(uint32_t a, uint32_t b) { return ptx::max_nan_f16x2(a, b); }
+    static __device__ __forceinline__ uint32_t min(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("min.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ float lo(uint32_t u) { return __half2float(__ushort_as_half(static_cast<unsigned short>(u))); }
+    static __device__ __forceinline__ float hi(uint32_t u) { return __half2float(__ushort_as_half(static_cast<unsigned short>(u >> 16))); }
+};
+template <>
+struct Pair<float> {
+    static constexpr uint32_t kInf = 0;
+};
 
 template <typename T>
 __device__ __forceinline__ T narrow(float x) {
@@ -125,99 +191,171 @@ __device__ __forceinline__ T narrow(float x) {
     else return T(x);
 }
 
-// Eight consecutive tokens of a row, aligned to 16 bytes of the row's own address, and their mask bits.
+// A row as 16-byte vectors ("groups") on 16-byte boundaries, whatever the row's own address, and their mask bits.
+// Groups [full0, full1) lie wholly in the row; the few tokens before and behind them (`edge`) are taken one per lane.
 template <typename T>
 struct RowView {
+    static constexpr int kVec = 16 / sizeof(T);
+    static constexpr uint32_t kAll = (1u << kVec) - 1u;
     const T* row;
     const int32_t* mask;
-    int64_t vocab;
+    uint32_t vocab;
     int32_t skew;  // elements from the 16-byte boundary below the row's start
-    __device__ int64_t groups() const { return (vocab + skew + 7) / 8; }
-    __device__ __forceinline__ int64_t first(int64_t g) const { return g * 8 - skew; }
-    struct Raw {
-        uint4 v[sizeof(T) / 2];
-    };
-    __device__ __forceinline__ Raw fetch(int64_t g) const {
-        const int64_t t = first(g);
-        Raw r;
-        if (t >= 0 && t + 8 <= vocab) {
-#pragma unroll
-            for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.v[i] = __ldg(reinterpret_cast<const uint4*>(row + t) + i);
-        } else {  // the row's ends
-            T e[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = t + i >= 0 && t + i < vocab ? row[t + i] : narrow<T>(-INFINITY);
-            memcpy(&r, e, sizeof r);
+    int32_t groups, full0, full1;
+    RowView() = default;
+    __device__ RowView(const T* r, const int32_t* m, int64_t n) : row(r), mask(m), vocab(static_cast<uint32_t>(n)) {
+        skew = static_cast<int32_t>((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T));
+        groups = static_cast<int32_t>((n + skew + kVec - 1) / kVec);
+        full0 = skew ? 1 : 0;
+        full1 = max(full0, static_cast<int32_t>((n + skew) / kVec));
+    }
+    __device__ __forceinline__ int32_t first(int32_t g) const { return g * kVec - skew; }
+    // A group of [full0, full1).
+    __device__ __forceinline__ uint4 fetch(int32_t g) const { return __ldg(reinterpret_cast<const uint4*>(row - skew) + g); }
+    static __device__ __forceinline__ void expand(const uint4& r, float (&x)[kVec]) {
+        if constexpr (sizeof(T) == 4) {
+            x[0] = __uint_as_float(r.x), x[1] = __uint_as_float(r.y), x[2] = __uint_as_float(r.z), x[3] = __uint_as_float(r.w);
+        } else {
+            x[0] = Pair<T>::lo(r.x), x[1] = Pair<T>::hi(r.x), x[2] = Pair<T>::lo(r.y), x[3] = Pair<T>::hi(r.y);
+            x[4] = Pair<T>::lo(r.z), x[5] = Pair<T>::hi(r.z), x[6] = Pair<T>::lo(r.w), x[7] = Pair<T>::hi(r.w);
         }
-        return r;
     }
-    static __device__ __forceinline__ void expand(const Raw& r, float (&x)[8]) {
-        T e[8];
-        memcpy(e, &r, sizeof r);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = widen(e[i]);
+    __device__ __forceinline__ uint32_t bits(int32_t g) const {
+        if (mask == nullptr) return kAll;
+        const uint32_t t = static_cast<uint32_t>(first(g)), w = t >> 5, sh = t & 31;
+        uint32_t b = static_cast<uint32_t>(__ldg(mask + w)) >> sh;
+        if (sh > 32 - kVec) b |= static_cast<uint32_t>(__ldg(mask + w + 1)) << (32 - sh);
+        return b & kAll;
     }
-    __device__ __forceinline__ void load(int64_t g, float (&x)[8]) const { expand(fetch(g), x); }
-    __device__ __forceinline__ uint32_t bits(int64_t g) const {
-        const int64_t t = first(g);
-        uint32_t b = 0xffu;
-        if (mask != nullptr) {
-            if (t >= 0) {
-                const int64_t w = t >> 5;
-                const int sh = t & 31;
-                b = static_cast<uint32_t>(mask[w]) >> sh;
-                if (sh > 24 && (w + 1) * 32 < vocab) b |= static_cast<uint32_t>(mask[w + 1]) << (32 - sh);
-            } else {
-                b = static_cast<uint32_t>(mask[0]) << -t;
-            }
-            b &= 0xffu;
-        }
-        if (t < 0) b &= 0xffu << -t;
-        if (t + 8 > vocab) b &= 0xffu >> (t + 8 - vocab);
-        return b;
+    // This lane's token outside the full groups of [g0, g1), or -1.
+    __device__ __forceinline__ int32_t edge(int32_t g0, int32_t g1) const {
+        const int lane = threadIdx.x & 31;
+        if (lane < kVec) return g0 == 0 && g1 > 0 && full0 && lane < min(first(1), static_cast<int32_t>(vocab)) ? lane : -1;
+        const int32_t t = first(full1) + lane - kVec;
+        return full1 >= g0 && full1 < g1 && full1 < groups && lane < 2 * kVec && t < static_cast<int32_t>(vocab) ? t : -1;
     }
+    __device__ __forceinline__ bool valid(int32_t t) const { return mask == nullptr || (static_cast<uint32_t>(mask[t >> 5]) >> (t & 31) & 1); }
 };
 
-// exp((x - top) * inv_t), float64: z = n ln2 / 64 + r, |r| <= ln2 / 128; 2^(n / 64) from a 64-entry table and the exponent
-// field, e^r by its series to r^5 (the next term is below 4e-17).  Relative error about 1e-16 + |z| 2^-53, far
-// below what decides a token; a third of the instructions of the library's exp.  Weights that come near the
-// subnormals (z < -690) take that.
-__device__ __forceinline__ double weight_of(float x, double top, double inv_t, const double* table) {
-    const double z = (static_cast<double>(x) - top) * inv_t;
-    if (z < -690.0) return exp(z);
+// exp((x - top) / T), float64: t = (x - top) * rate in units of 2^(1/512) splits into an integer n and |r| <= 1/2; 2^(n / 512)
+// comes from a table and the exponent field, 2^(r / 512) from its series to r^3 (the next term is below 1e-14
+// relative), far below what decides a token.  Branch-free, a quarter of the instructions of the library's exp.
+// Weights between 2^-1022 and 2^-1075 stay near 2^-1022, smaller ones are 0.
+__device__ __forceinline__ double weight_of(float x, double top, double rate, const double* table) {
     constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer in the low bits
-    const double shifted = fma(z, 92.332482616893656877, kMagic);  // 64 / ln 2
+    constexpr double kLn = 0.0013538030870311432;  // ln 2 / 512
+    const double t = (static_cast<double>(x) - top) * rate;
+    const double shifted = t + kMagic;
     const int n = __double2loint(shifted);
-    const double r = fma(shifted - kMagic, -0.010830424696249145, z);  // ln 2 / 64
-    double e = fma(r, 1.0 / 120.0, 1.0 / 24.0);
-    e = fma(e, r, 1.0 / 6.0);
-    e = fma(e, r, 0.5);
+    const double r = t - (shifted - kMagic);
+    double e = fma(r, kLn * kLn * kLn / 6.0, kLn * kLn / 2.0);
+    e = fma(e, r, kLn);
     e = fma(e, r, 1.0);
-    e = fma(e, r, 1.0);
-    e *= table[n & 63];
-    return __hiloint2double(__double2hiint(e) + (n >> 6) * 1048576, __double2loint(e));
+    e *= table[n & (kTable - 1)];
+    e = __hiloint2double(__double2hiint(e) + (max(n, -1022 * kTable) >> 9) * 1048576, __double2loint(e));
+    return t < -1075.0 * kTable ? 0.0 : e;
 }
 
-// Calls f(token of element 0, x[8], valid bits) for the groups [g0, g1) with any valid token; several groups' loads are
-// in flight at once.
+// Calls f(x, token, live) for the valid tokens of the groups [g0, g1), two per lane at a time.  Rounds in which every
+// token is valid go straight from the registers; in others the valid tokens of a round of one vector per lane go
+// through the warp's queue in shared memory, so that f's cost follows their number and not the vocabulary
+// (grammar masks keep 0.1 - 60 % of it).  A queue entry is 16 bits of score and 16 of offset for 16-bit
+// types, 8 bytes for float32.
 template <typename T, typename F>
-__device__ __forceinline__ void each_group(const RowView<T>& v, int64_t g0, int64_t g1, F f) {
-    constexpr int kBatch = sizeof(T) == 4 ? 2 : 4;
-    for (int64_t g = g0 + (threadIdx.x & 31); g < g1; g += 32 * kBatch) {
-        uint32_t b[kBatch];
-        typename RowView<T>::Raw raw[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) b[i] = g + 32 * i < g1 ? v.bits(g + 32 * i) : 0u;
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-            if (b[i]) raw[i] = v.fetch(g + 32 * i);
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-            if (b[i]) {
-                float x[8];
-                v.expand(raw[i], x);
-                f(v.first(g + 32 * i), x, b[i]);
+__device__ __forceinline__ void each_token(const RowView<T>& v, int32_t g0, int32_t g1, uint32_t* queue, F f) {
+    constexpr bool kHalf = sizeof(T) == 2;
+    constexpr int kVec = RowView<T>::kVec, kBatch = 4;
+    constexpr int kGroups = 65536 / kVec;  // offsets stay within 16 bits
+    const int lane = threadIdx.x & 31;
+    const uint32_t below = (1u << lane) - 1u;
+    const int32_t a = max(g0, v.full0), z = min(g1, v.full1);
+    for (int32_t base = a; base < z; base += kGroups) {
+        const int groups = min(z - base, kGroups);
+        const int32_t t0 = v.first(base);
+        int fill = 0;
+        auto pop = [&](int i) {
+            const bool live = i < fill;
+            float x = -INFINITY;
+            int32_t t = t0;
+            if (live) {
+                if constexpr (kHalf) {
+                    const uint32_t e = queue[i];
+                    x = Pair<T>::lo(e);
+                    t += e >> 16;
+                } else {
+                    const uint2 e = reinterpret_cast<const uint2*>(queue)[i];
+                    x = __uint_as_float(e.x);
+                    t += e.y;
+                }
             }
+            f(x, static_cast<uint32_t>(t), x > -INFINITY);
+        };
+        for (int i0 = 0; i0 < groups; i0 += 32 * kBatch) {
+            uint32_t b[kBatch];
+            uint4 raw[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) b[i] = i0 + 32 * i + lane < groups ? v.bits(base + i0 + 32 * i + lane) : 0u;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+                if (b[i]) raw[i] = v.fetch(base + i0 + 32 * i + lane);
+            // Rolled, so that f exists once per way: the round's vector moves to the front instead of being indexed.
+#pragma unroll 1
+            for (int i = 0; i < kBatch; ++i) {
+                const bool ends = i0 + 32 * (i + 1) >= groups;  // the last round empties the queue
+                const uint32_t bits = b[0];
+                uint4 now = raw[0];
+#pragma unroll
+                for (int j = 1; j < kBatch; ++j) b[j - 1] = b[j], raw[j - 1] = raw[j];
+                const uint32_t at = (i0 + 32 * i + lane) * kVec;
+                if (__all_sync(0xffffffffu, bits == RowView<T>::kAll)) {
+                    uint32_t t = t0 + at;
+#pragma unroll 1
+                    for (int j = 0; j < kVec; j += 2, t += 2) {
+                        float x0, x1;
+                        if constexpr (kHalf) {
+                            x0 = Pair<T>::lo(now.x), x1 = Pair<T>::hi(now.x);
+                            now.x = now.y, now.y = now.z, now.z = now.w;
+                        } else {
+                            x0 = __uint_as_float(now.x), x1 = __uint_as_float(now.y);
+                            now.x = now.z, now.y = now.w;
+                        }
+                        f(x0, t, x0 > -INFINITY);
+                        f(x1, t + 1, x1 > -INFINITY);
+                    }
+                } else if (__any_sync(0xffffffffu, bits != 0)) {
+#pragma unroll
+                    for (int j = 0; j < kVec; ++j) {
+                        const bool in = (bits >> j) & 1;
+                        const uint32_t who = __ballot_sync(0xffffffffu, in);
+                        const int to = fill + __popc(who & below);
+                        if (in) {
+                            if constexpr (kHalf) {
+                                const uint32_t w = (j >> 1) == 0 ? now.x : (j >> 1) == 1 ? now.y : (j >> 1) == 2 ? now.z : now.w;
+                                queue[to] = ptx::prmt(w, at + j, j & 1 ? 0x5432u : 0x5410u);
+                            } else {
+                                reinterpret_cast<uint2*>(queue)[to] = make_uint2(j == 0 ? now.x : j == 1 ? now.y : j == 2 ? now.z : now.w, at + j);
+                            }
+                        }
+                        fill += __popc(who);
+                    }
+                    __syncwarp();
+                }
+#pragma unroll 1
+                while (fill >= 64 || (ends && fill > 0)) {
+                    const int from = max(fill - 64, 0);
+                    pop(from + lane);
+                    pop(from + 32 + lane);
+                    fill = from;
+                    __syncwarp();
+                }
+                if (ends) break;
+            }
+        }
+    }
+    const int32_t t = v.edge(g0, g1);
+    if (__any_sync(0xffffffffu, t >= 0)) {
+        const float x = t >= 0 && v.valid(t) ? widen(v.row[t]) : -INFINITY;
+        f(x, static_cast<uint32_t>(t), x > -INFINITY);
     }
 }
 
@@ -230,80 +368,6 @@ __device__ __forceinline__ int64_t warp_sum(int64_t v) {
 #pragma unroll
     for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
     return v;
-}
-
-// Mass and count over the cluster of the tokens with key > cut_above and key >= floor_key, in a fixed order of sums.
-template <typename T>
-__device__ MassCount sum_above(cg::cluster_group& cluster, Shared& sh, const RowView<T>& v, int64_t g0, int64_t g1, double top, double inv_t,
-                               uint64_t above, uint64_t floor_key, bool weigh, int& turn) {
-    double mass = 0.0;
-    int64_t count = 0;
-    each_group(v, g0, g1, [&](int64_t t, const float(&x)[8], uint32_t b) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (!((b >> i) & 1) || !(x[i] > -INFINITY)) continue;
-            const uint64_t k = order_key(x[i], static_cast<uint32_t>(t + i));
-            if (k > above && k >= floor_key) {
-                if (weigh) mass += weight_of(x[i], top, inv_t, sh.exp_table);
-                ++count;
-            }
-        }
-    });
-    mass = warp_sum(mass);
-    count = warp_sum(count);
-    const int warp = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) sh.warp_mass[warp] = mass, sh.warp_count[warp] = count;
-    __syncthreads();
-    const int c = cluster.num_blocks(), rank = cluster.block_rank();
-    if (threadIdx.x < c) {
-        MassCount mc{0.0, 0};
-        for (int w = 0; w < kWarps; ++w) mc.mass += sh.warp_mass[w], mc.count += sh.warp_count[w];
-        *cluster.map_shared_rank(&sh.part[turn][rank], threadIdx.x) = mc;
-    }
-    cluster.sync();
-    MassCount all{0.0, 0};
-    for (int r = 0; r < c; ++r) all.mass += sh.part[turn][r].mass, all.count += sh.part[turn][r].count;
-    turn ^= 1;
-    return all;
-}
-
-// Sorts the first n (<= kCap) entries descending; entries behind n must be 0.  m: n rounded up to a power of two.
-__device__ void sort_desc(uint64_t* a, int m) {
-    for (int size = 2; size <= m; size <<= 1)
-        for (int step = size >> 1; step > 0; step >>= 1) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < m / 2; i += kThreads) {
-                const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
-                const bool down = (lo & size) == 0;
-                const uint64_t x = a[lo], y = a[hi];
-                if ((x < y) == down) a[lo] = y, a[hi] = x;
-            }
-        }
-    __syncthreads();
-}
-
-// Inclusive scan of a[0, n) in place.
-__device__ void scan_in_place(double* a, int n, Shared& sh) {
-    const int per = (n + kThreads - 1) / kThreads;
-    const int lo = min(n, static_cast<int>(threadIdx.x) * per), hi = min(n, lo + per);
-    double s = 0.0;
-    for (int i = lo; i < hi; ++i) s += a[i], a[i] = s;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    double run = s;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const double up = __shfl_up_sync(0xffffffffu, run, d);
-        if (lane >= d) run += up;
-    }
-    __syncthreads();
-    if (lane == 31) sh.warp_mass[warp] = run;
-    __syncthreads();
-    double before = 0.0;
-    for (int w = 0; w < warp; ++w) before += sh.warp_mass[w];
-    const double up = __shfl_up_sync(0xffffffffu, run, 1);
-    if (lane > 0) before += up;
-    for (int i = lo; i < hi; ++i) a[i] += before;
-    __syncthreads();
 }
 
 // Sum of the values of the threads before this one, and of all (through `all`).
@@ -328,66 +392,708 @@ __device__ V block_before(V v, V* warp_totals, V& all) {
     return before + run - v;
 }
 
-__device__ __forceinline__ int round_pow2(int n) {
-    int m = 2;
-    while (m < n) m <<= 1;
-    return m;
+// Where the shortest of the first k tokens and the nucleus ends among the list's n (<= kCap) tokens, in any order:
+// the order key of the last one kept.  `above` is the mass before the list, `rest` the mass behind it (both 0 where
+// the list is the whole row); through `kept` how many of the list's tokens the nucleus keeps, through `mass`
+// the mass of the first k.  By bisection: over the scores' order bits, 10 - 30 steps of a block-wide sum over keys in
+// registers, then, where the end falls inside a run of equal scores, over tokens.  (A bitonic sort of the list
+// took 2.5 times as long at 250 tokens, and far longer at 4,096.)
+__device__ __noinline__ uint64_t list_cut(Shared& sh, int n, int64_t k, double p, double above, double rest, int& kept, double& mass) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int rounds = (n + kThreads - 1) / kThreads;
+    uint32_t v[kWide], t[kWide];
+    double w[kWide];
+    uint32_t lo = 0xffffffffu, hi = 0;
+#pragma unroll
+    for (int r = 0; r < kWide; ++r) {
+        const int i = r * kThreads + threadIdx.x;
+        v[r] = 0, t[r] = 0xffffffffu, w[r] = 0.0;
+        if (i < n) {
+            const uint64_t key = sh.list[i];
+            v[r] = static_cast<uint32_t>(key >> 32) >> sh.shift, t[r] = 0xffffffffu - static_cast<uint32_t>(key);
+            if (p < 1.0) w[r] = weight_of(order_value(static_cast<uint32_t>(key >> 32)), sh.top, sh.rate, sh.exp_table);
+            lo = min(lo, v[r]), hi = max(hi, v[r]);
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) sh.pick = 0xffffffffu, sh.last = 0;
+    __syncthreads();
+    lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) atomicMin(&sh.pick, lo), atomicMax(&sh.last, hi);
+    __syncthreads();
+    const uint32_t lowest = sh.pick, highest = sh.last;
+    int turn = 0;
+    // Sums over the list, alternating between two sets of warp totals so that one barrier per step does.
+    auto count = [&](auto in) {
+        uint32_t c = 0;
+#pragma unroll
+        for (int r = 0; r < kWide; ++r)
+            if (r < rounds) c += in(v[r], t[r]);
+        c = __reduce_add_sync(0xffffffffu, c);
+        uint32_t* totals = reinterpret_cast<uint32_t*>(sh.step_mass[turn ^= 1]);
+        if (lane == 0) totals[warp] = c;
+        __syncthreads();
+        return __reduce_add_sync(0xffffffffu, lane < kWarps ? totals[lane] : 0u);
+    };
+    auto weigh = [&](auto in) {
+        double m = 0.0;
+#pragma unroll
+        for (int r = 0; r < kWide; ++r)
+            if (r < rounds && in(v[r], t[r])) m += w[r];
+        m = warp_sum(m);
+        double* totals = sh.step_mass[turn ^= 1];
+        if (lane == 0) totals[warp] = m;
+        __syncthreads();
+        return warp_sum(lane < kWarps ? totals[lane] : 0.0);
+    };
+    // The token of the j-th (from 1) of the equal scores x, in token order.
+    auto token_of = [&](uint32_t x, uint32_t j) {
+        uint32_t a = 0, b = 0xfffffffeu;
+        while (a < b) {
+            const uint32_t mid = a + (b - a) / 2;
+            if (count([&](uint32_t y, uint32_t s) { return y == x && s <= mid; }) >= j) b = mid;
+            else a = mid + 1;
+        }
+        return a;
+    };
+    uint32_t cut_v = 0, cut_t = 0xfffffffeu;  // entries behind the list carry token 0xffffffff
+    kept = n;
+    if (k < n) {
+        uint32_t a = lowest, b = highest;
+        while (a < b) {
+            const uint32_t mid = a + (b - a) / 2;
+            if (count([&](uint32_t y, uint32_t) { return y > mid; }) < k) b = mid;
+            else a = mid + 1;
+        }
+        cut_v = a;
+        const uint32_t need = static_cast<uint32_t>(k) - count([&](uint32_t y, uint32_t) { return y > cut_v; });
+        if (need < count([&](uint32_t y, uint32_t s) { return y == cut_v && s != 0xffffffffu; })) cut_t = token_of(cut_v, need);
+        kept = static_cast<int>(k);
+    }
+    mass = 0.0;
+    if (p < 1.0) {
+        auto first_k = [&](uint32_t y, uint32_t s) { return y > cut_v || (y == cut_v && s <= cut_t); };
+        mass = weigh(first_k);
+        const double limit = p * (above + mass + rest);
+        uint32_t a = lowest, b = highest;
+        while (a < b) {
+            const uint32_t mid = a + (b - a) / 2;
+            if (above + weigh([&](uint32_t y, uint32_t s) { return y > mid && first_k(y, s); }) < limit) b = mid;
+            else a = mid + 1;
+        }
+        const double before = above + weigh([&](uint32_t y, uint32_t s) { return y > a && first_k(y, s); });
+        const uint32_t ahead = count([&](uint32_t y, uint32_t s) { return y > a && first_k(y, s); });
+        const uint32_t ties = count([&](uint32_t y, uint32_t s) { return y == a && s != 0xffffffffu && first_k(y, s); });
+        // The j-th of the equal scores is kept iff before + (j - 1) of their weights is below the limit.
+        const double one = weight_of(order_value(sh.shift == 0 ? a : (a << sh.shift) | ((a >> (31 - sh.shift)) ? 0u : (1u << sh.shift) - 1u)), sh.top, sh.rate, sh.exp_table);
+        uint32_t j = 0;
+        for (uint32_t bit = 1u << 12; bit; bit >>= 1)
+            if (j + bit <= ties && before + (j + bit - 1) * one < limit) j += bit;
+        kept = static_cast<int>(ahead + j);
+        if (j < ties) {
+            if (j > 0) {
+                cut_t = token_of(a, j);
+                cut_v = a;
+            } else {  // not even the first: only where the limit lies in the mass above the list
+                cut_v = a + 1, cut_t = 0;
+            }
+        } else if (a > cut_v) {
+            cut_v = a, cut_t = 0xfffffffeu;
+        }
+    }
+    __syncthreads();
+    // Back to a full order key: the constant low bits are zeros for positive scores and ones for negative ones.
+    const uint32_t bits = sh.shift == 0 ? cut_v : (cut_v << sh.shift) | ((cut_v >> (31 - sh.shift)) ? 0u : (1u << sh.shift) - 1u);
+    return (static_cast<uint64_t>(bits) << 32) | (0xffffffffu - cut_t);
 }
 
-// The list path: all tokens in play are in sh.list (unsorted).  Returns through token / kept.
-__device__ void finish_list(Shared& sh, int n, double top, double inv_t, int64_t k, double p, double min_p, double u, int64_t* token,
-                            int64_t* kept_out) {
-    const int m = round_pow2(n);
-    for (int i = n + threadIdx.x; i < m; i += kThreads) sh.list[i] = 0;
-    sort_desc(sh.list, m);
-    int keep = static_cast<int>(min(static_cast<int64_t>(n), k));
-    for (int i = threadIdx.x; i < keep; i += kThreads) sh.weight[i] = weight_of(order_value(static_cast<uint32_t>(sh.list[i] >> 32)), top, inv_t, sh.exp_table);
-    __syncthreads();
-    if (threadIdx.x == 0) sh.pick = 0;
-    __syncthreads();
-    if (min_p > 0.0) {
-        uint32_t mine = 0;
-        for (int i = threadIdx.x; i < keep; i += kThreads) mine += sh.weight[i] >= min_p;
-        if (mine) atomicAdd(&sh.pick, mine);
-        __syncthreads();
+// The list path: the tokens in play are in sh.list, in token order.  Cuts, weighs and draws.
+__device__ __noinline__ void finish_list(Shared& sh, int n, int64_t* token, int64_t* kept_out) {
+    const double top = sh.top, rate = sh.rate, p = sh.top_p, u = sh.u;
+    const int64_t k = sh.k;
+    const float floor_x = sh.floor_x;
+    uint64_t cut = 0;
+    if (k < n || p < 1.0) {
+        int kept;
+        double mass;
+        cut = list_cut(sh, n, k, p, 0.0, 0.0, kept, mass);
     }
-    const int by_min = min_p > 0.0 ? static_cast<int>(sh.pick) : keep;
-    int by_p = keep;
-    if (p < 1.0) {
-        scan_in_place(sh.weight, keep, sh);
-        const double limit = p * sh.weight[keep - 1];
-        if (threadIdx.x == 0) sh.pick = 0;
-        __syncthreads();
-        uint32_t mine = 0;
-        for (int i = threadIdx.x; i < keep; i += kThreads) mine += i == 0 || sh.weight[i - 1] < limit;
-        if (mine) atomicAdd(&sh.pick, mine);
-        __syncthreads();
-        by_p = static_cast<int>(sh.pick);
-    }
-    keep = min(by_p, by_min);
-    // Token order: descending keys of the complement of the token.
-    const int mk = round_pow2(keep);
-    __syncthreads();
-    for (int i = threadIdx.x; i < mk; i += kThreads)
-        sh.list[i] = i < keep ? (sh.list[i] << 32) | (sh.list[i] >> 32) : 0;
-    sort_desc(sh.list, mk);
-    for (int i = threadIdx.x; i < keep; i += kThreads) sh.weight[i] = weight_of(order_value(static_cast<uint32_t>(sh.list[i])), top, inv_t, sh.exp_table);
-    __syncthreads();
-    scan_in_place(sh.weight, keep, sh);
-    const double total = sh.weight[keep - 1], target = u * total;
-    if (threadIdx.x == 0) sh.pick = 0xffffffffu;
-    __syncthreads();
-    // First entry whose running mass exceeds the target; after rounding, the first that reaches the total.
-    for (int i = threadIdx.x; i < keep; i += kThreads)
-        if (sh.weight[i] > target || sh.weight[i] >= total) {
-            atomicMin(&sh.pick, static_cast<uint32_t>(i));
-            break;
+    cut = max(cut, static_cast<uint64_t>(order_bits(floor_x)) << 32);
+    // Running masses in token order, consecutive tokens per thread.
+    constexpr int kPer = kWide;
+    const int per = (n + kThreads - 1) / kThreads, first = threadIdx.x * per;
+    double w[kPer], sum = 0.0;
+    int count = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        w[j] = 0.0;
+        if (j < per && first + j < n) {
+            const uint64_t key = sh.list[first + j];
+            if (key >= cut) w[j] = weight_of(order_value(static_cast<uint32_t>(key >> 32)), top, rate, sh.exp_table), ++count;
+            sum += w[j];
         }
+    }
+    double total;
+    double run = block_before(sum, sh.warp_mass, total);
+    const double target = u * total;
+    int kept;
+    block_before(count, reinterpret_cast<int*>(sh.warp_count), kept);
+    if (threadIdx.x == 0) sh.pick = 0xffffffffu, sh.last = 0;
+    __syncthreads();
+    // The first token whose running mass exceeds the target; without one (rounding at the very end) the last with mass.
+    int hit = -1, last = -1;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        run += w[j];
+        if (w[j] > 0.0) {
+            last = first + j;
+            if (hit < 0 && run > target) hit = first + j;
+        }
+    }
+    if (hit >= 0) atomicMin(&sh.pick, static_cast<uint32_t>(hit));
+    if (last >= 0) atomicMax(&sh.last, static_cast<uint32_t>(last));
     __syncthreads();
     if (threadIdx.x == 0) {
-        *token = 0xffffffffu - static_cast<uint32_t>(sh.list[sh.pick] >> 32);
-        *kept_out = keep;
+        *token = 0xffffffffu - static_cast<uint32_t>(sh.list[sh.pick != 0xffffffffu ? sh.pick : sh.last]);
+        *kept_out = kept;
     }
+}
+
+// A score's bin: one rounding, so higher scores never lie in later bins.
+__device__ __forceinline__ int bin_of(float x, float at, float scale) { return static_cast<int>(fminf(fmaxf(fmaf(x, -scale, at), 0.f), kBins - 1.f)); }
+
+// The passes below are functions of their own, with the row's state in shared memory: inlined together they would
+// share one register budget (64, for two CTAs of 512 per SM) and spill in their loops.
+
+// Mass (0 unless `weigh`) and count over the cluster of the tokens with key > above and key >= floor_key, summed in a fixed order.
+template <typename T>
+__device__ __noinline__ MassCount sum_above(Shared& sh, const RowView<T>& shared_view, uint32_t* queue, uint64_t above, uint64_t floor_key, bool weigh, int& turn) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const RowView<T> view = shared_view;
+    const int c = cluster.num_blocks(), rank = cluster.block_rank(), warp = threadIdx.x >> 5;
+    double mass = 0.0;
+    int64_t count = 0;
+    each_token(view, sh.bounds[warp], sh.bounds[warp + 1], queue, [&](float x, uint32_t t, bool live) {
+        const uint64_t k = order_key(x, t);
+        if (live && k > above && k >= floor_key) {
+            if (weigh) mass += weight_of(x, sh.top, sh.rate, sh.exp_table);
+            ++count;
+        }
+    });
+    mass = warp_sum(mass);
+    count = warp_sum(count);
+    if ((threadIdx.x & 31) == 0) sh.warp_mass[warp] = mass, sh.warp_count[warp] = count;
+    __syncthreads();
+    if (threadIdx.x < c) {
+        MassCount mc{0.0, 0};
+        for (int w = 0; w < kWarps; ++w) mc.mass += sh.warp_mass[w], mc.count += sh.warp_count[w];
+        *cluster.map_shared_rank(&sh.part[turn][rank], threadIdx.x) = mc;
+    }
+    cluster.sync();
+    MassCount all{0.0, 0};
+    for (int r = 0; r < c; ++r) all.mass += sh.part[turn][r].mass, all.count += sh.part[turn][r].count;
+    turn ^= 1;
+    return all;
+}
+
+// The smallest order key whose preceding count (weigh: mass) is below the limit, by bisection from `lo`.
+template <typename T>
+__device__ __noinline__ uint64_t bisect(Shared& sh, const RowView<T>& view, uint32_t* queue, uint64_t lo, double limit, bool weigh, int& turn) {
+    uint64_t hi = ~0ull;
+    while (lo < hi) {
+        const uint64_t mid = lo + (hi - lo) / 2;
+        const MassCount mc = sum_above(sh, view, queue, mid, 0, weigh, turn);
+        if ((weigh ? mc.mass : static_cast<double>(mc.count)) < limit) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+// The first pass: statistics of the row over the cluster.
+template <typename T>
+__device__ __noinline__ RowStats first_pass(Shared& sh, const RowView<T>& shared_view) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const RowView<T> view = shared_view;
+    const int c = cluster.num_blocks(), rank = cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int32_t g0 = sh.bounds[warp], g1 = sh.bounds[warp + 1];
+    constexpr int kVec = RowView<T>::kVec;
+    RowStats st{-INFINITY, {}, 0, 0};
+    {
+        uint32_t valid = 0, nan2 = Pair<T>::kInf ^ 0x80008000u, max2 = nan2, min2 = Pair<T>::kInf;
+        float nan1 = -INFINITY, min1 = INFINITY;
+        constexpr int kBatch = 6;
+        const int32_t z = min(g1, view.full1);
+        for (int32_t g = max(g0, view.full0) + lane; g < z; g += 32 * kBatch) {
+            uint32_t b[kBatch];
+            uint4 raw[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+                if (g + 32 * i < z) raw[i] = view.fetch(g + 32 * i);
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) b[i] = g + 32 * i < z ? view.bits(g + 32 * i) : 0u;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                if (g + 32 * i >= z) break;
+                valid += __popc(b[i]);
+                if constexpr (sizeof(T) == 2) {  // two tokens per instruction; hidden ones become -inf (for the minimum +inf)
+                    const uint32_t lo = (b[i] & 0xfu) * 0x10204080u, hi = (b[i] >> 4) * 0x10204080u;
+                    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t keep = ptx::prmt(j < 2 ? lo : hi, 0u, j & 1 ? 0xBBAAu : 0x9988u);
+                        nan2 = Pair<T>::max_nan(nan2, w[j]);
+                        max2 = Pair<T>::max(max2, ptx::select_bits(w[j], keep, Pair<T>::kInf ^ 0x80008000u));
+                        min2 = Pair<T>::min(min2, ptx::select_bits(w[j], keep, Pair<T>::kInf));
+                    }
+                } else {
+                    float x[kVec];
+                    view.expand(raw[i], x);
+#pragma unroll
+                    for (int j = 0; j < kVec; ++j) {
+                        const bool in = (b[i] >> j) & 1;
+                        nan1 = ptx::max_nan(nan1, x[j]);
+                        st.max = fmaxf(st.max, in ? x[j] : -INFINITY);
+                        min1 = fminf(min1, in ? x[j] : INFINITY);
+                    }
+                }
+            }
+        }
+        if constexpr (sizeof(T) == 2) {
+            st.max = fmaxf(Pair<T>::lo(max2), Pair<T>::hi(max2));
+            min1 = fminf(Pair<T>::lo(min2), Pair<T>::hi(min2));
+            nan1 = ptx::max_nan(Pair<T>::lo(nan2), Pair<T>::hi(nan2));
+        }
+        const int32_t t = view.edge(g0, g1);
+        if (t >= 0) {
+            const float x = widen(view.row[t]);
+            nan1 = ptx::max_nan(nan1, x);
+            if (view.valid(t)) st.max = fmaxf(st.max, x), min1 = fminf(min1, x), ++valid;
+        }
+        st.finite = valid;
+        st.flags = (nan1 != nan1 ? 1u : 0u) | (valid ? 2u : 0u) | (min1 == -INFINITY ? 4u : 0u);
+        float m = st.max;
+        st.low[2] = m;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+            if (d == 4) st.low[1] = m;
+        }
+        st.low[0] = st.max = m;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            st.low[1] = fminf(st.low[1], __shfl_xor_sync(0xffffffffu, st.low[1], d));
+            st.low[2] = fminf(st.low[2], __shfl_xor_sync(0xffffffffu, st.low[2], d));
+            st.finite += __shfl_xor_sync(0xffffffffu, st.finite, d);
+            st.flags |= __shfl_xor_sync(0xffffffffu, st.flags, d);
+        }
+    }
+    RowStats* warp_stats = sh.warp_stats;
+    if (lane == 0) warp_stats[warp] = st;
+    if (threadIdx.x == 0) sh.list_count = 0;
+    __syncthreads();
+    if (threadIdx.x < c) {
+        RowStats a = warp_stats[0];
+        for (int w = 1; w < kWarps; ++w) merge(a, warp_stats[w]);
+        *cluster.map_shared_rank(&sh.stats[rank], threadIdx.x) = a;
+    }
+    cluster.sync();
+    st = sh.stats[0];
+    for (int i = 1; i < c; ++i) merge(st, sh.stats[i]);
+    return st;
+}
+
+// Collects the keys of the tokens with x >= low into rank 0's list, in token order; returns their number in the whole
+// row, or more than kCap where a warp's segment or the list overflowed.
+template <typename T>
+__device__ __noinline__ uint32_t collect(Shared& sh, const RowView<T>& shared_view, float low) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const RowView<T> view = shared_view;
+    const int c = cluster.num_blocks(), rank = cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int32_t g0 = sh.bounds[warp], g1 = sh.bounds[warp + 1];
+    constexpr int kVec = RowView<T>::kVec, kBatch = 6;
+    const uint32_t below = (1u << lane) - 1u;
+    uint32_t fill = 0;
+    uint64_t* segment = sh.segment[warp];
+    auto append = [&](uint32_t in, int32_t t, const float (&x)[kVec]) {  // this lane's consecutive tokens
+        uint32_t at = __popc(in), run = at;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t up = __shfl_up_sync(0xffffffffu, run, d);
+            if (lane >= d) run += up;
+        }
+        at = fill + run - at;
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+            if ((in >> j) & 1) {
+                if (at < kSegment) segment[at] = order_key(x[j], static_cast<uint32_t>(t + j));
+                ++at;
+            }
+        fill += __shfl_sync(0xffffffffu, run, 31);
+    };
+    auto edge = [&](bool front) {
+        const int32_t t = view.edge(g0, g1);
+        const float x = t >= 0 && (lane < kVec) == front && view.valid(t) ? widen(view.row[t]) : -INFINITY;
+        const bool in = x >= low;
+        const uint32_t who = __ballot_sync(0xffffffffu, in);
+        const uint32_t at = fill + __popc(who & below);
+        if (in && at < kSegment) segment[at] = order_key(x, static_cast<uint32_t>(t));
+        fill += __popc(who);
+    };
+    __syncthreads();  // the segments' space had other uses
+    edge(true);
+    const int32_t z = min(g1, view.full1);
+    for (int32_t g = max(g0, view.full0); g < z; g += 32 * kBatch) {
+        uint32_t b[kBatch];
+        uint4 raw[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) b[i] = g + 32 * i + lane < z ? view.bits(g + 32 * i + lane) : 0u;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (b[i]) raw[i] = view.fetch(g + 32 * i + lane);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            float x[kVec];
+            uint32_t in = 0;
+            if (b[i]) {
+                view.expand(raw[i], x);
+                float m = x[0];
+#pragma unroll
+                for (int j = 1; j < kVec; ++j) m = fmaxf(m, x[j]);
+                if (m >= low) {
+#pragma unroll
+                    for (int j = 0; j < kVec; ++j) in |= static_cast<uint32_t>(x[j] >= low) << j;
+                    in &= b[i];
+                }
+            }
+            if (__any_sync(0xffffffffu, in != 0)) append(in, view.first(g + 32 * i + lane), x);
+        }
+    }
+    edge(false);
+    const uint32_t reported = fill <= kSegment ? fill : kCap + 1;
+    if (lane < c) *cluster.map_shared_rank(&sh.warp_counts[rank * kWarps + warp], lane) = reported;
+    cluster.sync();
+    uint32_t before = 0, all = 0;
+    for (int i = lane; i < c * kWarps; i += 32) {
+        const uint32_t n = sh.warp_counts[i];
+        all += n;
+        if (i < rank * kWarps + warp) before += n;
+    }
+    before = __reduce_add_sync(0xffffffffu, before);
+    all = __reduce_add_sync(0xffffffffu, all);
+    if (all <= kCap) {
+        uint64_t* dst = cluster.map_shared_rank(sh.list, 0) + before;
+        for (uint32_t i = lane; i < fill; i += 32) dst[i] = segment[i];
+    }
+    cluster.sync();
+    return all;
+}
+
+// Counts of the tokens up to sh.first_k by value bins of width sh.width below the maximum, in sh.merged (a token further
+// down is in the last bin), the same in every CTA.
+template <typename T>
+__device__ __noinline__ void count_bins(Shared& sh, const RowView<T>& shared_view, uint32_t* queue) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const RowView<T> view = shared_view;
+    const int c = cluster.num_blocks(), warp = threadIdx.x >> 5;
+    const Place end = place_of(sh.first_k);
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.bins[i] = 0;
+    __syncthreads();
+    const float at = sh.bin_at, scale = sh.bin_scale;
+    each_token(view, sh.bounds[warp], sh.bounds[warp + 1], queue, [&](float x, uint32_t t, bool live) {
+        if (live && end.keeps(x, t)) atomicAdd(&sh.bins[bin_of(x, at, scale)], 1u);
+    });
+    cluster.sync();
+    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+        uint32_t n = 0;
+        for (int q = 0; q < c; ++q) n += cluster.map_shared_rank(sh.bins, q)[i];
+        sh.merged[i] = n;
+    }
+    cluster.sync();
+}
+
+// Moves every CTA's sh.list (sh.list_count keys, in no order) behind rank 0's; returns their number.
+__device__ __noinline__ uint32_t pool(Shared& sh) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const int c = cluster.num_blocks(), rank = cluster.block_rank();
+    __syncthreads();
+    if (threadIdx.x < c) *cluster.map_shared_rank(&sh.list_counts[rank], threadIdx.x) = sh.list_count;
+    cluster.sync();
+    uint32_t before = 0, all = 0;
+    for (int i = 0; i < c; ++i) {
+        if (i < rank) before += sh.list_counts[i];
+        all += sh.list_counts[i];
+    }
+    if (rank != 0) {
+        uint64_t* dst = cluster.map_shared_rank(sh.list, 0) + before;
+        for (uint32_t i = threadIdx.x; i < sh.list_count; i += kThreads) dst[i] = sh.list[i];
+    }
+    cluster.sync();
+    return all;
+}
+
+// The keys of bin b's tokens into sh.list (no order).
+template <typename T>
+__device__ __noinline__ void collect_bin(Shared& sh, const RowView<T>& shared_view, uint32_t* queue, int b) {
+    const RowView<T> view = shared_view;
+    const int warp = threadIdx.x >> 5;
+    __syncthreads();
+    if (threadIdx.x == 0) sh.list_count = 0;
+    __syncthreads();
+    const float at = sh.bin_at, scale = sh.bin_scale;
+    each_token(view, sh.bounds[warp], sh.bounds[warp + 1], queue, [&](float x, uint32_t t, bool live) {
+        if (live && bin_of(x, at, scale) == b) sh.list[atomicAdd(&sh.list_count, 1u)] = order_key(x, t);
+    });
+}
+
+// The weighing pass around the bracket [sh.b0, sh.b1] of bins, among the tokens up to sh.first_k: masses above and below
+// it and the number of kept tokens above it to rank 0 (sh.above, sh.below, sh.counts, sh.spans), the bracket's keys
+// into sh.list.
+template <typename T>
+__device__ __noinline__ void weigh_bracket(Shared& sh, const RowView<T>& shared_view, uint32_t* queue) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const RowView<T> view = shared_view;
+    const int rank = cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const Place end = place_of(sh.first_k);
+    const double top = sh.top, rate = sh.rate;
+    const int b0 = sh.b0, b1 = sh.b1;
+    const float at = sh.bin_at, scale = sh.bin_scale, floor_x = sh.floor_x;
+    double above = 0.0, below = 0.0, kept_above = 0.0;
+    int count = 0;
+    each_token(view, sh.bounds[warp], sh.bounds[warp + 1], queue, [&](float x, uint32_t t, bool live) {
+        if (!live || !end.keeps(x, t)) return;
+        const int bin = bin_of(x, at, scale);
+        if (bin >= b0 && bin <= b1) {
+            sh.list[atomicAdd(&sh.list_count, 1u)] = order_key(x, t);
+            return;
+        }
+        const double w = weight_of(x, top, rate, sh.exp_table);
+        if (bin > b1) below += w;
+        else above += w;
+        if (bin < b0 && x >= floor_x) kept_above += w, ++count;
+    });
+    above = warp_sum(above), below = warp_sum(below), kept_above = warp_sum(kept_above);
+    count = __reduce_add_sync(0xffffffffu, count);
+    if (lane == 0) {
+        sh.warp_mass[warp] = above, sh.warp_below[warp] = below, sh.warp_count[warp] = count;
+        *cluster.map_shared_rank(&sh.spans[rank * kWarps + warp], 0) = kept_above;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double a = 0.0, b = 0.0;
+        int64_t n = 0;
+        for (int w = 0; w < kWarps; ++w) a += sh.warp_mass[w], b += sh.warp_below[w], n += sh.warp_count[w];
+        *cluster.map_shared_rank(&sh.above[rank], 0) = a;
+        *cluster.map_shared_rank(&sh.below[rank], 0) = b;
+        *cluster.map_shared_rank(&sh.counts[rank], 0) = n;
+    }
+}
+
+// Mass of the tokens up to `end` by spans, and their number, to rank 0.
+template <typename T>
+__device__ __noinline__ void weigh_spans(Shared& sh, const RowView<T>& shared_view, uint32_t* queue, Place end) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const RowView<T> view = shared_view;
+    const int rank = cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const double top = sh.top, rate = sh.rate;
+    double mass = 0.0;
+    int count = 0;
+    each_token(view, sh.bounds[warp], sh.bounds[warp + 1], queue, [&](float x, uint32_t t, bool live) {
+        if (live && end.keeps(x, t)) mass += weight_of(x, top, rate, sh.exp_table), ++count;
+    });
+    mass = warp_sum(mass);
+    count = __reduce_add_sync(0xffffffffu, count);
+    __syncthreads();
+    if (lane == 0) {
+        sh.warp_count[warp] = count;
+        *cluster.map_shared_rank(&sh.spans[rank * kWarps + warp], 0) = mass;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int64_t all = 0;
+        for (int w = 0; w < kWarps; ++w) all += sh.warp_count[w];
+        *cluster.map_shared_rank(&sh.counts[rank], 0) = all;
+    }
+    cluster.sync();
+}
+
+// The nucleus: the place where it ends in sh.cut and the kept masses by spans on rank 0, or false where the estimate
+// or the list does not serve.
+template <typename T>
+__device__ __noinline__ bool find_nucleus(Shared& sh, const RowView<T>& shared_view, uint32_t* queue, int64_t* kept_out, int32_t* status_out) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const int c = cluster.num_blocks(), rank = cluster.block_rank(), lane = threadIdx.x & 31;
+    const int64_t groups = shared_view.groups;
+    // Where the nucleus ends, by the bins' counts and middle weights.  The estimate is good to about a part
+    // in a thousand of the mass; a miss tells the exact masses around the bracket, which place the next one.
+    count_bins<T>(sh, shared_view, queue);
+    const float step = sh.width * static_cast<float>(sh.rate / kTable);  // log2 of the weights' ratio from bin to bin
+    float mine = 0.f, all;
+    for (int i = 0; i < kPerThread; ++i) {
+        const int at = threadIdx.x * kPerThread + i;
+        mine += sh.merged[at] * exp2f(-(at + 0.5f) * step);
+    }
+    const float run = block_before(mine, reinterpret_cast<float*>(sh.warp_mass), all);
+    float goal = static_cast<float>(sh.top_p) * all, slack = 1e-3f;
+    bool found = false;
+    for (int attempt = 0; attempt < 3 && !found; ++attempt, slack = 2e-4f) {
+        __syncthreads();
+        if (threadIdx.x == 0) sh.bin[0] = 0, sh.bin[1] = sh.bin[2] = kBins - 1, sh.bin_count = 0, sh.list_count = 0;
+        __syncthreads();
+#pragma unroll 1
+        for (int side = 0; side < 3; ++side) {
+            const float want = side == 0 ? goal - slack * all : side == 1 ? goal + slack * all : goal;
+            if (run < want && want <= run + mine) {
+                float before = run;
+                int i = threadIdx.x * kPerThread;
+                for (const int last = i + kPerThread - 1; i < last; ++i) {
+                    const float m = sh.merged[i] * exp2f(-(i + 0.5f) * step);
+                    if (before + m >= want) break;
+                    before += m;
+                }
+                sh.bin[side] = i;
+            }
+        }
+        __syncthreads();
+        int b0 = max(sh.bin[0] - 1, 0), b1 = min(sh.bin[1] + 1, kBins - 1);
+        uint32_t inside = 0;
+        for (int i = b0 + threadIdx.x; i <= b1; i += kThreads) inside += sh.merged[i];
+        inside = __reduce_add_sync(0xffffffffu, inside);
+        if (lane == 0) atomicAdd(&sh.bin_count, inside);
+        __syncthreads();
+        inside = sh.bin_count;
+        if (inside > kCap) b0 = b1 = sh.bin[2], inside = sh.merged[b0];
+        if (inside > kCap || inside == 0) break;
+        if (threadIdx.x == 0) sh.b0 = b0, sh.b1 = b1;
+        __syncthreads();
+        weigh_bracket<T>(sh, shared_view, queue);
+        const uint32_t n = pool(sh);
+        if (rank == 0) {
+            double above = 0.0, below = 0.0;
+            for (int i = 0; i < c; ++i) above += sh.above[i], below += sh.below[i];
+            int kept;
+            double mass;
+            const uint64_t key = list_cut(sh, static_cast<int>(n), n, sh.top_p, above, below, kept, mass);
+        const double limit = sh.top_p * (above + mass + below);
+            // Outside the bracket: not one of its tokens kept, or all of them with more below.
+            const bool ends_inside = kept > 0 && (above + mass >= limit || b1 == kBins - 1);
+            if (ends_inside) {
+                // The bracket's kept tokens join their spans as integers: the order of the additions does not matter.
+                    for (int i = threadIdx.x; i < c * kWarps; i += kThreads) sh.extra[i] = 0;
+                if (threadIdx.x == 0) sh.passed = 0;
+                __syncthreads();
+                uint32_t passed = 0;
+                for (int i = threadIdx.x; i < n; i += kThreads) {
+                const Place at = place_of(sh.list[i]);
+                if (sh.list[i] < key || at.x < sh.floor_x) continue;
+                ++passed;
+                    const int64_t g = (static_cast<int64_t>(at.t) + shared_view.skew) / RowView<T>::kVec;
+                    int q = static_cast<int>(g * c / groups);  // the CTA whose slice [groups q / c, groups (q + 1) / c) holds g
+                    while (g >= groups * (q + 1) / c) ++q;
+                    while (g < groups * q / c) --q;
+                    const int64_t from = groups * q / c, len = groups * (q + 1) / c - from;
+                    int w = static_cast<int>((g - from) * kWarps / len);
+                    while (g >= from + len * (w + 1) / kWarps) ++w;
+                    while (g < from + len * w / kWarps) --w;
+                    atomicAdd(&sh.extra[q * kWarps + w], static_cast<unsigned long long>(weight_of(at.x, sh.top, sh.rate, sh.exp_table) * 0x1p50));
+                }
+                if (passed) atomicAdd(&sh.passed, passed);
+                __syncthreads();
+                for (int i = threadIdx.x; i < c * kWarps; i += kThreads) sh.spans[i] += sh.extra[i] * 0x1p-50;
+                if (threadIdx.x == 0) {
+                    int64_t all_count = sh.passed;
+                    for (int i = 0; i < c; ++i) all_count += sh.counts[i];
+                    *kept_out = all_count;
+                    *status_out = BMS_STATUS_OK;
+                }
+            }
+            if (threadIdx.x < c) {
+                *cluster.map_shared_rank(&sh.cut, threadIdx.x) = key;
+                *cluster.map_shared_rank(&sh.found, threadIdx.x) = ends_inside;
+                // How far the end lies before the bracket (negative) or behind it.
+                *cluster.map_shared_rank(&sh.goal, threadIdx.x) = static_cast<float>(kept == 0 ? limit - above : limit - above - mass);
+            }
+        }
+        cluster.sync();
+        found = sh.found;
+        if (!found) {  // the same correction from the estimated mass at the bracket's edge
+            const float off = sh.goal;
+            __syncthreads();
+            const int edge = off <= 0.f ? b0 : b1 + 1;
+            if (edge / kPerThread == threadIdx.x) {
+                float e = run;
+                for (int i = threadIdx.x * kPerThread; i < edge; ++i) e += sh.merged[i] * exp2f(-(i + 0.5f) * step);
+                sh.goal = e + off;
+            }
+            __syncthreads();
+            goal = sh.goal;
+        }
+    }
+    return found;
+}
+
+// The lowest valid token with the score, through rank 0's sh.pick.
+template <typename T>
+__device__ __noinline__ uint32_t lowest_at(Shared& sh, const RowView<T>& shared_view, float score) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const RowView<T> view = shared_view;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int32_t g0 = sh.bounds[warp], g1 = sh.bounds[warp + 1];
+    constexpr int kVec = RowView<T>::kVec;
+    if (threadIdx.x == 0) sh.pick = 0xffffffffu;
+    cluster.sync();
+    uint32_t best = 0xffffffffu;
+    for (int32_t g = max(g0, view.full0) + lane; g < min(g1, view.full1) && best == 0xffffffffu; g += 32) {
+        const uint32_t b = view.bits(g);
+        if (b == 0) continue;
+        float x[kVec];
+        view.expand(view.fetch(g), x);
+#pragma unroll
+        for (int i = kVec - 1; i >= 0; --i)
+            if (((b >> i) & 1) && x[i] == score) best = static_cast<uint32_t>(view.first(g) + i);
+    }
+    const int32_t t = view.edge(g0, g1);
+    if (t >= 0 && view.valid(t) && widen(view.row[t]) == score) best = min(best, static_cast<uint32_t>(t));
+    best = __reduce_min_sync(0xffffffffu, best);
+    if (lane == 0 && best != 0xffffffffu) atomicMin(cluster.map_shared_rank(&sh.pick, 0), best);
+    cluster.sync();
+    return sh.pick;
+}
+
+// Walks the span that holds the target, one token per thread and round, to the drawn token (sh.token).
+template <typename T>
+__device__ __noinline__ void walk_span(Shared& sh, const RowView<T>& shared_view, int span, Place end) {
+    const RowView<T> view = shared_view;
+    const double target = sh.target;
+    double before = sh.before;
+    const int32_t s0 = max(view.first(sh.bounds[span]), 0);
+    const int32_t s1 = static_cast<int32_t>(min(static_cast<int64_t>(view.vocab), static_cast<int64_t>(sh.bounds[span + 1]) * RowView<T>::kVec - view.skew));
+    if (threadIdx.x == 0) sh.token = -1;
+    for (int32_t base = s0; base < s1; base += kThreads) {
+        const int32_t t = base + threadIdx.x;
+        double w = 0.0;
+        if (t < s1 && view.valid(t)) {
+            const float x = widen(view.row[t]);
+            if (x > -INFINITY && end.keeps(x, static_cast<uint32_t>(t))) w = weight_of(x, sh.top, sh.rate, sh.exp_table);
+        }
+        double all;
+        const double run = before + block_before(w, sh.warp_mass, all) + w;
+        // The first token that crosses the target; without one (rounding at the very end) the last one with mass.
+        if (threadIdx.x == 0) sh.pick = 0xffffffffu, sh.last = 0;
+        __syncthreads();
+        if (w > 0.0) {
+            if (run > target) atomicMin(&sh.pick, threadIdx.x);
+            atomicMax(&sh.last, threadIdx.x + 1);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            if (sh.pick != 0xffffffffu) sh.token = base + static_cast<int32_t>(sh.pick);
+            else if (sh.last) sh.token = base + static_cast<int32_t>(sh.last) - 1;
+        }
+        if (sh.pick != 0xffffffffu) break;
+        before += all;
+    }
+    __syncthreads();
 }
 
 template <typename T>
@@ -419,71 +1125,22 @@ __global__ void __launch_bounds__(kThreads, 2) filter_sample_kernel(const Filter
         if (rank == 0 && threadIdx.x == 0) finish(-1, 0, code);
         return;
     }
-    const T* row = static_cast<const T*>(p.logits) + r * p.vocab;
-    const RowView<T> view{row, p.masks ? p.masks + mrow * p.words : nullptr, p.vocab,
-                          static_cast<int32_t>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T))};
-    const int64_t groups = view.groups();
-    const int64_t c0 = groups * rank / c, c1 = groups * (rank + 1) / c;
-    const int64_t g0 = c0 + (c1 - c0) * warp / kWarps, g1 = c0 + (c1 - c0) * (warp + 1) / kWarps;
-
-    if (threadIdx.x < 64) sh.exp_table[threadIdx.x] = exp2(threadIdx.x / 64.0);
-
-    // Pass 1: maximum and count of valid finite tokens, NaN anywhere.
-    RowStats st{-INFINITY, {}, 0, 0};
-    {
-        constexpr int kBatch = sizeof(T) == 4 ? 2 : 4;
-        for (int64_t g = g0 + lane; g < g1; g += 32 * kBatch) {
-            uint32_t b[kBatch];
-            typename RowView<T>::Raw raw[kBatch];
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i)
-                if (g + 32 * i < g1) raw[i] = view.fetch(g + 32 * i);
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) b[i] = g + 32 * i < g1 ? view.bits(g + 32 * i) : 0u;
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                if (g + 32 * i >= g1) break;
-                float x[8];
-                view.expand(raw[i], x);
-                if (b[i]) st.flags |= 2;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    if (x[j] != x[j]) st.flags |= 1;
-                    const float xv = (b[i] >> j) & 1 ? x[j] : -INFINITY;
-                    st.max = fmaxf(st.max, xv);
-                    st.finite += xv > -INFINITY;
-                }
-            }
-        }
-        float m = st.max;
-        st.low[2] = m;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-            if (d == 4) st.low[1] = m;
-        }
-        st.low[0] = st.max = m;
-#pragma unroll
-        for (int d = 16; d; d >>= 1) {
-            st.low[1] = fminf(st.low[1], __shfl_xor_sync(0xffffffffu, st.low[1], d));
-            st.low[2] = fminf(st.low[2], __shfl_xor_sync(0xffffffffu, st.low[2], d));
-            st.finite += __shfl_xor_sync(0xffffffffu, st.finite, d);
-            st.flags |= __shfl_xor_sync(0xffffffffu, st.flags, d);
-        }
+    RowView<T>& view = *reinterpret_cast<RowView<T>*>(sh.view);
+    static_assert(sizeof(RowView<T>) <= sizeof sh.view, "space of the view");
+    if (threadIdx.x == 0) {
+        view = RowView<T>(static_cast<const T*>(p.logits) + r * p.vocab, p.masks ? p.masks + mrow * p.words : nullptr, p.vocab);
+        const int64_t g = view.groups, c0 = g * rank / c, slice = g * (rank + 1) / c - c0;
+        for (int w = 0; w <= kWarps; ++w) sh.bounds[w] = static_cast<int32_t>(c0 + slice * w / kWarps);
     }
-    RowStats* warp_stats = reinterpret_cast<RowStats*>(sh.weight);
-    if (lane == 0) warp_stats[warp] = st;
-    if (threadIdx.x == 0) sh.list_count = 0;
+    uint32_t* queue = sh.queue[warp];
+    static_assert(2 * kQueue<float> >= kQueue<__half>, "queue space");
     __syncthreads();
-    if (threadIdx.x < c) {
-        RowStats a = warp_stats[0];
-        for (int w = 1; w < kWarps; ++w) merge(a, warp_stats[w]);
-        *cluster.map_shared_rank(&sh.stats[rank], threadIdx.x) = a;
-    }
-    cluster.sync();
-    st = sh.stats[0];
-    for (int i = 1; i < c; ++i) merge(st, sh.stats[i]);
+
+    RowStats st = first_pass<T>(sh, view);
     const bool greedy = temp == 0.0;
+    int turn = 0;
+    if (!greedy && (st.flags & 5) == 4)  // scores of -inf are valid but never drawn: count the others
+        st.finite = static_cast<uint32_t>(sum_above<T>(sh, view, queue, 0, 0, false, turn).count);
     if (st.flags & 1) code = BMS_STATUS_NAN;
     else if (!greedy && st.max == INFINITY) code = BMS_STATUS_POS_INF;
     else if (!(st.flags & 2)) code = BMS_STATUS_EMPTY;
@@ -493,114 +1150,60 @@ __global__ void __launch_bounds__(kThreads, 2) filter_sample_kernel(const Filter
         if (rank == 0 && threadIdx.x == 0) finish(-1, 0, code);
         return;  // nothing remote is outstanding: the statistics arrived before the barrier
     }
-    const float topf = st.max;
-    const double top = topf;
-    int turn = 0;
-
-    if (greedy) {  // lowest valid token that holds the maximum
-        if (threadIdx.x == 0) sh.pick = 0xffffffffu;
-        cluster.sync();
-        uint32_t best = 0xffffffffu;
-        for (int64_t g = g0 + lane; g < g1 && best == 0xffffffffu; g += 32) {
-            const uint32_t b = view.bits(g);
-            if (b == 0) continue;
-            float x[8];
-            view.load(g, x);
-#pragma unroll
-            for (int i = 7; i >= 0; --i)
-                if (((b >> i) & 1) && x[i] == topf) best = static_cast<uint32_t>(view.first(g) + i);
-        }
-        best = __reduce_min_sync(0xffffffffu, best);
-        if (lane == 0 && best != 0xffffffffu) atomicMin(cluster.map_shared_rank(&sh.pick, 0), best);
-        cluster.sync();
-        if (rank == 0 && threadIdx.x == 0) finish(sh.pick, 1, BMS_STATUS_OK);
+    if (greedy) {
+        const uint32_t token = lowest_at<T>(sh, view, st.max);
+        if (rank == 0 && threadIdx.x == 0) finish(token, 1, BMS_STATUS_OK);
         return;
     }
-
-    const double inv_t = fmin(1.0 / temp, DBL_MAX);
     const int64_t k = top_k > 0 ? min(top_k, static_cast<int64_t>(st.finite)) : st.finite;
     const bool k_cuts = k < st.finite;
-
-    // Collects the keys of the finite tokens that `in(x)` accepts into rank 0's list; returns their number in the whole row
-    // (above kCap: the list is not complete).
-    auto collect = [&](auto in) -> uint32_t {
-        __syncthreads();
-        if (threadIdx.x == 0) sh.list_count = 0;
-        __syncthreads();
-        each_group(view, g0, g1, [&](int64_t t, const float(&x)[8], uint32_t b) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (((b >> i) & 1) && x[i] > -INFINITY && in(x[i])) {
-                    const uint32_t at = atomicAdd(&sh.list_count, 1u);
-                    if (at < kCap) sh.list[at] = order_key(x[i], static_cast<uint32_t>(t + i));
-                }
-        });
-        __syncthreads();
-        if (c == 1) return sh.list_count;
-        if (threadIdx.x < c) *cluster.map_shared_rank(&sh.list_counts[rank], threadIdx.x) = sh.list_count;
-        cluster.sync();
-        uint32_t before = 0, all = 0;
-        for (int i = 0; i < c; ++i) {
-            if (i < rank) before += sh.list_counts[i];
-            all += sh.list_counts[i];
+    static_assert(kTable == kThreads, "an entry per thread");
+    sh.exp_table[threadIdx.x] = exp2(threadIdx.x / static_cast<double>(kTable));
+    if (threadIdx.x == 64) {
+        sh.topf = st.max, sh.top = st.max;
+        sh.top_p = top_p, sh.u = u, sh.k = k;
+        sh.rate = fmin(kTable / 0.69314718055994530942 / temp, DBL_MAX);
+        sh.width = static_cast<float>(fmin(40.0 * temp, 1e30)) / kBins;  // 40 T below the maximum weighs 4e-18
+        sh.bin_scale = 1.0f / sh.width;
+        sh.bin_at = sh.topf * sh.bin_scale;
+        sh.shift = sizeof(T) == 4 ? 0 : std::is_same_v<T, __half> ? 13 : 16;
+        sh.first_k = static_cast<uint64_t>(order_bits(-INFINITY)) << 32;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        // min-p as a score: the lowest float whose weight reaches it (weights grow with the score), by a 33-way search.
+        uint32_t lo = order_bits(-FLT_MAX), hi = order_bits(st.max);
+        while (min_p > 0.0 && lo < hi) {
+            const uint32_t at = lo + static_cast<uint32_t>((static_cast<uint64_t>(hi - lo) * (lane + 1)) / 33);
+            const uint32_t reach = __ballot_sync(0xffffffffu, weight_of(order_value(at), sh.top, sh.rate, sh.exp_table) >= min_p);
+            const int first = reach ? __ffs(reach) - 1 : 32;
+            const uint32_t base = lo, width = hi - lo;
+            if (first < 32) hi = base + static_cast<uint32_t>((static_cast<uint64_t>(width) * (first + 1)) / 33);
+            if (first > 0) lo = base + static_cast<uint32_t>((static_cast<uint64_t>(width) * first) / 33) + 1;
         }
-        if (all <= kCap && rank != 0) {
-            uint64_t* dst = cluster.map_shared_rank(sh.list, 0) + before;
-            for (uint32_t i = threadIdx.x; i < sh.list_count; i += kThreads) dst[i] = sh.list[i];
-        }
-        cluster.sync();
-        return all;
-    };
+        if (lane == 0) sh.floor_x = min_p > 0.0 ? order_value(hi) : -INFINITY;
+    }
+    __syncthreads();
     auto from_list = [&](uint32_t n) {
         if (rank == 0) {
-            finish_list(sh, static_cast<int>(n), top, inv_t, k, top_p, min_p, u, &p.tokens[r], &p.kept[r]);
+            finish_list(sh, static_cast<int>(n), &p.tokens[r], &p.kept[r]);
             if (threadIdx.x == 0) p.status[r] = BMS_STATUS_OK;
         }
     };
 
     // The tokens that can be kept, where a bound is known without another pass.
-    if (st.finite <= kCap) return from_list(collect([](float) { return true; }));
-    if (k_cuts) {
-        const float low = k <= kWarps * c ? st.low[0] : k <= 4 * kWarps * c ? st.low[1] : st.low[2];
-        if (k <= kThreads * c && low > -INFINITY) {
-            const uint32_t n = collect([&](float x) { return x >= low; });
-            if (n <= kCap) return from_list(n);
-        }
-    } else if (min_p > 0.0 && top_p >= 1.0) {
-        // A little below the smallest weight kept, so that rounding here decides nothing.
-        const double floor_x = top + temp * (log(min_p) - 1e-9) - 1e-12 * (fabs(top) + 1.0);
-        const float low = __double2float_rd(floor_x);
-        const uint32_t n = collect([&](float x) { return x >= low; });
+    float low = INFINITY;
+    if (st.finite <= kCap) low = -FLT_MAX;
+    else if (k_cuts && k <= kThreads * c) low = k <= kWarps * c ? st.low[0] : k <= 4 * kWarps * c ? st.low[1] : st.low[2];
+    else if (!k_cuts && min_p > 0.0 && top_p >= 1.0) low = fmaxf(sh.floor_x, -FLT_MAX);
+    if (low > -INFINITY && low < INFINITY) {
+        const uint32_t n = collect<T>(sh, view, low);
         if (n <= kCap) return from_list(n);
     }
 
-    // Counts of the tokens with key >= from by value bins of width span / kBins below the maximum, in sh.merged (a
-    // token further down is in the last bin), the same in every CTA.
-    const float span = static_cast<float>(fmin(40.0 * temp, 1e30));
-    const float bin_scale = 2.0f * kBins / span;
-    auto bin_of = [&](float x) { return static_cast<int>(fminf((0.5f * topf - 0.5f * x) * bin_scale, kBins - 1.0f)); };
-    auto count_bins = [&](uint64_t from) {
-        for (int i = threadIdx.x; i < kBins; i += kThreads) sh.bins[i] = 0;
-        __syncthreads();
-        each_group(view, g0, g1, [&](int64_t t, const float(&x)[8], uint32_t b) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (((b >> i) & 1) && x[i] > -INFINITY && (from == 0 || order_key(x[i], static_cast<uint32_t>(t + i)) >= from))
-                    atomicAdd(&sh.bins[bin_of(x[i])], 1u);
-        });
-        cluster.sync();
-        for (int i = threadIdx.x; i < kBins; i += kThreads) {
-            uint32_t n = 0;
-            for (int q = 0; q < c; ++q) n += cluster.map_shared_rank(sh.bins, q)[i];
-            sh.merged[i] = n;
-        }
-        cluster.sync();
-    };
-
-    // Cut of the first k tokens: exact counts find the bin that holds rank k; its tokens, sorted, give the key.
-    uint64_t cut = 0;
+    // End of the first k tokens: exact counts find the bin that holds rank k; its tokens, sorted, give the place.
     if (k_cuts) {
-        count_bins(0);
+        count_bins<T>(sh, view, queue);
         uint32_t mine = 0, all;
         for (int i = 0; i < kPerThread; ++i) mine += sh.merged[threadIdx.x * kPerThread + i];
         uint32_t run = block_before(mine, reinterpret_cast<uint32_t*>(sh.warp_mass), all);
@@ -613,283 +1216,85 @@ __global__ void __launch_bounds__(kThreads, 2) filter_sample_kernel(const Filter
         __syncthreads();
         const int bin = sh.bin[0];
         const uint32_t before = sh.bin_count, inside = sh.merged[bin];
-        if (before + inside <= kCap && bin < kBins - 1) return from_list(collect([&](float x) { return bin_of(x) <= bin; }));
+        if (before + inside <= kCap && bin < kBins - 1) {
+            // A score a little below the bin: all of the first k tokens lie above it.
+            low = sh.topf - (bin + 1) * sh.width - 1e-5f * (fabsf(sh.topf) + sh.width * kBins);
+            if (bin_of(low, sh.bin_at, sh.bin_scale) > bin) {
+                const uint32_t n = collect<T>(sh, view, fmaxf(low, -FLT_MAX));
+                if (n <= kCap) return from_list(n);
+            }
+        }
         if (inside <= kCap) {
-            const uint32_t n = collect([&](float x) { return bin_of(x) == bin; });
+            collect_bin<T>(sh, view, queue, bin);
+            const uint32_t n = pool(sh);
             if (rank == 0) {
-                const int m = round_pow2(n);
-                for (int i = n + threadIdx.x; i < m; i += kThreads) sh.list[i] = 0;
-                sort_desc(sh.list, m);
-                if (threadIdx.x < c) *cluster.map_shared_rank(&sh.cut, threadIdx.x) = sh.list[k - before - 1];
+                int kept;
+                double mass;
+                const uint64_t key = list_cut(sh, static_cast<int>(n), k - before, 1.0, 0.0, 0.0, kept, mass);
+                if (threadIdx.x < c) *cluster.map_shared_rank(&sh.cut, threadIdx.x) = key;
             }
             cluster.sync();
-            cut = sh.cut;
         } else {
-            uint64_t lo = 0, hi = ~0ull;
-            while (lo < hi) {
-                const uint64_t mid = lo + (hi - lo) / 2;
-                if (sum_above(cluster, sh, view, g0, g1, top, inv_t, mid, 0, false, turn).count < k) hi = mid;
-                else lo = mid + 1;
-            }
-            cut = lo;
+            const uint64_t key = bisect<T>(sh, view, queue, 0, static_cast<double>(k), false, turn);
+            if (threadIdx.x == 0) sh.cut = key;
         }
+        __syncthreads();
+        if (threadIdx.x == 0) sh.first_k = sh.cut;
+        __syncthreads();
     }
+    uint64_t cut = sh.first_k;
+    bool have_spans = false;
     if (top_p < 1.0) {
-        // Where the nucleus ends, by the bins' counts and middle weights.  The estimate is good to about a part
-        // in a thousand of the mass; a miss tells the exact masses around the bracket, which place the next one.
-        count_bins(cut);
-        const float step = span / kBins * static_cast<float>(inv_t) * 1.44269504f;
-        float mine = 0.f, all;
-        for (int i = 0; i < kPerThread; ++i) {
-            const int at = threadIdx.x * kPerThread + i;
-            mine += sh.merged[at] * exp2f(-(at + 0.5f) * step);
+        have_spans = find_nucleus<T>(sh, view, queue, &p.kept[r], &p.status[r]);
+        if (!have_spans) {
+            const double limit = top_p * sum_above<T>(sh, view, queue, 0, cut, true, turn).mass;
+            cut = bisect<T>(sh, view, queue, cut, limit, true, turn);
+        } else {
+            cut = max(cut, sh.cut);
         }
-        const float run = block_before(mine, reinterpret_cast<float*>(sh.warp_mass), all);
-        float goal = static_cast<float>(top_p) * all, slack = 1e-3f;
-        bool found = false;
-        uint64_t nucleus = 0;
-        for (int attempt = 0; attempt < 3 && !found; ++attempt, slack = 2e-4f) {
-            __syncthreads();
-            if (threadIdx.x == 0) sh.bin[0] = 0, sh.bin[1] = sh.bin[2] = kBins - 1, sh.bin_count = 0;
-            __syncthreads();
-#pragma unroll
-            for (int side = 0; side < 3; ++side) {
-                const float want = side == 0 ? goal - slack * all : side == 1 ? goal + slack * all : goal;
-                if (run < want && want <= run + mine) {
-                    float before = run;
-                    int i = threadIdx.x * kPerThread;
-                    for (const int last = i + kPerThread - 1; i < last; ++i) {
-                        const float m = sh.merged[i] * exp2f(-(i + 0.5f) * step);
-                        if (before + m >= want) break;
-                        before += m;
-                    }
-                    sh.bin[side] = i;
-                }
-            }
-            __syncthreads();
-            int b0 = max(sh.bin[0] - 1, 0), b1 = min(sh.bin[1] + 1, kBins - 1);
-            uint32_t inside = 0;
-            for (int i = b0 + threadIdx.x; i <= b1; i += kThreads) inside += sh.merged[i];
-            inside = __reduce_add_sync(0xffffffffu, inside);
-            if (lane == 0) atomicAdd(&sh.bin_count, inside);
-            __syncthreads();
-            inside = sh.bin_count;
-            if (inside > kCap) b0 = b1 = sh.bin[2], inside = sh.merged[b0];
-            if (inside > kCap || inside == 0) break;
-            double above = 0.0, below = 0.0;
-            __syncthreads();
-            if (threadIdx.x == 0) sh.list_count = 0;
-            __syncthreads();
-            each_group(view, g0, g1, [&](int64_t t, const float(&x)[8], uint32_t b) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (!((b >> i) & 1) || !(x[i] > -INFINITY)) continue;
-                    const uint64_t key = order_key(x[i], static_cast<uint32_t>(t + i));
-                    if (key < cut) continue;
-                    const int bin = bin_of(x[i]);
-                    if (bin >= b0 && bin <= b1) {
-                        sh.list[atomicAdd(&sh.list_count, 1u)] = key;
-                    } else {
-                        const double w = weight_of(x[i], top, inv_t, sh.exp_table);
-                        if (bin < b0) above += w;
-                        else below += w;
-                    }
-                }
-            });
-            above = warp_sum(above), below = warp_sum(below);
-            __syncthreads();
-            if (lane == 0) sh.warp_mass[warp] = above, sh.spans[warp] = below;
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                above = below = 0.0;
-                for (int w = 0; w < kWarps; ++w) above += sh.warp_mass[w], below += sh.spans[w];
-                *cluster.map_shared_rank(&sh.above[rank], 0) = above;
-                *cluster.map_shared_rank(&sh.below[rank], 0) = below;
-            }
-            if (threadIdx.x < c) *cluster.map_shared_rank(&sh.list_counts[rank], threadIdx.x) = sh.list_count;
-            cluster.sync();
-            uint32_t mine = 0, n = 0;
-            for (int i = 0; i < c; ++i) {
-                if (i < rank) mine += sh.list_counts[i];
-                n += sh.list_counts[i];
-            }
-            if (rank != 0) {
-                uint64_t* dst = cluster.map_shared_rank(sh.list, 0) + mine;
-                for (uint32_t i = threadIdx.x; i < sh.list_count; i += kThreads) dst[i] = sh.list[i];
-            }
-            cluster.sync();
-            if (rank == 0) {
-                above = below = 0.0;
-                for (int i = 0; i < c; ++i) above += sh.above[i], below += sh.below[i];
-                const int m = round_pow2(n);
-                for (int i = n + threadIdx.x; i < m; i += kThreads) sh.list[i] = 0;
-                sort_desc(sh.list, m);
-                for (int i = threadIdx.x; i < n; i += kThreads)
-                    sh.weight[i] = weight_of(order_value(static_cast<uint32_t>(sh.list[i] >> 32)), top, inv_t, sh.exp_table);
-                if (threadIdx.x == 0) sh.pick = 0;
-                __syncthreads();
-                scan_in_place(sh.weight, n, sh);
-                const double limit = top_p * (above + sh.weight[n - 1] + below);
-                uint32_t kept = 0;
-                for (int i = threadIdx.x; i < n; i += kThreads) kept += above + (i ? sh.weight[i - 1] : 0.0) < limit;
-                if (kept) atomicAdd(&sh.pick, kept);
-                __syncthreads();
-                // Outside the bracket: not one of its tokens kept, or all of them with more below.
-                const bool ends_inside = sh.pick > 0 && (above + sh.weight[n - 1] >= limit || b1 == kBins - 1);
-                if (threadIdx.x < c) {
-                    *cluster.map_shared_rank(&sh.cut, threadIdx.x) = ends_inside ? sh.list[sh.pick - 1] : 0;
-                    *cluster.map_shared_rank(&sh.found, threadIdx.x) = ends_inside;
-                    // How far the end lies before the bracket (negative) or behind it.
-                    *cluster.map_shared_rank(&sh.goal, threadIdx.x) = static_cast<float>(sh.pick == 0 ? limit - above : limit - above - sh.weight[n - 1]);
-                }
-            }
-            cluster.sync();
-            found = sh.found;
-            nucleus = sh.cut;
-            if (!found) {  // the same correction from the estimated mass at the bracket's edge
-                const float off = sh.goal;
-                __syncthreads();
-                const int edge = off <= 0.f ? b0 : b1 + 1;
-                if (edge / kPerThread == threadIdx.x) {
-                    float e = run;
-                    for (int i = threadIdx.x * kPerThread; i < edge; ++i) e += sh.merged[i] * exp2f(-(i + 0.5f) * step);
-                    sh.goal = e + off;
-                }
-                __syncthreads();
-                goal = sh.goal;
-            }
-        }
-        if (!found) {
-            const double limit = top_p * sum_above(cluster, sh, view, g0, g1, top, inv_t, 0, cut, true, turn).mass;
-            uint64_t lo = cut, hi = ~0ull;
-            while (lo < hi) {
-                const uint64_t mid = lo + (hi - lo) / 2;
-                if (sum_above(cluster, sh, view, g0, g1, top, inv_t, mid, 0, true, turn).mass < limit) hi = mid;
-                else lo = mid + 1;
-            }
-            nucleus = lo;
-        }
-        cut = max(cut, nucleus);
     }
-    // Kept mass of every warp's span, in token order.
-    double mass = 0.0;
-    int64_t count = 0;
-    each_group(view, g0, g1, [&](int64_t t, const float(&x)[8], uint32_t b) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (!((b >> i) & 1) || !(x[i] > -INFINITY) || order_key(x[i], static_cast<uint32_t>(t + i)) < cut) continue;
-            const double w = weight_of(x[i], top, inv_t, sh.exp_table);
-            if (w >= min_p) mass += w, ++count;
+    // min-p: no token below its score, any token at it.
+    const Place end = place_of(max(cut, static_cast<uint64_t>(order_bits(sh.floor_x)) << 32));
+    // Kept masses by spans, unless the nucleus left them; rank 0 finds the span that holds the target.
+    if (!have_spans) {
+        weigh_spans<T>(sh, view, queue, end);
+        if (rank == 0 && threadIdx.x == 0) {
+            int64_t all = 0;
+            for (int i = 0; i < c; ++i) all += sh.counts[i];
+            p.kept[r] = all;
+            p.status[r] = BMS_STATUS_OK;
         }
-    });
-    mass = warp_sum(mass);
-    count = warp_sum(count);
-    if (lane == 0) sh.warp_count[warp] = count;
-    if (lane < c) *cluster.map_shared_rank(&sh.spans[rank * kWarps + warp], lane) = mass;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        int64_t all = 0;
-        for (int w = 0; w < kWarps; ++w) all += sh.warp_count[w];
-        cluster.map_shared_rank(&sh.part[turn][rank], 0)->count = all;
+    }
+    if (rank == 0) {
+        __syncthreads();
+        // Running masses of the spans, in token order.
+        static_assert(kMaxCluster * kWarps <= kThreads, "a span per thread");
+        const double mine = threadIdx.x < c * kWarps ? sh.spans[threadIdx.x] : 0.0;
+        double total;
+        const double before = block_before(mine, sh.warp_mass, total);
+        const double target = u * total;
+        if (threadIdx.x == 0) sh.pick = 0xffffffffu, sh.last = 0;
+        __syncthreads();
+        // The first span whose running mass exceeds the target; without one (rounding at the very end) the last with mass.
+        if (mine > 0.0) {
+            if (before + mine > target) atomicMin(&sh.pick, threadIdx.x);
+            atomicMax(&sh.last, threadIdx.x);
+        }
+        __syncthreads();
+        const uint32_t owner = sh.pick != 0xffffffffu ? sh.pick : sh.last;
+        if (threadIdx.x == owner) {
+            for (int i = 0; i < c; ++i) {
+                *cluster.map_shared_rank(&sh.owner, i) = static_cast<int32_t>(owner);
+                *cluster.map_shared_rank(&sh.target, i) = target;
+                *cluster.map_shared_rank(&sh.before, i) = before;
+            }
+        }
     }
     cluster.sync();
-    if (threadIdx.x == 0) {
-        double total = 0.0;
-        for (int i = 0; i < c * kWarps; ++i) total += sh.spans[i];
-        const double target = u * total;
-        double run = 0.0;
-        int owner = -1;
-        for (int i = 0; i < c * kWarps; ++i) {
-            if (sh.spans[i] > 0.0) {
-                owner = i;
-                sh.before = run;
-                if (run + sh.spans[i] > target) break;
-            }
-            run += sh.spans[i];
-        }
-        sh.owner = owner;
-        sh.weight[0] = target;
+    if (sh.owner / kWarps == rank) {
+        walk_span<T>(sh, view, sh.owner % kWarps, end);
+        if (threadIdx.x == 0) p.tokens[r] = sh.token;
     }
-    __syncthreads();
-    if (rank == 0 && threadIdx.x == 0) {
-        int64_t all = 0;
-        for (int i = 0; i < c; ++i) all += sh.part[turn][i].count;
-        p.kept[r] = all;
-        p.status[r] = BMS_STATUS_OK;
-    }
-    if (sh.owner / kWarps != rank) return;
-    // The owner CTA walks the span that holds the target, one group per thread and round.
-    const double target = sh.weight[0];
-    double before = sh.before;
-    const int w0 = sh.owner % kWarps;
-    const int64_t s0 = c0 + (c1 - c0) * w0 / kWarps, s1 = c0 + (c1 - c0) * (w0 + 1) / kWarps;
-    if (threadIdx.x == 0) sh.token = -1, sh.found = 0;
-    __syncthreads();
-    for (int64_t base = s0; base < s1; base += kThreads) {
-        const int64_t g = base + threadIdx.x;
-        double w[8], sum = 0.0;
-        int last = -1;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = 0.0;
-        if (g < s1) {
-            const uint32_t b = view.bits(g);
-            float x[8];
-            if (b) view.load(g, x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (!((b >> i) & 1) || !(x[i] > -INFINITY) || order_key(x[i], static_cast<uint32_t>(view.first(g) + i)) < cut) continue;
-                const double wi = weight_of(x[i], top, inv_t, sh.exp_table);
-                if (wi >= min_p && wi > 0.0) w[i] = wi, sum += wi, last = i;
-            }
-        }
-        double run = sum;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const double up = __shfl_up_sync(0xffffffffu, run, d);
-            if (lane >= d) run += up;
-        }
-        __syncthreads();
-        if (lane == 31) sh.warp_mass[warp] = run;
-        __syncthreads();
-        double start = before, all = before;
-        for (int i = 0; i < kWarps; ++i) {
-            if (i < warp) start += sh.warp_mass[i];
-            all += sh.warp_mass[i];
-        }
-        const double upv = __shfl_up_sync(0xffffffffu, run, 1);
-        if (lane > 0) start += upv;
-        // Tokens are in thread order: the first crossing thread wins; without one (rounding at the very
-        // end) the last token with mass.
-        double at = start;
-        int hit = -1;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            at += w[i];
-            if (hit < 0 && w[i] > 0.0 && at > target) hit = i;
-        }
-        if (threadIdx.x == 0) sh.pick = 0xffffffffu;
-        __syncthreads();
-        if (hit >= 0) atomicMin(&sh.pick, threadIdx.x);
-        __syncthreads();
-        const bool crossed = sh.pick != 0xffffffffu;
-        if (crossed) {
-            if (sh.pick == threadIdx.x) sh.token = view.first(g) + hit;
-            break;
-        }
-        // Remember the last token with mass so far.
-        const int any = __syncthreads_or(last >= 0);
-        if (any) {
-            if (threadIdx.x == 0) sh.list_base = 0;
-            __syncthreads();
-            if (last >= 0) atomicMax(&sh.list_base, threadIdx.x);
-            __syncthreads();
-            if (sh.list_base == threadIdx.x) sh.token = view.first(g) + last;
-        }
-        before = all;
-        __syncthreads();
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) p.tokens[r] = sh.token;
 }
 
 template <typename T>
@@ -897,19 +1302,22 @@ int launch_filter(const FilterParams& p, int device, cudaStream_t stream) {
     static bool ready[kMaxDevices];
     static int sms[kMaxDevices];
     auto kernel = filter_sample_kernel<T>;
+    constexpr size_t smem = sizeof(Shared);
+    static_assert(2 * (smem + 1024) <= 228 * 1024, "two CTAs per SM");
     if (!ready[device]) {
-        BMS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(Shared))), "cudaFuncSetAttribute(smem)");
+        BMS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)), "cudaFuncSetAttribute(smem)");
         BMS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "cudaFuncSetAttribute(cluster)");
         BMS_CUDA(cudaDeviceGetAttribute(&sms[device], cudaDevAttrMultiProcessorCount, device), "sm count");
         ready[device] = true;
     }
     int c = 1;
     while (c < 8 && p.rows * c * 2 <= sms[device] && p.vocab / (2 * c) >= 4096) c *= 2;
+    if (getenv("FC")) c = atoi(getenv("FC"));
     if (p.rows * c > 2147483647LL) return fail(BMS_ERROR_UNSUPPORTED, "too many rows");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(p.rows * c));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = sizeof(Shared);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -932,6 +1340,7 @@ extern "C" int bms_filtered_sample_batch(const void* logits, int32_t dtype, cons
     if (dtype != BMS_FLOAT32 && dtype != BMS_BFLOAT16 && dtype != BMS_FLOAT16)
         return fail(BMS_ERROR_INVALID_ARGUMENT, "logits must be float32, bfloat16 or float16 (dtype code %d)", dtype);
     if (vocab <= 0 || vocab > 2147483647LL) return fail(BMS_ERROR_INVALID_ARGUMENT, "invalid vocabulary size");
+    if (vocab > 2147479552LL) return fail(BMS_ERROR_UNSUPPORTED, "vocabulary beyond 2^31 - 4096 tokens");  // 32-bit token arithmetic
     if (rows < 0) return fail(BMS_ERROR_INVALID_ARGUMENT, "rows must not be negative");
     if (filter == nullptr) return fail(BMS_ERROR_INVALID_ARGUMENT, "filter must not be NULL");
     const bms_filter& f = *filter;
