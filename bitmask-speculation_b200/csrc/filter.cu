@@ -27,7 +27,6 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
-#include <cstdlib>
 #include <cstring>
 #include <type_traits>
 
@@ -70,14 +69,13 @@ struct FilterParams {
 
 struct RowStats {
     float max;               // maximum of the valid tokens
-    float low[3];            // smallest maximum of the groups of 32, 8 and 1 lanes
-    uint32_t finite, flags;  // valid tokens; 1 NaN, 2 some valid token, 4 a valid -inf
+    float low;               // smallest maximum of the half-lanes
+    uint32_t finite, flags;  // valid finite tokens; 1 NaN, 2 some valid token, 4 a full segment
 };
 
 __device__ __forceinline__ void merge(RowStats& a, const RowStats& o) {
     a.max = fmaxf(a.max, o.max);
-#pragma unroll
-    for (int i = 0; i < 3; ++i) a.low[i] = fminf(a.low[i], o.low[i]);
+    a.low = fminf(a.low, o.low);
     a.finite += o.finite;
     a.flags |= o.flags;
 }
@@ -94,6 +92,13 @@ struct MassCount {
     int64_t count;
 };
 
+// A warp's rounds in flight: a vector per lane, copied without registers (cp.async); a lane reads only
+// what it copied itself, so no barrier is needed.  (Loads ahead into rotating registers stall at the first move.)
+constexpr int kAhead = 4;
+struct Ring {
+    uint4 vec[kAhead][32];
+};
+
 struct Shared {
     double top, rate, top_p, u;     // the row: maximum, 512 / (T ln 2), nucleus, uniform
     float topf, floor_x;            // maximum; lowest score that min-p keeps
@@ -105,21 +110,27 @@ struct Shared {
     int32_t b0, b1;                 // bracket of bins
     alignas(16) unsigned char view[64];  // RowView
     union {
-        uint64_t list[kCap];   // order keys
-        uint32_t bins[kBins];  // this CTA's counts, until every CTA has read them
+        uint64_t list[kCap];  // order keys
+        struct {
+            uint32_t bins[kBins];    // this CTA's counts, until every CTA has read them
+            uint32_t merged[kBins];  // the row's counts
+        };
+        Ring first_ring[kWarps];  // of the passes that collect, which write the list at their end
     };
     union {
         struct {
-            uint32_t merged[kBins];  // the row's counts
             uint32_t queue[kWarps][2 * kQueue<float>];
+            Ring ring[kWarps];       // of the passes over single tokens
         };
         uint64_t segment[kWarps][kSegment];  // keys that a warp collected, until they are in the list
-        RowStats warp_stats[kWarps];
     };
+    RowStats warp_stats[kWarps];
+    uint32_t fills[kWarps];  // tokens in the warps' segments
     double exp_table[kTable];
     double spans[kMaxCluster * kWarps];
     unsigned long long extra[kMaxCluster * kWarps];  // kept bracket tokens' mass by span, units of 2^-50
     uint32_t warp_counts[kMaxCluster * kWarps];
+    float group_max[kMaxCluster * kWarps * 4];  // of the 8-lane groups of every warp
     MassCount part[2][kMaxCluster];
     RowStats stats[kMaxCluster];
     double warp_mass[kWarps], warp_below[kWarps], step_mass[2][kWarps];
@@ -128,7 +139,7 @@ struct Shared {
     double target, before;
     uint64_t cut;
     uint32_t list_counts[kMaxCluster];
-    uint32_t list_count, bin_count, pick, last, passed;
+    uint32_t list_count, bin_count, pick, last, passed, low_bits;
     int32_t bin[3];
     float goal, floor;
     int32_t found, owner, token;
@@ -183,6 +194,7 @@ struct Pair<__half> {
 template <>
 struct Pair<float> {
     static constexpr uint32_t kInf = 0;
+    static __device__ __forceinline__ float lo(uint32_t u) { return __uint_as_float(u); }
 };
 
 template <typename T>
@@ -237,6 +249,45 @@ struct RowView {
     __device__ __forceinline__ bool valid(int32_t t) const { return mask == nullptr || (static_cast<uint32_t>(mask[t >> 5]) >> (t & 31) & 1); }
 };
 
+// The full groups of a warp's span, a round of one vector per lane at a time, kAhead - 1 rounds ahead (the mask bits one).
+template <typename T>
+struct Stream {
+    const RowView<T>& v;
+    Ring& ring;
+    int32_t z, lane;
+    int32_t g, ahead;  // this lane's groups: of the current round, of the next one to copy
+    int32_t slot = 0;
+    uint32_t word;     // mask bits of the next round
+    __device__ __forceinline__ void copy(int to) {
+        if (ahead < z) ptx::cp_async_16(ptx::smem_addr(&ring.vec[to][lane]), reinterpret_cast<const uint4*>(v.row - v.skew) + ahead);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        ahead += 32;
+    }
+    __device__ __forceinline__ uint32_t bits_of(int32_t at) const { return at < z ? v.bits(at) : 0u; }
+    __device__ __forceinline__ Stream(const RowView<T>& view, Ring& r, int32_t g0, int32_t g1) : v(view), ring(r), z(min(g1, view.full1)), lane(threadIdx.x & 31) {
+        g = ahead = max(g0, view.full0) + lane;
+        for (int i = 0; i < kAhead - 1; ++i) copy(i);
+        word = bits_of(g);
+    }
+    __device__ __forceinline__ bool more() const { return g - lane < z; }
+    // The current round's vector, and its bits (0 behind the span's end); starts the copy of a later one.
+    __device__ __forceinline__ uint32_t take(uint4& now) {
+        const uint32_t bits = word;
+        word = bits_of(g + 32);
+        copy((slot + kAhead - 1) % kAhead);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+        now = ring.vec[slot][lane];
+        return bits;
+    }
+    __device__ __forceinline__ void next() { slot = (slot + 1) % kAhead, g += 32; }
+    // Element j of the current round's vector.
+    __device__ __forceinline__ float element(int j) const { return widen(reinterpret_cast<const T*>(&ring.vec[slot][lane])[j]); }
+    __device__ __forceinline__ uint32_t raw_element(int j) const {
+        if constexpr (sizeof(T) == 2) return reinterpret_cast<const uint16_t*>(&ring.vec[slot][lane])[j];
+        else return reinterpret_cast<const uint32_t*>(&ring.vec[slot][lane])[j];
+    }
+};
+
 // exp((x - top) / T), float64: t = (x - top) * rate in units of 2^(1/512) splits into an integer n and |r| <= 1/2; 2^(n / 512)
 // comes from a table and the exponent field, 2^(r / 512) from its series to r^3 (the next term is below 1e-14
 // relative), far below what decides a token.  Branch-free, a quarter of the instructions of the library's exp.
@@ -256,101 +307,100 @@ __device__ __forceinline__ double weight_of(float x, double top, double rate, co
     return t < -1075.0 * kTable ? 0.0 : e;
 }
 
-// Calls f(x, token, live) for the valid tokens of the groups [g0, g1), two per lane at a time.  Rounds in which every
-// token is valid go straight from the registers; in others the valid tokens of a round of one vector per lane go
-// through the warp's queue in shared memory, so that f's cost follows their number and not the vocabulary
-// (grammar masks keep 0.1 - 60 % of it).  A queue entry is 16 bits of score and 16 of offset for 16-bit
-// types, 8 bytes for float32.
+// Calls f(x, token, live) for the valid tokens of the warp's span.  Rounds (one vector per lane) in which every token is
+// valid go straight from the registers, unrolled; in others the valid tokens go through the warp's queue in shared
+// memory, two per lane at a time, so that f's cost follows their number and not the vocabulary (grammar
+// masks keep 0.1 - 60 % of it).  A queue entry is 16 bits of score and 16 of offset for 16-bit types, 8 bytes
+// for float32.
 template <typename T, typename F>
-__device__ __forceinline__ void each_token(const RowView<T>& v, int32_t g0, int32_t g1, uint32_t* queue, F f) {
+__device__ __forceinline__ void each_token(Shared& sh, const RowView<T>& v, F f) {
     constexpr bool kHalf = sizeof(T) == 2;
-    constexpr int kVec = RowView<T>::kVec, kBatch = 4;
+    constexpr int kVec = RowView<T>::kVec;
     constexpr int kGroups = 65536 / kVec;  // offsets stay within 16 bits
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int32_t g0 = sh.bounds[warp], g1 = sh.bounds[warp + 1];
+    uint32_t* queue = sh.queue[warp];
     const uint32_t below = (1u << lane) - 1u;
-    const int32_t a = max(g0, v.full0), z = min(g1, v.full1);
-    for (int32_t base = a; base < z; base += kGroups) {
-        const int groups = min(z - base, kGroups);
+    auto push = [&](int to, uint32_t value, uint32_t offset) {
+        if constexpr (kHalf) queue[to] = value | (offset << 16);
+        else reinterpret_cast<uint2*>(queue)[to] = make_uint2(value, offset);
+    };
+    for (int32_t base = max(g0, v.full0); base < min(g1, v.full1); base += kGroups) {
+        const int32_t last = min(min(g1, v.full1), base + kGroups);
         const int32_t t0 = v.first(base);
         int fill = 0;
-        auto pop = [&](int i) {
-            const bool live = i < fill;
-            float x = -INFINITY;
-            int32_t t = t0;
-            if (live) {
-                if constexpr (kHalf) {
-                    const uint32_t e = queue[i];
-                    x = Pair<T>::lo(e);
-                    t += e >> 16;
-                } else {
-                    const uint2 e = reinterpret_cast<const uint2*>(queue)[i];
-                    x = __uint_as_float(e.x);
-                    t += e.y;
+        for (Stream<T> stream(v, sh.ring[warp], base, last); stream.more(); stream.next()) {
+            uint4 now;
+            const uint32_t bits = stream.take(now);
+            const uint32_t at = (stream.g - base) * kVec;
+            if (__all_sync(0xffffffffu, bits == RowView<T>::kAll)) {
+                float x[kVec];
+                v.expand(now, x);
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) f(x[j], static_cast<uint32_t>(t0 + at + j), x[j] > -INFINITY);
+                continue;
+            }
+            const int most = __reduce_max_sync(0xffffffffu, __popc(bits));
+            if (most > 3) {
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) {
+                    const bool in = (bits >> j) & 1;
+                    const uint32_t who = __ballot_sync(0xffffffffu, in);
+                    if (in) push(fill + __popc(who & below), (&now.x)[kHalf ? j >> 1 : j] >> (kHalf && (j & 1) ? 16 : 0) & (kHalf ? 0xffffu : 0xffffffffu), at + j);
+                    fill += __popc(who);
+                }
+            } else {  // a few tokens per lane: one per lane and step
+                uint32_t rest = bits;
+#pragma unroll 1
+                for (int i = 0; i < most; ++i, rest &= rest - 1) {
+                    const uint32_t who = __ballot_sync(0xffffffffu, rest != 0);
+                    if (rest) {
+                        const int j = __ffs(rest) - 1;
+                        push(fill + __popc(who & below), stream.raw_element(j), at + j);
+                    }
+                    fill += __popc(who);
                 }
             }
-            f(x, static_cast<uint32_t>(t), x > -INFINITY);
-        };
-        for (int i0 = 0; i0 < groups; i0 += 32 * kBatch) {
-            uint32_t b[kBatch];
-            uint4 raw[kBatch];
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) b[i] = i0 + 32 * i + lane < groups ? v.bits(base + i0 + 32 * i + lane) : 0u;
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i)
-                if (b[i]) raw[i] = v.fetch(base + i0 + 32 * i + lane);
-            // Rolled, so that f exists once per way: the round's vector moves to the front instead of being indexed.
+            __syncwarp();
+            const bool ends = stream.g - lane + 32 >= stream.z;  // the last round empties the queue
 #pragma unroll 1
-            for (int i = 0; i < kBatch; ++i) {
-                const bool ends = i0 + 32 * (i + 1) >= groups;  // the last round empties the queue
-                const uint32_t bits = b[0];
-                uint4 now = raw[0];
+            while (fill >= 64 || (ends && fill > 0)) {
+                const int from = max(fill - 64, 0);
 #pragma unroll
-                for (int j = 1; j < kBatch; ++j) b[j - 1] = b[j], raw[j - 1] = raw[j];
-                const uint32_t at = (i0 + 32 * i + lane) * kVec;
-                if (__all_sync(0xffffffffu, bits == RowView<T>::kAll)) {
-                    uint32_t t = t0 + at;
-#pragma unroll 1
-                    for (int j = 0; j < kVec; j += 2, t += 2) {
-                        float x0, x1;
+                for (int i = 0; i < 2; ++i) {
+                    const int k = from + 32 * i + lane;
+                    float x = -INFINITY;
+                    uint32_t t = 0;
+                    if (k < fill) {
                         if constexpr (kHalf) {
-                            x0 = Pair<T>::lo(now.x), x1 = Pair<T>::hi(now.x);
-                            now.x = now.y, now.y = now.z, now.z = now.w;
+                            const uint32_t e = queue[k];
+                            x = Pair<T>::lo(e);
+                            t = t0 + (e >> 16);
                         } else {
-                            x0 = __uint_as_float(now.x), x1 = __uint_as_float(now.y);
-                            now.x = now.z, now.y = now.w;
+                            const uint2 e = reinterpret_cast<const uint2*>(queue)[k];
+                            x = __uint_as_float(e.x);
+                            t = t0 + e.y;
                         }
-                        f(x0, t, x0 > -INFINITY);
-                        f(x1, t + 1, x1 > -INFINITY);
                     }
-                } else if (__any_sync(0xffffffffu, bits != 0)) {
-#pragma unroll
-                    for (int j = 0; j < kVec; ++j) {
-                        const bool in = (bits >> j) & 1;
-                        const uint32_t who = __ballot_sync(0xffffffffu, in);
-                        const int to = fill + __popc(who & below);
-                        if (in) {
-                            if constexpr (kHalf) {
-                                const uint32_t w = (j >> 1) == 0 ? now.x : (j >> 1) == 1 ? now.y : (j >> 1) == 2 ? now.z : now.w;
-                                queue[to] = ptx::prmt(w, at + j, j & 1 ? 0x5432u : 0x5410u);
-                            } else {
-                                reinterpret_cast<uint2*>(queue)[to] = make_uint2(j == 0 ? now.x : j == 1 ? now.y : j == 2 ? now.z : now.w, at + j);
-                            }
-                        }
-                        fill += __popc(who);
-                    }
-                    __syncwarp();
+                    f(x, t, x > -INFINITY);
                 }
-#pragma unroll 1
-                while (fill >= 64 || (ends && fill > 0)) {
-                    const int from = max(fill - 64, 0);
-                    pop(from + lane);
-                    pop(from + 32 + lane);
-                    fill = from;
-                    __syncwarp();
-                }
-                if (ends) break;
+                fill = from;
+                __syncwarp();
             }
         }
+        // A queue left by sparse rounds before a last dense one.
+        while (fill > 0) {
+            const int from = max(fill - 32, 0);
+            float x = -INFINITY;
+            uint32_t t = 0;
+            if (from + lane < fill) {
+                if constexpr (kHalf) x = Pair<T>::lo(queue[from + lane]), t = t0 + (queue[from + lane] >> 16);
+                else x = __uint_as_float(queue[2 * (from + lane)]), t = t0 + queue[2 * (from + lane) + 1];
+            }
+            f(x, t, x > -INFINITY);
+            fill = from;
+        }
+        __syncwarp();
     }
     const int32_t t = v.edge(g0, g1);
     if (__any_sync(0xffffffffu, t >= 0)) {
@@ -456,7 +506,7 @@ __device__ __noinline__ uint64_t list_cut(Shared& sh, int n, int64_t k, double p
         }
         return a;
     };
-    uint32_t cut_v = 0, cut_t = 0xfffffffeu;  // entries behind the list carry token 0xffffffff
+    uint32_t cut_v = lowest, cut_t = 0xfffffffeu;  // all of the list; entries behind it carry token 0xffffffff
     kept = n;
     if (k < n) {
         uint32_t a = lowest, b = highest;
@@ -513,7 +563,31 @@ __device__ __noinline__ void finish_list(Shared& sh, int n, int64_t* token, int6
     const int64_t k = sh.k;
     const float floor_x = sh.floor_x;
     uint64_t cut = 0;
-    if (k < n || p < 1.0) {
+    if (n <= kThreads && (k < n || p < 1.0)) {
+        // A thread per token counts and weighs the tokens ahead of its own in the order: no barriers on the way.
+        double* weights = reinterpret_cast<double*>(sh.segment);
+        const int i = threadIdx.x;
+        const uint64_t key = i < n ? sh.list[i] : 0;
+        const double w = i < n ? weight_of(order_value(static_cast<uint32_t>(key >> 32)), top, rate, sh.exp_table) : 0.0;
+        weights[i] = w;
+        __syncthreads();
+        int ahead = 0;
+        double before = 0.0;
+        if ((i & ~31) < n) {
+#pragma unroll 4
+            for (int j = 0; j < n; ++j)
+                if (sh.list[j] > key) ++ahead, before += weights[j];
+        }
+        const bool in = i < n && ahead < k;
+        double total;
+        block_before(in ? w : 0.0, sh.warp_mass, total);
+        const bool keep = in && (p >= 1.0 || before < p * total);
+        if (threadIdx.x == 0) sh.cut = ~0ull;
+        __syncthreads();
+        if (keep) atomicMin(reinterpret_cast<unsigned long long*>(&sh.cut), static_cast<unsigned long long>(key));
+        __syncthreads();
+        cut = sh.cut;
+    } else if (k < n || p < 1.0) {
         int kept;
         double mass;
         cut = list_cut(sh, n, k, p, 0.0, 0.0, kept, mass);
@@ -560,20 +634,22 @@ __device__ __noinline__ void finish_list(Shared& sh, int n, int64_t* token, int6
 }
 
 // A score's bin: one rounding, so higher scores never lie in later bins.
-__device__ __forceinline__ int bin_of(float x, float at, float scale) { return static_cast<int>(fminf(fmaxf(fmaf(x, -scale, at), 0.f), kBins - 1.f)); }
+__device__ __forceinline__ int bin_of(float x, float at, float scale) {
+    return __float_as_int(fminf(fmaxf(fmaf(x, -scale, at), 0.f), kBins - 1.f) + 8388608.f) & (kBins - 1);  // adding 2^23 rounds to an integer
+}
 
 // The passes below are functions of their own, with the row's state in shared memory: inlined together they would
 // share one register budget (64, for two CTAs of 512 per SM) and spill in their loops.
 
 // Mass (0 unless `weigh`) and count over the cluster of the tokens with key > above and key >= floor_key, summed in a fixed order.
 template <typename T>
-__device__ __noinline__ MassCount sum_above(Shared& sh, const RowView<T>& shared_view, uint32_t* queue, uint64_t above, uint64_t floor_key, bool weigh, int& turn) {
+__device__ __noinline__ MassCount sum_above(Shared& sh, const RowView<T>& shared_view, uint64_t above, uint64_t floor_key, bool weigh, int& turn) {
     cg::cluster_group cluster = cg::this_cluster();
     const RowView<T> view = shared_view;
     const int c = cluster.num_blocks(), rank = cluster.block_rank(), warp = threadIdx.x >> 5;
     double mass = 0.0;
     int64_t count = 0;
-    each_token(view, sh.bounds[warp], sh.bounds[warp + 1], queue, [&](float x, uint32_t t, bool live) {
+    each_token(sh, view, [&](float x, uint32_t t, bool live) {
         const uint64_t k = order_key(x, t);
         if (live && k > above && k >= floor_key) {
             if (weigh) mass += weight_of(x, sh.top, sh.rate, sh.exp_table);
@@ -598,102 +674,181 @@ __device__ __noinline__ MassCount sum_above(Shared& sh, const RowView<T>& shared
 
 // The smallest order key whose preceding count (weigh: mass) is below the limit, by bisection from `lo`.
 template <typename T>
-__device__ __noinline__ uint64_t bisect(Shared& sh, const RowView<T>& view, uint32_t* queue, uint64_t lo, double limit, bool weigh, int& turn) {
+__device__ __noinline__ uint64_t bisect(Shared& sh, const RowView<T>& view, uint64_t lo, double limit, bool weigh, int& turn) {
     uint64_t hi = ~0ull;
     while (lo < hi) {
         const uint64_t mid = lo + (hi - lo) / 2;
-        const MassCount mc = sum_above(sh, view, queue, mid, 0, weigh, turn);
+        const MassCount mc = sum_above(sh, view, mid, 0, weigh, turn);
         if ((weigh ? mc.mass : static_cast<double>(mc.count)) < limit) hi = mid;
         else lo = mid + 1;
     }
     return lo;
 }
 
-// The first pass: statistics of the row over the cluster.
+// Appends this lane's tokens `in` of the current round (tokens from t on) to the warp's segment in token order.
 template <typename T>
-__device__ __noinline__ RowStats first_pass(Shared& sh, const RowView<T>& shared_view) {
+__device__ __forceinline__ void append(uint64_t* segment, uint32_t& fill, uint32_t in, const Stream<T>& stream, int32_t t) {
+    const int lane = threadIdx.x & 31;
+    uint32_t run = __popc(in);
+    uint32_t at = fill - run;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, run, d);
+        if (lane >= d) run += up;
+    }
+    at += run;
+    fill += __shfl_sync(0xffffffffu, run, 31);
+#pragma unroll 1
+    for (; in; in &= in - 1, ++at) {
+        const int j = __ffs(in) - 1;
+        if (at < kSegment) segment[at] = order_key(stream.element(j), static_cast<uint32_t>(t + j));
+    }
+}
+
+// Drops a segment's tokens with x < low, in place; returns how many stay.
+__device__ __forceinline__ uint32_t filter(uint64_t* segment, uint32_t have, float low) {
+    const int lane = threadIdx.x & 31;
+    const uint64_t key = static_cast<uint64_t>(order_bits(low)) << 32;
+    uint32_t fill = 0;
+    for (uint32_t i = 0; i < have; i += 32) {  // entries only move forward
+        const uint64_t k = i + lane < have ? segment[i + lane] : 0;
+        const uint32_t who = __ballot_sync(0xffffffffu, k >= key);
+        __syncwarp();
+        if (k >= key) segment[fill + __popc(who & ((1u << lane) - 1u))] = k;
+        __syncwarp();
+        fill += __popc(who);
+    }
+    return fill;
+}
+
+// A row's edge tokens (front or back of the full groups), one per lane, likewise.
+template <typename T>
+__device__ __forceinline__ void append_edge(const RowView<T>& view, uint64_t* segment, uint32_t& fill, float low, int32_t g0, int32_t g1, bool front) {
+    const int lane = threadIdx.x & 31;
+    const int32_t t = view.edge(g0, g1);
+    const float x = t >= 0 && (lane < RowView<T>::kVec) == front && view.valid(t) ? widen(view.row[t]) : -INFINITY;
+    const uint32_t who = __ballot_sync(0xffffffffu, x >= low);
+    const uint32_t at = fill + __popc(who & ((1u << lane) - 1u));
+    if (x >= low && at < kSegment) segment[at] = order_key(x, static_cast<uint32_t>(t));
+    fill += __popc(who);
+}
+
+// The valid tokens with x >= low of a vector, one bit each.
+template <typename T>
+__device__ __forceinline__ uint32_t reaching(const uint4& now, uint32_t bits, float low) {
+    constexpr int kVec = RowView<T>::kVec;
+    float x[kVec];
+    RowView<T>::expand(now, x);
+    uint32_t in = 0;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) in |= static_cast<uint32_t>(x[j] >= low) << j;
+    return in & bits;
+}
+
+// The first pass: statistics of the row over the cluster, and, while it streams, the tokens that can matter: a warp keeps
+// those that reach a bound which only rises.  mode 1 (top-k of at most 32): the smallest of its lanes' maxima so far,
+// which at least 32 tokens reach (about 32 ln 32 of them stay: they fit the segment); mode 2 (min-p): its maximum
+// so far less `drop`; mode 0: none, for sparse masks.  A warp whose segment is full stops keeping, and the row needs
+// another pass.
+template <typename T>
+__device__ __noinline__ RowStats first_pass(Shared& sh, const RowView<T>& shared_view, int mode, float drop) {
     cg::cluster_group cluster = cg::this_cluster();
     const RowView<T> view = shared_view;
     const int c = cluster.num_blocks(), rank = cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int32_t g0 = sh.bounds[warp], g1 = sh.bounds[warp + 1];
     constexpr int kVec = RowView<T>::kVec;
-    RowStats st{-INFINITY, {}, 0, 0};
-    {
-        uint32_t valid = 0, nan2 = Pair<T>::kInf ^ 0x80008000u, max2 = nan2, min2 = Pair<T>::kInf;
-        float nan1 = -INFINITY, min1 = INFINITY;
-        constexpr int kBatch = 6;
-        const int32_t z = min(g1, view.full1);
-        for (int32_t g = max(g0, view.full0) + lane; g < z; g += 32 * kBatch) {
-            uint32_t b[kBatch];
-            uint4 raw[kBatch];
+    uint64_t* segment = sh.segment[warp];
+    uint32_t fill = 0, finite = 0, some = 0, nan2 = Pair<T>::kInf ^ 0x80008000u, max2 = nan2;
+    float nan1 = -INFINITY, max_a = -INFINITY, max_b = -INFINITY, low = -FLT_MAX;
+    append_edge(view, segment, fill, low, g0, g1, true);
+#pragma unroll 1
+    for (Stream<T> stream(view, sh.first_ring[warp], g0, g1); stream.more(); stream.next()) {
+        uint4 now;
+        const uint32_t bits = stream.take(now);
+        if (stream.g >= stream.z) now = make_uint4(0, 0, 0, 0);
+        const uint32_t w[4] = {now.x, now.y, now.z, now.w};
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i)
-                if (g + 32 * i < z) raw[i] = view.fetch(g + 32 * i);
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (sizeof(T) == 2) nan2 = Pair<T>::max_nan(nan2, w[j]);
+            else nan1 = ptx::max_nan(nan1, __uint_as_float(w[j]));
+        }
+        if (!__any_sync(0xffffffffu, bits != 0)) continue;
+        finite += __popc(bits);
+        some |= bits;
+        float best, least = INFINITY;  // of this vector's valid tokens
+        if constexpr (sizeof(T) == 2) {  // two tokens per instruction; hidden ones become -inf (for the minimum +inf)
+            const uint32_t lo = (bits & 0xfu) * 0x10204080u, hi = (bits >> 4) * 0x10204080u;
+            uint32_t top2 = Pair<T>::kInf ^ 0x80008000u, min2 = Pair<T>::kInf;
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) b[i] = g + 32 * i < z ? view.bits(g + 32 * i) : 0u;
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t keep = ptx::prmt(j < 2 ? lo : hi, 0u, j & 1 ? 0xBBAAu : 0x9988u);
+                top2 = Pair<T>::max(top2, ptx::select_bits(w[j], keep, Pair<T>::kInf ^ 0x80008000u));
+                min2 = Pair<T>::min(min2, ptx::select_bits(w[j], keep, Pair<T>::kInf));
+            }
+            max2 = Pair<T>::max(max2, top2);
+            best = fmaxf(Pair<T>::lo(top2), Pair<T>::hi(top2));
+            least = fminf(Pair<T>::lo(min2), Pair<T>::hi(min2));
+        } else {
+            float m[kVec];
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                if (g + 32 * i >= z) break;
-                valid += __popc(b[i]);
-                if constexpr (sizeof(T) == 2) {  // two tokens per instruction; hidden ones become -inf (for the minimum +inf)
-                    const uint32_t lo = (b[i] & 0xfu) * 0x10204080u, hi = (b[i] >> 4) * 0x10204080u;
-                    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t keep = ptx::prmt(j < 2 ? lo : hi, 0u, j & 1 ? 0xBBAAu : 0x9988u);
-                        nan2 = Pair<T>::max_nan(nan2, w[j]);
-                        max2 = Pair<T>::max(max2, ptx::select_bits(w[j], keep, Pair<T>::kInf ^ 0x80008000u));
-                        min2 = Pair<T>::min(min2, ptx::select_bits(w[j], keep, Pair<T>::kInf));
-                    }
-                } else {
-                    float x[kVec];
-                    view.expand(raw[i], x);
-#pragma unroll
-                    for (int j = 0; j < kVec; ++j) {
-                        const bool in = (b[i] >> j) & 1;
-                        nan1 = ptx::max_nan(nan1, x[j]);
-                        st.max = fmaxf(st.max, in ? x[j] : -INFINITY);
-                        min1 = fminf(min1, in ? x[j] : INFINITY);
-                    }
-                }
+            for (int j = 0; j < kVec; ++j) {
+                const bool in = (bits >> j) & 1;
+                m[j] = in ? __uint_as_float(w[j]) : -INFINITY;
+                least = fminf(least, in ? __uint_as_float(w[j]) : INFINITY);
+            }
+            const float a = fmaxf(m[0], m[1]), o = fmaxf(m[2], m[3]);
+            max_a = fmaxf(max_a, a), max_b = fmaxf(max_b, o);
+            best = fmaxf(a, o);
+        }
+        if (__any_sync(0xffffffffu, least == -INFINITY)) finite -= __popc(bits & ~reaching<T>(now, bits, -FLT_MAX));  // valid, never drawn
+        if (fill <= kSegment && __any_sync(0xffffffffu, best >= low)) {
+            // No room for a whole round: drop what the bound has passed.  What stays full is given up.
+            if (fill + 32 * kVec > kSegment && mode) fill = filter(segment, fill, low);
+            append<T>(segment, fill, reaching<T>(now, bits, low), stream, view.first(stream.g));
+            if (mode) {
+                if constexpr (sizeof(T) == 2) max_a = Pair<T>::lo(max2), max_b = Pair<T>::hi(max2);
+                const float lane_bound = fmaxf(max_a, max_b);
+                const uint32_t o = order_bits(lane_bound);
+                low = mode == 1 ? order_value(__reduce_min_sync(0xffffffffu, o)) : __fsub_rd(order_value(__reduce_max_sync(0xffffffffu, o)), drop);
+                low = fmaxf(low, -FLT_MAX);
             }
         }
-        if constexpr (sizeof(T) == 2) {
-            st.max = fmaxf(Pair<T>::lo(max2), Pair<T>::hi(max2));
-            min1 = fminf(Pair<T>::lo(min2), Pair<T>::hi(min2));
-            nan1 = ptx::max_nan(Pair<T>::lo(nan2), Pair<T>::hi(nan2));
-        }
-        const int32_t t = view.edge(g0, g1);
-        if (t >= 0) {
-            const float x = widen(view.row[t]);
-            nan1 = ptx::max_nan(nan1, x);
-            if (view.valid(t)) st.max = fmaxf(st.max, x), min1 = fminf(min1, x), ++valid;
-        }
-        st.finite = valid;
-        st.flags = (nan1 != nan1 ? 1u : 0u) | (valid ? 2u : 0u) | (min1 == -INFINITY ? 4u : 0u);
-        float m = st.max;
-        st.low[2] = m;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-            if (d == 4) st.low[1] = m;
-        }
-        st.low[0] = st.max = m;
-#pragma unroll
-        for (int d = 16; d; d >>= 1) {
-            st.low[1] = fminf(st.low[1], __shfl_xor_sync(0xffffffffu, st.low[1], d));
-            st.low[2] = fminf(st.low[2], __shfl_xor_sync(0xffffffffu, st.low[2], d));
-            st.finite += __shfl_xor_sync(0xffffffffu, st.finite, d);
-            st.flags |= __shfl_xor_sync(0xffffffffu, st.flags, d);
-        }
     }
-    RowStats* warp_stats = sh.warp_stats;
-    if (lane == 0) warp_stats[warp] = st;
-    if (threadIdx.x == 0) sh.list_count = 0;
+    if (fill <= kSegment) append_edge(view, segment, fill, low, g0, g1, false);
+    if constexpr (sizeof(T) == 2) {
+        max_a = Pair<T>::lo(max2), max_b = Pair<T>::hi(max2);
+        nan1 = ptx::max_nan(Pair<T>::lo(nan2), Pair<T>::hi(nan2));
+    }
+    RowStats st{-INFINITY, fminf(max_a, max_b), 0, 0};
+    st.max = fmaxf(max_a, max_b);
+    const int32_t t = view.edge(g0, g1);
+    if (t >= 0) {
+        const float x = widen(view.row[t]);
+        nan1 = ptx::max_nan(nan1, x);
+        if (view.valid(t)) st.max = fmaxf(st.max, x), some = 1, finite += x > -INFINITY;
+    }
+    st.finite = finite;
+    st.flags = (nan1 != nan1 ? 1u : 0u) | (some ? 2u : 0u);
+    float m = st.max;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        if (d == 4 && (lane & 7) == 0)
+            for (int i = 0; i < c; ++i) cluster.map_shared_rank(sh.group_max, i)[(rank * kWarps + warp) * 4 + lane / 8] = m;
+    }
+    st.max = m;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+        st.low = fminf(st.low, __shfl_xor_sync(0xffffffffu, st.low, d));
+        st.finite += __shfl_xor_sync(0xffffffffu, st.finite, d);
+        st.flags |= __shfl_xor_sync(0xffffffffu, st.flags, d);
+    }
+    if (fill > kSegment) st.flags |= 4;
+    if (lane == 0) sh.warp_stats[warp] = st, sh.fills[warp] = fill;
     __syncthreads();
     if (threadIdx.x < c) {
-        RowStats a = warp_stats[0];
-        for (int w = 1; w < kWarps; ++w) merge(a, warp_stats[w]);
+        RowStats a = sh.warp_stats[0];
+        for (int w = 1; w < kWarps; ++w) merge(a, sh.warp_stats[w]);
         *cluster.map_shared_rank(&sh.stats[rank], threadIdx.x) = a;
     }
     cluster.sync();
@@ -702,75 +857,14 @@ __device__ __noinline__ RowStats first_pass(Shared& sh, const RowView<T>& shared
     return st;
 }
 
-// Collects the keys of the tokens with x >= low into rank 0's list, in token order; returns their number in the whole
-// row, or more than kCap where a warp's segment or the list overflowed.
-template <typename T>
-__device__ __noinline__ uint32_t collect(Shared& sh, const RowView<T>& shared_view, float low) {
+// The segments' tokens with x >= low into rank 0's list, in token order; returns their number in the whole row, or more
+// than kCap where the list overflowed.  Every warp's segment is whole.
+__device__ __noinline__ uint32_t gather(Shared& sh, float low) {
     cg::cluster_group cluster = cg::this_cluster();
-    const RowView<T> view = shared_view;
     const int c = cluster.num_blocks(), rank = cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int32_t g0 = sh.bounds[warp], g1 = sh.bounds[warp + 1];
-    constexpr int kVec = RowView<T>::kVec, kBatch = 6;
-    const uint32_t below = (1u << lane) - 1u;
-    uint32_t fill = 0;
     uint64_t* segment = sh.segment[warp];
-    auto append = [&](uint32_t in, int32_t t, const float (&x)[kVec]) {  // this lane's consecutive tokens
-        uint32_t at = __popc(in), run = at;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const uint32_t up = __shfl_up_sync(0xffffffffu, run, d);
-            if (lane >= d) run += up;
-        }
-        at = fill + run - at;
-#pragma unroll
-        for (int j = 0; j < kVec; ++j)
-            if ((in >> j) & 1) {
-                if (at < kSegment) segment[at] = order_key(x[j], static_cast<uint32_t>(t + j));
-                ++at;
-            }
-        fill += __shfl_sync(0xffffffffu, run, 31);
-    };
-    auto edge = [&](bool front) {
-        const int32_t t = view.edge(g0, g1);
-        const float x = t >= 0 && (lane < kVec) == front && view.valid(t) ? widen(view.row[t]) : -INFINITY;
-        const bool in = x >= low;
-        const uint32_t who = __ballot_sync(0xffffffffu, in);
-        const uint32_t at = fill + __popc(who & below);
-        if (in && at < kSegment) segment[at] = order_key(x, static_cast<uint32_t>(t));
-        fill += __popc(who);
-    };
-    __syncthreads();  // the segments' space had other uses
-    edge(true);
-    const int32_t z = min(g1, view.full1);
-    for (int32_t g = max(g0, view.full0); g < z; g += 32 * kBatch) {
-        uint32_t b[kBatch];
-        uint4 raw[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) b[i] = g + 32 * i + lane < z ? view.bits(g + 32 * i + lane) : 0u;
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-            if (b[i]) raw[i] = view.fetch(g + 32 * i + lane);
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            float x[kVec];
-            uint32_t in = 0;
-            if (b[i]) {
-                view.expand(raw[i], x);
-                float m = x[0];
-#pragma unroll
-                for (int j = 1; j < kVec; ++j) m = fmaxf(m, x[j]);
-                if (m >= low) {
-#pragma unroll
-                    for (int j = 0; j < kVec; ++j) in |= static_cast<uint32_t>(x[j] >= low) << j;
-                    in &= b[i];
-                }
-            }
-            if (__any_sync(0xffffffffu, in != 0)) append(in, view.first(g + 32 * i + lane), x);
-        }
-    }
-    edge(false);
-    const uint32_t reported = fill <= kSegment ? fill : kCap + 1;
-    if (lane < c) *cluster.map_shared_rank(&sh.warp_counts[rank * kWarps + warp], lane) = reported;
+    const uint32_t fill = filter(segment, sh.fills[warp], low);
+    if (lane < c) *cluster.map_shared_rank(&sh.warp_counts[rank * kWarps + warp], lane) = fill;
     cluster.sync();
     uint32_t before = 0, all = 0;
     for (int i = lane; i < c * kWarps; i += 32) {
@@ -788,20 +882,78 @@ __device__ __noinline__ uint32_t collect(Shared& sh, const RowView<T>& shared_vi
     return all;
 }
 
-// Counts of the tokens up to sh.first_k by value bins of width sh.width below the maximum, in sh.merged (a token further
-// down is in the last bin), the same in every CTA.
+// A score that at least k tokens reach, close to the k-th: the k-th largest of the maxima of disjoint groups of lanes,
+// whole warps' where these are enough (about -G ln(1 - k / G) tokens reach the k-th of G), else of 8 lanes (at most
+// kThreads of them in the cluster).
+__device__ __noinline__ float kth_maximum(Shared& sh, int k, int c) {
+    const int n = 4 * kWarps * c, step = k * 5 <= 4 * kWarps * c ? 4 : 1, i = threadIdx.x;
+    float mine = -INFINITY;
+    if (i < n && i % step == 0)
+        for (int j = 0; j < step; ++j) mine = fmaxf(mine, sh.group_max[i + j]);
+    __syncthreads();
+    if (i < n && i % step == 0) sh.group_max[i] = mine;
+    if (i == 0) sh.low_bits = 0;
+    __syncthreads();
+    int ahead = 0;
+    if (i < n && i % step == 0)
+#pragma unroll 4
+        for (int j = 0; j < n; j += step) ahead += sh.group_max[j] > mine || (sh.group_max[j] == mine && j < i);
+    if (i < n && i % step == 0 && ahead == k - 1) sh.low_bits = order_bits(mine);
+    __syncthreads();
+    return sh.low_bits ? order_value(sh.low_bits) : -INFINITY;
+}
+
+// A pass that collects the tokens with x >= low into rank 0's list, in token order; returns as gather does, or more
+// than kCap where a segment overflowed.
 template <typename T>
-__device__ __noinline__ void count_bins(Shared& sh, const RowView<T>& shared_view, uint32_t* queue) {
+__device__ __noinline__ uint32_t collect(Shared& sh, const RowView<T>& shared_view, float low) {
     cg::cluster_group cluster = cg::this_cluster();
     const RowView<T> view = shared_view;
-    const int c = cluster.num_blocks(), warp = threadIdx.x >> 5;
+    const int c = cluster.num_blocks(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int32_t g0 = sh.bounds[warp], g1 = sh.bounds[warp + 1];
+    constexpr int kVec = RowView<T>::kVec;
+    uint32_t fill = 0;
+    uint64_t* segment = sh.segment[warp];
+    __syncthreads();  // the segments' space had other uses
+    append_edge(view, segment, fill, low, g0, g1, true);
+#pragma unroll 1
+    for (Stream<T> stream(view, sh.first_ring[warp], g0, g1); stream.more(); stream.next()) {
+        uint4 now;
+        const uint32_t bits = stream.take(now);
+        float best = -INFINITY;
+        if (bits) {
+            float x[kVec];
+            view.expand(now, x);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) best = fmaxf(best, x[j]);
+        }
+        if (__any_sync(0xffffffffu, best >= low)) append<T>(segment, fill, bits ? reaching<T>(now, bits, low) : 0u, stream, view.first(stream.g));
+    }
+    append_edge(view, segment, fill, low, g0, g1, false);
+    if (lane == 0) sh.fills[warp] = min(fill, static_cast<uint32_t>(kSegment));
+    const int over = __syncthreads_or(fill > kSegment);
+    if (threadIdx.x < c) *cluster.map_shared_rank(&sh.list_counts[cluster.block_rank()], threadIdx.x) = over;
+    cluster.sync();
+    uint32_t any = 0;
+    for (int i = 0; i < c; ++i) any |= sh.list_counts[i];
+    const uint32_t n = gather(sh, low);
+    return any ? kCap + 1 : n;
+}
+
+// Counts of the tokens up to sh.first_k by value bins of width sh.width below the maximum, in sh.merged (a token further
+// down is in the last bin), the same in every CTA.
+template <typename T, bool kEnd>
+__device__ __noinline__ void count_bins_to(Shared& sh, const RowView<T>& shared_view) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const RowView<T> view = shared_view;
+    const int c = cluster.num_blocks();
     const Place end = place_of(sh.first_k);
     __syncthreads();
     for (int i = threadIdx.x; i < kBins; i += kThreads) sh.bins[i] = 0;
     __syncthreads();
     const float at = sh.bin_at, scale = sh.bin_scale;
-    each_token(view, sh.bounds[warp], sh.bounds[warp + 1], queue, [&](float x, uint32_t t, bool live) {
-        if (live && end.keeps(x, t)) atomicAdd(&sh.bins[bin_of(x, at, scale)], 1u);
+    each_token(sh, view, [&](float x, uint32_t t, bool live) {
+        if (live && (!kEnd || end.keeps(x, t))) atomicAdd(&sh.bins[bin_of(x, at, scale)], 1u);
     });
     cluster.sync();
     for (int i = threadIdx.x; i < kBins; i += kThreads) {
@@ -810,6 +962,12 @@ __device__ __noinline__ void count_bins(Shared& sh, const RowView<T>& shared_vie
         sh.merged[i] = n;
     }
     cluster.sync();
+}
+
+template <typename T>
+__device__ __forceinline__ void count_bins(Shared& sh, const RowView<T>& view) {
+    if (place_of(sh.first_k).x > -INFINITY) count_bins_to<T, true>(sh, view);
+    else count_bins_to<T, false>(sh, view);
 }
 
 // Moves every CTA's sh.list (sh.list_count keys, in no order) behind rank 0's; returns their number.
@@ -834,14 +992,13 @@ __device__ __noinline__ uint32_t pool(Shared& sh) {
 
 // The keys of bin b's tokens into sh.list (no order).
 template <typename T>
-__device__ __noinline__ void collect_bin(Shared& sh, const RowView<T>& shared_view, uint32_t* queue, int b) {
+__device__ __noinline__ void collect_bin(Shared& sh, const RowView<T>& shared_view, int b) {
     const RowView<T> view = shared_view;
-    const int warp = threadIdx.x >> 5;
     __syncthreads();
     if (threadIdx.x == 0) sh.list_count = 0;
     __syncthreads();
     const float at = sh.bin_at, scale = sh.bin_scale;
-    each_token(view, sh.bounds[warp], sh.bounds[warp + 1], queue, [&](float x, uint32_t t, bool live) {
+    each_token(sh, view, [&](float x, uint32_t t, bool live) {
         if (live && bin_of(x, at, scale) == b) sh.list[atomicAdd(&sh.list_count, 1u)] = order_key(x, t);
     });
 }
@@ -849,8 +1006,8 @@ __device__ __noinline__ void collect_bin(Shared& sh, const RowView<T>& shared_vi
 // The weighing pass around the bracket [sh.b0, sh.b1] of bins, among the tokens up to sh.first_k: masses above and below
 // it and the number of kept tokens above it to rank 0 (sh.above, sh.below, sh.counts, sh.spans), the bracket's keys
 // into sh.list.
-template <typename T>
-__device__ __noinline__ void weigh_bracket(Shared& sh, const RowView<T>& shared_view, uint32_t* queue) {
+template <typename T, bool kEnd, bool kFloor>
+__device__ __noinline__ void weigh_bracket_to(Shared& sh, const RowView<T>& shared_view) {
     cg::cluster_group cluster = cg::this_cluster();
     const RowView<T> view = shared_view;
     const int rank = cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -860,8 +1017,8 @@ __device__ __noinline__ void weigh_bracket(Shared& sh, const RowView<T>& shared_
     const float at = sh.bin_at, scale = sh.bin_scale, floor_x = sh.floor_x;
     double above = 0.0, below = 0.0, kept_above = 0.0;
     int count = 0;
-    each_token(view, sh.bounds[warp], sh.bounds[warp + 1], queue, [&](float x, uint32_t t, bool live) {
-        if (!live || !end.keeps(x, t)) return;
+    each_token(sh, view, [&](float x, uint32_t t, bool live) {
+        if (!live || (kEnd && !end.keeps(x, t))) return;
         const int bin = bin_of(x, at, scale);
         if (bin >= b0 && bin <= b1) {
             sh.list[atomicAdd(&sh.list_count, 1u)] = order_key(x, t);
@@ -870,8 +1027,10 @@ __device__ __noinline__ void weigh_bracket(Shared& sh, const RowView<T>& shared_
         const double w = weight_of(x, top, rate, sh.exp_table);
         if (bin > b1) below += w;
         else above += w;
-        if (bin < b0 && x >= floor_x) kept_above += w, ++count;
+        if (kFloor && bin < b0 && x >= floor_x) kept_above += w;
+        count += bin < b0 && (!kFloor || x >= floor_x);
     });
+    if (!kFloor) kept_above = above;
     above = warp_sum(above), below = warp_sum(below), kept_above = warp_sum(kept_above);
     count = __reduce_add_sync(0xffffffffu, count);
     if (lane == 0) {
@@ -889,17 +1048,24 @@ __device__ __noinline__ void weigh_bracket(Shared& sh, const RowView<T>& shared_
     }
 }
 
-// Mass of the tokens up to `end` by spans, and their number, to rank 0.
 template <typename T>
-__device__ __noinline__ void weigh_spans(Shared& sh, const RowView<T>& shared_view, uint32_t* queue, Place end) {
+__device__ __forceinline__ void weigh_bracket(Shared& sh, const RowView<T>& view) {
+    const bool end = place_of(sh.first_k).x > -INFINITY, floor = sh.floor_x > -INFINITY;
+    if (end) floor ? weigh_bracket_to<T, true, true>(sh, view) : weigh_bracket_to<T, true, false>(sh, view);
+    else floor ? weigh_bracket_to<T, false, true>(sh, view) : weigh_bracket_to<T, false, false>(sh, view);
+}
+
+// Mass of the tokens up to `end` by spans, and their number, to rank 0.
+template <typename T, bool kEnd>
+__device__ __noinline__ void weigh_spans(Shared& sh, const RowView<T>& shared_view, Place end) {
     cg::cluster_group cluster = cg::this_cluster();
     const RowView<T> view = shared_view;
     const int rank = cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const double top = sh.top, rate = sh.rate;
     double mass = 0.0;
     int count = 0;
-    each_token(view, sh.bounds[warp], sh.bounds[warp + 1], queue, [&](float x, uint32_t t, bool live) {
-        if (live && end.keeps(x, t)) mass += weight_of(x, top, rate, sh.exp_table), ++count;
+    each_token(sh, view, [&](float x, uint32_t t, bool live) {
+        if (live && (!kEnd || end.keeps(x, t))) mass += weight_of(x, top, rate, sh.exp_table), ++count;
     });
     mass = warp_sum(mass);
     count = __reduce_add_sync(0xffffffffu, count);
@@ -920,18 +1086,18 @@ __device__ __noinline__ void weigh_spans(Shared& sh, const RowView<T>& shared_vi
 // The nucleus: the place where it ends in sh.cut and the kept masses by spans on rank 0, or false where the estimate
 // or the list does not serve.
 template <typename T>
-__device__ __noinline__ bool find_nucleus(Shared& sh, const RowView<T>& shared_view, uint32_t* queue, int64_t* kept_out, int32_t* status_out) {
+__device__ __noinline__ bool find_nucleus(Shared& sh, const RowView<T>& shared_view, int64_t* kept_out, int32_t* status_out) {
     cg::cluster_group cluster = cg::this_cluster();
     const int c = cluster.num_blocks(), rank = cluster.block_rank(), lane = threadIdx.x & 31;
     const int64_t groups = shared_view.groups;
     // Where the nucleus ends, by the bins' counts and middle weights.  The estimate is good to about a part
     // in a thousand of the mass; a miss tells the exact masses around the bracket, which place the next one.
-    count_bins<T>(sh, shared_view, queue);
+    count_bins<T>(sh, shared_view);
     const float step = sh.width * static_cast<float>(sh.rate / kTable);  // log2 of the weights' ratio from bin to bin
     float mine = 0.f, all;
     for (int i = 0; i < kPerThread; ++i) {
         const int at = threadIdx.x * kPerThread + i;
-        mine += sh.merged[at] * exp2f(-(at + 0.5f) * step);
+        mine += sh.merged[at] * exp2f(-at * step);
     }
     const float run = block_before(mine, reinterpret_cast<float*>(sh.warp_mass), all);
     float goal = static_cast<float>(sh.top_p) * all, slack = 1e-3f;
@@ -947,7 +1113,7 @@ __device__ __noinline__ bool find_nucleus(Shared& sh, const RowView<T>& shared_v
                 float before = run;
                 int i = threadIdx.x * kPerThread;
                 for (const int last = i + kPerThread - 1; i < last; ++i) {
-                    const float m = sh.merged[i] * exp2f(-(i + 0.5f) * step);
+                    const float m = sh.merged[i] * exp2f(-i * step);
                     if (before + m >= want) break;
                     before += m;
                 }
@@ -966,7 +1132,7 @@ __device__ __noinline__ bool find_nucleus(Shared& sh, const RowView<T>& shared_v
         if (inside > kCap || inside == 0) break;
         if (threadIdx.x == 0) sh.b0 = b0, sh.b1 = b1;
         __syncthreads();
-        weigh_bracket<T>(sh, shared_view, queue);
+        weigh_bracket<T>(sh, shared_view);
         const uint32_t n = pool(sh);
         if (rank == 0) {
             double above = 0.0, below = 0.0;
@@ -1018,11 +1184,11 @@ __device__ __noinline__ bool find_nucleus(Shared& sh, const RowView<T>& shared_v
         found = sh.found;
         if (!found) {  // the same correction from the estimated mass at the bracket's edge
             const float off = sh.goal;
-            __syncthreads();
+            count_bins<T>(sh, shared_view);  // the list has taken the counts' place
             const int edge = off <= 0.f ? b0 : b1 + 1;
             if (edge / kPerThread == threadIdx.x) {
                 float e = run;
-                for (int i = threadIdx.x * kPerThread; i < edge; ++i) e += sh.merged[i] * exp2f(-(i + 0.5f) * step);
+                for (int i = threadIdx.x * kPerThread; i < edge; ++i) e += sh.merged[i] * exp2f(-i * step);
                 sh.goal = e + off;
             }
             __syncthreads();
@@ -1132,15 +1298,15 @@ __global__ void __launch_bounds__(kThreads, 2) filter_sample_kernel(const Filter
         const int64_t g = view.groups, c0 = g * rank / c, slice = g * (rank + 1) / c - c0;
         for (int w = 0; w <= kWarps; ++w) sh.bounds[w] = static_cast<int32_t>(c0 + slice * w / kWarps);
     }
-    uint32_t* queue = sh.queue[warp];
     static_assert(2 * kQueue<float> >= kQueue<__half>, "queue space");
     __syncthreads();
 
-    RowStats st = first_pass<T>(sh, view);
+    // What the first pass can keep: see there.  (A greedy row keeps nothing that is used.)
+    const int mode = top_k > 0 && top_k <= 32 ? 1 : min_p > 0.0 && top_p >= 1.0 ? 2 : 0;
+    const float drop = mode == 2 ? __double2float_ru(-temp * (log(min_p) - 1e-6)) : 0.f;
+    RowStats st = first_pass<T>(sh, view, mode, drop);
     const bool greedy = temp == 0.0;
     int turn = 0;
-    if (!greedy && (st.flags & 5) == 4)  // scores of -inf are valid but never drawn: count the others
-        st.finite = static_cast<uint32_t>(sum_above<T>(sh, view, queue, 0, 0, false, turn).count);
     if (st.flags & 1) code = BMS_STATUS_NAN;
     else if (!greedy && st.max == INFINITY) code = BMS_STATUS_POS_INF;
     else if (!(st.flags & 2)) code = BMS_STATUS_EMPTY;
@@ -1191,19 +1357,20 @@ __global__ void __launch_bounds__(kThreads, 2) filter_sample_kernel(const Filter
         }
     };
 
-    // The tokens that can be kept, where a bound is known without another pass.
-    float low = INFINITY;
-    if (st.finite <= kCap) low = -FLT_MAX;
-    else if (k_cuts && k <= kThreads * c) low = k <= kWarps * c ? st.low[0] : k <= 4 * kWarps * c ? st.low[1] : st.low[2];
-    else if (!k_cuts && min_p > 0.0 && top_p >= 1.0) low = fmaxf(sh.floor_x, -FLT_MAX);
-    if (low > -INFINITY && low < INFINITY) {
-        const uint32_t n = collect<T>(sh, view, low);
+    // The tokens that can be kept, where a bound is known: the first pass has them, or another pass collects them.
+    float low = -INFINITY;
+    if (k_cuts) low = k * 5 <= 4 * 4 * kWarps * c && 4 * kWarps * c <= kThreads ? kth_maximum(sh, static_cast<int>(k), c) : k <= 2 * kThreads * c ? st.low : -INFINITY;
+    else if (top_p >= 1.0) low = sh.floor_x;
+    const bool have = !(st.flags & 4) && (mode != 0 || st.finite <= kCap || low > -INFINITY);
+    if (have || st.finite <= kCap || low > -INFINITY) {
+        low = fmaxf(low, -FLT_MAX);
+        const uint32_t n = have ? gather(sh, low) : collect<T>(sh, view, low);
         if (n <= kCap) return from_list(n);
     }
 
     // End of the first k tokens: exact counts find the bin that holds rank k; its tokens, sorted, give the place.
     if (k_cuts) {
-        count_bins<T>(sh, view, queue);
+        count_bins<T>(sh, view);
         uint32_t mine = 0, all;
         for (int i = 0; i < kPerThread; ++i) mine += sh.merged[threadIdx.x * kPerThread + i];
         uint32_t run = block_before(mine, reinterpret_cast<uint32_t*>(sh.warp_mass), all);
@@ -1225,7 +1392,7 @@ __global__ void __launch_bounds__(kThreads, 2) filter_sample_kernel(const Filter
             }
         }
         if (inside <= kCap) {
-            collect_bin<T>(sh, view, queue, bin);
+            collect_bin<T>(sh, view, bin);
             const uint32_t n = pool(sh);
             if (rank == 0) {
                 int kept;
@@ -1235,7 +1402,7 @@ __global__ void __launch_bounds__(kThreads, 2) filter_sample_kernel(const Filter
             }
             cluster.sync();
         } else {
-            const uint64_t key = bisect<T>(sh, view, queue, 0, static_cast<double>(k), false, turn);
+            const uint64_t key = bisect<T>(sh, view, 0, static_cast<double>(k), false, turn);
             if (threadIdx.x == 0) sh.cut = key;
         }
         __syncthreads();
@@ -1245,10 +1412,10 @@ __global__ void __launch_bounds__(kThreads, 2) filter_sample_kernel(const Filter
     uint64_t cut = sh.first_k;
     bool have_spans = false;
     if (top_p < 1.0) {
-        have_spans = find_nucleus<T>(sh, view, queue, &p.kept[r], &p.status[r]);
+        have_spans = find_nucleus<T>(sh, view, &p.kept[r], &p.status[r]);
         if (!have_spans) {
-            const double limit = top_p * sum_above<T>(sh, view, queue, 0, cut, true, turn).mass;
-            cut = bisect<T>(sh, view, queue, cut, limit, true, turn);
+            const double limit = top_p * sum_above<T>(sh, view, 0, cut, true, turn).mass;
+            cut = bisect<T>(sh, view, cut, limit, true, turn);
         } else {
             cut = max(cut, sh.cut);
         }
@@ -1257,7 +1424,8 @@ __global__ void __launch_bounds__(kThreads, 2) filter_sample_kernel(const Filter
     const Place end = place_of(max(cut, static_cast<uint64_t>(order_bits(sh.floor_x)) << 32));
     // Kept masses by spans, unless the nucleus left them; rank 0 finds the span that holds the target.
     if (!have_spans) {
-        weigh_spans<T>(sh, view, queue, end);
+        if (end.x > -INFINITY) weigh_spans<T, true>(sh, view, end);
+        else weigh_spans<T, false>(sh, view, end);
         if (rank == 0 && threadIdx.x == 0) {
             int64_t all = 0;
             for (int i = 0; i < c; ++i) all += sh.counts[i];
@@ -1310,9 +1478,11 @@ int launch_filter(const FilterParams& p, int device, cudaStream_t stream) {
         BMS_CUDA(cudaDeviceGetAttribute(&sms[device], cudaDevAttrMultiProcessorCount, device), "sm count");
         ready[device] = true;
     }
-    int c = 1;
-    while (c < 8 && p.rows * c * 2 <= sms[device] && p.vocab / (2 * c) >= 4096) c *= 2;
-    if (getenv("FC")) c = atoi(getenv("FC"));
+    // CTAs per row.  Few rows are split for latency (8 rows of 248,320: 74 / 41 / 30 / 26 us with 1 / 2 / 4 / 8); up to two rows per SM,
+    // 4 keep one slow row (a wide nucleus) from ending the launch alone (256 mixed rows: 342 / 243 / 231 / 294 us); many rows keep the
+    // SMs busy by themselves (1,152 rows: 1.15 / 1.17 / 1.42 ms with 1 / 2 / 4).
+    int c = p.rows * 8 <= sms[device] ? 8 : p.rows <= 2 * sms[device] ? 4 : p.rows <= 4 * sms[device] ? 2 : 1;
+    while (c > 1 && p.vocab / c < 4096) c /= 2;
     if (p.rows * c > 2147483647LL) return fail(BMS_ERROR_UNSUPPORTED, "too many rows");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(p.rows * c));
