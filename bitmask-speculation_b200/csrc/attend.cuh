@@ -46,11 +46,9 @@ struct Layout {
 
 struct Control {
     uint64_t full[12], empty[12];
-    uint64_t q_full, s_full[2], p_full[2], o_full[2];
+    uint64_t q_full, s_full[2], p_full[2][2], o_full[2];
     float ref[kTile], sum[kTile];
-    int64_t scan[kThreads / 32];
-    int64_t total, start_off;
-    int32_t start_seq;
+    int32_t item_tiles[2], item_wide[2];  // of the item whose queries are in place, by the item's parity; 0 tiles: no more
     uint32_t tmem, poison, abort;
 };
 
@@ -62,6 +60,7 @@ struct Params {
     float scale2;      // |scale| log2(e)
     uint32_t negate;   // sign bits for queries of a negative scale
     int32_t group, tile_tokens;
+    int32_t group_inv;  // 65536 / group, rounded up: r / group = r * group_inv >> 16 for rows r < 128
 };
 
 // ---- schedule ---------------------------------------------------------------------------------
@@ -102,18 +101,24 @@ __device__ __forceinline__ bool lengths_fit(const AttendParams& a, int s) {
     return x >= 0 && y >= x && y <= a.tokens && len >= y - x && len <= static_cast<int64_t>(a.width) * a.page_size;
 }
 
+// A sequence without its total.
 __device__ __forceinline__ Shape sequence_shape(const Params& p, int s) {
     Shape h{0, 0, 0, 0, false};
     if (!lengths_fit(p.a, s)) return h;
     h.n = p.a.query_start[s + 1] - p.a.query_start[s];
-    if (h.n == 0) return h;
     h.past = p.a.seq_lens[s] - h.n;
     h.wide = h.n > p.tile_tokens;
     const int32_t per = h.wide ? 2 * p.tile_tokens : p.tile_tokens;
     h.tiles = (h.n + per - 1) / per;
-    for (int q = 0; q < h.tiles; ++q) h.total += query_range(p, h.n, h.past, h.wide, q).steps;
     return h;
 }
+
+// Where a part of the line of steps starts.
+struct Start {
+    int64_t total, off;  // all steps; the part's first step within its sequence
+    int32_t seq;
+    Shape shape;
+};
 
 // Walks the items of a CTA's part of the line of steps.
 struct Walk {
@@ -122,11 +127,12 @@ struct Walk {
     int32_t st0, st1;   // steps of the current item that belong to the part
     Shape shape;
     Range range;
-    __device__ __forceinline__ void start(const Params& p, int seq, int64_t off, int64_t count) {
-        s = seq, left = count;
+    __device__ __forceinline__ void start(const Params& p, const Start& at, int64_t count) {
+        s = at.seq, left = count;
         head = qt = st0 = 0;
         if (count <= 0) return;
-        shape = sequence_shape(p, s);
+        shape = at.shape;
+        const int64_t off = at.off;
         head = static_cast<int32_t>(off / shape.total);
         int64_t rest = off % shape.total;
         for (;; ++qt) {
@@ -150,7 +156,7 @@ struct Walk {
             if (++head == p.a.kv_heads) {
                 head = 0;
                 do shape = sequence_shape(p, ++s);
-                while (shape.total == 0);
+                while (shape.n == 0);
             }
         }
         range = query_range(p, shape.n, shape.past, shape.wide, qt);
@@ -160,36 +166,66 @@ struct Walk {
     __device__ __forceinline__ bool whole() const { return st0 == 0 && st1 == range.steps; }
 };
 
-// Total steps, and the sequence and offset at which part `c` of `parts` starts.  All threads of the block take part.
+// Finds where part `c` of `ctas` starts.  All threads of the block take part; the sequences' totals come one per thread,
+// or, for prompts of many query tiles, one per warp with the tiles over its lanes.
 template <int kBlock>
-__device__ void locate(const Params& p, int64_t* scan, int64_t& total, int64_t& off, int32_t& seq, int c, int ctas) {
+struct LocateSpace {
+    int64_t totals[kBlock], scan[kBlock / 32];
+    Start start;
+};
+
+template <int kBlock>
+__device__ void locate(const Params& p, LocateSpace<kBlock>& sp, int c, int ctas) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     constexpr int kW = kBlock / 32;
-    int64_t target = -1, run = 0;
+    const bool by_warp = p.a.tokens > 2LL * p.tile_tokens * p.a.seqs;
+    const bool once = p.a.seqs <= kBlock;  // one round: the second pass has the totals already
+    int64_t target = -1, mine = 0, v = 0;
     for (int pass = 0; pass < 2; ++pass) {
-        run = 0;
+        int64_t run = 0;
         for (int base = 0; base < p.a.seqs; base += kBlock) {
             const int s = base + threadIdx.x;
-            const int64_t mine = s < p.a.seqs ? sequence_shape(p, s).total * p.a.kv_heads : 0;
-            int64_t v = mine;
+            if (pass == 0 || !once) {
+                __syncthreads();
+                if (by_warp) {
+                    for (int i = warp; i < kBlock && base + i < p.a.seqs; i += kW) {
+                        const Shape h = sequence_shape(p, base + i);
+                        int t = 0;
+                        for (int q = lane; q < h.tiles; q += 32) t += query_range(p, h.n, h.past, h.wide, q).steps;
+                        t = __reduce_add_sync(0xffffffffu, t);
+                        if (lane == 0) sp.totals[i] = t;
+                    }
+                } else if (s < p.a.seqs) {
+                    const Shape h = sequence_shape(p, s);
+                    int64_t t = 0;
+                    for (int q = 0; q < h.tiles; ++q) t += query_range(p, h.n, h.past, h.wide, q).steps;
+                    sp.totals[threadIdx.x] = t;
+                }
+                __syncthreads();
+                mine = s < p.a.seqs ? sp.totals[threadIdx.x] * p.a.kv_heads : 0;
+                v = mine;
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int64_t up = __shfl_up_sync(0xffffffffu, v, d);
-                if (lane >= d) v += up;
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int64_t up = __shfl_up_sync(0xffffffffu, v, d);
+                    if (lane >= d) v += up;
+                }
+                if (lane == 31) sp.scan[warp] = v;
+                __syncthreads();
+                int64_t all = run;
+                for (int w = 0; w < kW; ++w) {
+                    if (w == warp) v += all;
+                    all += sp.scan[w];
+                }
+                run = all;
             }
-            __syncthreads();
-            if (lane == 31) scan[warp] = v;
-            __syncthreads();
-            int64_t all = run;
-            for (int w = 0; w < kW; ++w) {
-                if (w == warp) v += all;
-                all += scan[w];
+            if (pass == 1 && mine > 0 && target >= v - mine && target < v) {
+                sp.start.seq = s, sp.start.off = target - (v - mine);
+                sp.start.shape = sequence_shape(p, s);
+                sp.start.shape.total = mine / p.a.kv_heads;
             }
-            if (pass == 1 && mine > 0 && target >= v - mine && target < v) seq = s, off = target - (v - mine);
-            run = all;
         }
         if (pass == 0) {
-            if (threadIdx.x == 0) total = run, seq = -1, off = 0;
+            if (threadIdx.x == 0) sp.start.total = run;
             const int64_t parts = min(static_cast<int64_t>(ctas), run);
             target = c < parts ? run * c / parts : -1;
         }
@@ -210,16 +246,20 @@ __device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t cols) {
 __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+// Operand descriptors come as their low word and a high word that all operands of one layout share: an address step is one
+// 32-bit addition, and the issuing thread keeps few registers.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc, bool add) {
     asm volatile(
-        "{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-        "r"(static_cast<uint32_t>(add))
+        "{ .reg .pred p; .reg .b64 da, db; setp.ne.u32 p, %5, 0; mov.b64 da, {%1, %3}; mov.b64 db, {%2, %3};\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p; }" ::"r"(d),
+        "r"(a), "r"(b), "r"(high), "r"(idesc), "r"(static_cast<uint32_t>(add))
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc, bool add) {
     asm volatile(
-        "{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
-        "r"(static_cast<uint32_t>(add))
+        "{ .reg .pred p; .reg .b64 db; setp.ne.u32 p, %5, 0; mov.b64 db, {%2, %3};\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p; }" ::"r"(d),
+        "r"(a), "r"(b), "r"(high), "r"(idesc), "r"(static_cast<uint32_t>(add))
         : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
@@ -251,11 +291,10 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
 #undef BMS_R8
 #undef BMS_W8
 
-// Shared-memory operand with 128-byte swizzle: start address, leading and stride offsets in 16-byte units, version 1.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
-    return static_cast<uint64_t>((addr >> 4) & 0x3fff) | (static_cast<uint64_t>((lead >> 4) & 0x3fff) << 16) |
-           (static_cast<uint64_t>((stride >> 4) & 0x3fff) << 32) | (1ull << 46) | (2ull << 61);
-}
+// Shared-memory operand with 128-byte swizzle: start address and leading offset in the low word, stride offset, version 1
+// and the swizzle mode in the high one (addresses and offsets in units of 16 bytes).
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t lead) { return ((addr >> 4) & 0x3fff) | (lead >> 4) << 16; }
+constexpr uint32_t kDescHigh = (1024 >> 4) | (1u << 14) | (2u << 29);  // 8 rows of 128 bytes from group to group
 
 // float32 accumulator, 16-bit inputs (kind: 0 float16, 1 bfloat16), A K-major, B K- or MN-major, M = 128.
 __host__ __device__ constexpr uint32_t instr_desc(uint32_t kind, bool b_mn, uint32_t n) {
@@ -269,18 +308,17 @@ __device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, i
         : "memory");
 }
 
-// Waits at most about a second; after that the CTA's abort flag ends every wait at once.
+// Waits at most about a second; after that the CTA's abort flag ends every wait.
 __device__ __forceinline__ void wait_bar(Control& c, uint64_t* bar, uint32_t parity) {
     const uint32_t addr = ptx::smem_addr(bar);
-    if (ptx::mbar_try_wait(addr, parity)) return;
-    const uint64_t t0 = ptx::globaltimer();
     volatile uint32_t* abort = &c.abort;
-    while (!ptx::mbar_try_wait(addr, parity)) {
+    uint64_t t0 = 0;
+    for (uint32_t i = 0; !ptx::mbar_try_wait(addr, parity); ++i) {
+        if ((i & 63u) != 63u) continue;
         if (*abort) return;
-        if (ptx::globaltimer() - t0 > kWaitNs) {
-            *abort = 1;
-            return;
-        }
+        const uint64_t now = ptx::globaltimer();
+        if (t0 == 0) t0 = now;
+        else if (now - t0 > kWaitNs) *abort = 1;
     }
 }
 
@@ -356,7 +394,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         ptx::mbar_init(ptx::smem_addr(&ctl.q_full), 8);
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(ptx::smem_addr(&ctl.s_full[i]), 1);
-            ptx::mbar_init(ptx::smem_addr(&ctl.p_full[i]), 4);
+            ptx::mbar_init(ptx::smem_addr(&ctl.p_full[i][0]), 4), ptx::mbar_init(ptx::smem_addr(&ctl.p_full[i][1]), 4);
             ptx::mbar_init(ptx::smem_addr(&ctl.o_full[i]), 1);
         }
         ptx::fence_mbarrier_init();
@@ -364,49 +402,61 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     }
     if (warp == kMmaWarp) tmem_alloc(&ctl.tmem, 512);
     fence_before();
-    locate<kThreads>(p, ctl.scan, ctl.total, ctl.start_off, ctl.start_seq, blockIdx.x, gridDim.x);
-    __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");  // not before the wait: the dependent reads this call's inputs early
+    // The space of Q serves the search before the first item.
+    LocateSpace<kThreads>& located = *reinterpret_cast<LocateSpace<kThreads>*>(tiles_smem + (q_smem - ptx::smem_addr(tiles_smem)));
+    locate<kThreads>(p, located, blockIdx.x, gridDim.x);
     fence_after();
     const uint32_t tmem = ctl.tmem;
-    const int64_t begin = part_begin(ctl.total, blockIdx.x, gridDim.x), end = part_begin(ctl.total, blockIdx.x + 1, gridDim.x);
-    // Registers: launched with 168 a thread; 2 x 128 x 224 + 128 x 40 is below 384 x 168.  Each role sets its own
+    const Start start = located.start;
+    __syncthreads();  // everyone has it before Q comes in
+    const int64_t begin = part_begin(start.total, blockIdx.x, gridDim.x), end = part_begin(start.total, blockIdx.x + 1, gridDim.x);
+    // Registers: launched with 168 a thread; 2 x 128 x 232 + 128 x 40 is exactly 384 x 168.  Each role sets its own
     // share inside its branch: after a join the compiler would have to assume the smaller one.
     if (warp >= kProducerWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        Walk walk;
-        walk.start(p, ctl.start_seq, ctl.start_off, end - begin);
         if (warp == kProducerWarp) {
+            Walk walk;
+            walk.start(p, start, end - begin);
             uint32_t seq = 0;  // tiles loaded so far
-            auto load = [&](const CUtensorMap* map, int tile) {
+            // Lane i loads box i of a tile.  Its page index (-1: nothing to load) is fetched a tile ahead of its use.
+            const int32_t box = min(a.page_size, kTile);
+            auto page_of = [&](int tile) {
+                const int32_t key = walk.range.tile(tile) * kTile + lane * box;
+                bool mine = lane < kTile / box && key <= walk.range.pmax;
+                if (mine && a.window > 0) mine = key + box - 1 > walk.range.pmin - a.window || key < a.sinks;
+                int32_t page = mine ? a.table[static_cast<int64_t>(walk.s) * a.width + key / a.page_size] : -1;
+                return page < a.pages ? page : -1;  // attend_finish_kernel reports pages outside the cache
+            };
+            auto load = [&](const CUtensorMap* map, int tile, int32_t page) {
                 const uint32_t stage = seq % kStages, round = seq / kStages;
                 ++seq;
                 wait_bar(ctl, &ctl.empty[stage], (round & 1) ^ 1);
-                const int32_t key0 = walk.range.tile(tile) * kTile;
-                const int32_t box = min(a.page_size, kTile);
-                const int32_t key = key0 + lane * box;  // lane i loads the tile's box i
-                bool mine = lane < kTile / box && key <= walk.range.pmax;
-                if (mine && a.window > 0) mine = key + box - 1 > walk.range.pmin - a.window || key < a.sinks;
-                int32_t page = 0;
-                if (mine) {
-                    page = a.table[static_cast<int64_t>(walk.s) * a.width + key / a.page_size];
-                    mine = page >= 0 && page < a.pages;  // attend_finish_kernel reports the others
-                }
+                const bool mine = page >= 0;
                 const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, mine));
                 const uint32_t bar = ptx::smem_addr(&ctl.full[stage]);
                 if (lane == 0) ptx::mbar_arrive_expect_tx(bar, boxes * box * D * 2);
                 __syncwarp();
                 if (mine && !*static_cast<volatile uint32_t*>(&ctl.abort)) {
+                    const int32_t slot = (walk.range.tile(tile) * kTile + lane * box) % a.page_size;
                     const uint32_t dst = ring + stage * L::kTileBytes + lane * box * 128;
 #pragma unroll
-                    for (int half = 0; half < D / 64; ++half) tma_page(dst + half * (kTile * 128), map, half * 64, walk.head, key % a.page_size, page, bar);
+                    for (int half = 0; half < D / 64; ++half) tma_page(dst + half * (kTile * 128), map, half * 64, walk.head, slot, page, bar);
                 }
             };
             for (; walk.valid(); walk.next(p)) {
                 const int t0 = walk.tile0(), t1 = walk.tile1(), ahead = walk.shape.wide ? 1 : 2;
-                for (int t = t0; t < min(t0 + ahead, t1); ++t) load(&k_map, t);
+                auto fetch = [&](int t) { return t < t1 ? page_of(t) : -1; };
+                // Pages of tiles t, t + 1, t + 2: values trail their keys by `ahead` tiles.
+                int32_t pg0 = fetch(t0), pg1 = fetch(t0 + 1), pg2 = fetch(t0 + 2);
+                load(&k_map, t0, pg0);
+                if (ahead == 2 && t0 + 1 < t1) load(&k_map, t0 + 1, pg1);
                 for (int t = t0; t < t1; ++t) {
-                    load(&v_map, t);
-                    if (t + ahead < t1) load(&k_map, t + ahead);
+                    const int32_t pg3 = fetch(t + 3);
+                    load(&v_map, t, pg0);
+                    if (t + ahead < t1) load(&k_map, t + ahead, ahead == 1 ? pg1 : pg2);
+                    pg0 = pg1, pg1 = pg2, pg2 = pg3;
                 }
             }
             // After an abort copies may still be in flight: they land before the shared memory goes away.
@@ -419,114 +469,122 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         } else if (warp == kMmaWarp) {
             if (lane == 0) {
                 constexpr uint32_t s_desc = instr_desc(Kind<T>::code, false, kTile), o_desc = instr_desc(Kind<T>::code, true, D);
-                uint32_t seq = 0, item = 0, p_round[2] = {0, 0};
+                uint32_t seq = 0, p_round = 0;  // p_round: a bit per half, the parity of its next round
                 auto ready = [&](uint32_t i) { wait_bar(ctl, &ctl.full[i % kStages], (i / kStages) & 1); };
                 auto stage_at = [&](uint32_t i) { return ring + (i % kStages) * L::kTileBytes; };
-                // Rolled loops: unrolled ones keep dozens of operand descriptors in registers and spill.
                 auto score = [&](int wg, int q_tile, uint32_t i) {
-#pragma unroll 1
+                    const uint32_t q_low = desc_low(q_smem + q_tile * L::kTileBytes, 16), k_low = desc_low(stage_at(i), 16);
+#pragma unroll
                     for (int k = 0; k < D / 16; ++k) {
-                        const uint32_t off = (k >> 2) * (kTile * 128) + (k & 3) * 32;
-                        mma_ss(tmem + wg * kTile, smem_desc(q_smem + q_tile * L::kTileBytes + off, 16, 1024), smem_desc(stage_at(i) + off, 16, 1024), s_desc, k > 0);
+                        const uint32_t off = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
+                        mma_ss(tmem + wg * kTile, q_low + off, k_low + off, kDescHigh, s_desc, k > 0);
                     }
                     mma_commit(&ctl.s_full[wg]);
                 };
                 auto output = [&](int wg, uint32_t i, bool add) {
-                    wait_bar(ctl, &ctl.p_full[wg], p_round[wg] & 1);
-                    ++p_round[wg];
-                    fence_after();
-#pragma unroll 1
-                    for (int k = 0; k < kTile / 16; ++k)
-                        mma_ts(tmem + 2 * kTile + wg * D, tmem + wg * kTile + k * 8, smem_desc(stage_at(i) + k * 2048, D == 128 ? kTile * 128 : 1024, 1024), o_desc, add || k > 0);
+                    const uint32_t v_low = desc_low(stage_at(i), D == 128 ? kTile * 128 : 1024);
+                    const uint32_t o_at = tmem + 2 * kTile + wg * D, p_at = tmem + wg * kTile;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {  // the weights come in two halves
+                        wait_bar(ctl, &ctl.p_full[wg][half], p_round >> wg & 1);
+                        fence_after();
+#pragma unroll
+                        for (int k = half * (kTile / 32); k < (half + 1) * (kTile / 32); ++k)
+                            mma_ts(o_at, p_at + k * 8, v_low + k * (2048 >> 4), kDescHigh, o_desc, add || k > 0);
+                    }
+                    p_round ^= 1u << wg;
                 };
-                for (; walk.valid(); walk.next(p), ++item) {
-                    const int n = walk.tile1() - walk.tile0();
+                // The first softmax warpgroup says what comes: the walk stays out of this thread's registers.
+                for (uint32_t item = 0;; ++item) {
                     wait_bar(ctl, &ctl.q_full, item & 1);
                     fence_after();
-                    if (walk.shape.wide) {
-                        ready(seq);
+                    const int n = ctl.item_tiles[item & 1];
+                    const bool wide = ctl.item_wide[item & 1];
+                    if (n == 0 || *static_cast<volatile uint32_t*>(&ctl.abort)) break;
+                    // Scores of the first tile (two tiles) ahead of the loop.
+                    for (int t = 0; t < (wide ? 2 : min(n, 2)); ++t) {
+                        if (t == 0 || !wide) ready(seq);
                         fence_after();
-                        score(0, 0, seq);
-                        score(1, 1, seq);
-                        mma_commit(&ctl.empty[seq % kStages]);
-                        for (int t = 0; t < n; ++t) {
-                            const uint32_t v_at = seq + 2 * t + 1, k_at = v_at + 1;
-                            ready(v_at);
-                            if (t + 1 < n) ready(k_at);
-                            fence_after();
-                            for (int wg = 0; wg < 2; ++wg) {
-                                output(wg, v_at, t > 0);
-                                if (t + 1 == n) mma_commit(&ctl.o_full[wg]);
-                                if (wg == 1) mma_commit(&ctl.empty[v_at % kStages]);
-                                if (t + 1 < n) score(wg, wg, k_at);
-                            }
-                            if (t + 1 < n) mma_commit(&ctl.empty[k_at % kStages]);
-                        }
-                        seq += 2 * n;
-                    } else {
-                        for (int t = 0; t < min(n, 2); ++t) {
-                            ready(seq);
-                            fence_after();
-                            score(t, 0, seq);
-                            mma_commit(&ctl.empty[seq % kStages]);
-                            ++seq;
-                        }
-                        for (int t = 0; t < n; ++t) {
-                            const int wg = t & 1;
-                            ready(seq);
-                            fence_after();
-                            output(wg, seq, t > 1);
-                            if (t + 2 >= n) mma_commit(&ctl.o_full[wg]);
-                            mma_commit(&ctl.empty[seq % kStages]);
-                            ++seq;
-                            if (t + 2 < n) {
-                                ready(seq);
-                                fence_after();
-                                score(wg, 0, seq);
-                                mma_commit(&ctl.empty[seq % kStages]);
-                                ++seq;
+                        score(t, wide ? t : 0, seq);
+                        if (t == 1 || !wide) mma_commit(&ctl.empty[seq % kStages]), ++seq;
+                    }
+                    for (int t = 0; t < n; ++t) {
+                        // Wide: both halves use this tile's values and the next one's keys.  Else: one half, and the keys after next.
+                        const bool more = t + (wide ? 1 : 2) < n;
+                        ready(seq);
+                        if (wide && more) ready(seq + 1);
+                        fence_after();
+#pragma unroll 1
+                        for (int wg = wide ? 0 : t & 1; wg < (wide ? 2 : (t & 1) + 1); ++wg) {
+                            output(wg, seq, t >= (wide ? 1 : 2));
+                            if (!more) mma_commit(&ctl.o_full[wg]);
+                            if (!wide || wg == 1) mma_commit(&ctl.empty[seq % kStages]);
+                            if (more) {
+                                if (!wide) {
+                                    ready(seq + 1);
+                                    fence_after();
+                                }
+                                score(wg, wide ? wg : 0, seq + 1);
+                                if (!wide || wg == 1) mma_commit(&ctl.empty[(seq + 1) % kStages]);
                             }
                         }
+                        seq += more ? 2 : 1;
                     }
                 }
             }
             __syncwarp();
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
         Walk walk;
-        walk.start(p, ctl.start_seq, ctl.start_off, end - begin);
+        walk.start(p, start, end - begin);
         // ---- softmax warpgroups -------------------------------------------------------------------
         const int wg = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t s_addr = lane_base + wg * kTile, o_addr = lane_base + 2 * kTile + wg * D;
-        uint32_t seq = 0, s_round = 0, o_round = 0;
-        for (; walk.valid(); walk.next(p)) {
+        uint32_t seq = 0, s_round = 0, o_round = 0, item = 0;
+        for (; walk.valid(); walk.next(p), ++item) {
             const Range& r = walk.range;
             const bool wide = walk.shape.wide;
             const int t0 = walk.tile0(), n = walk.tile1() - t0;
             const int32_t q_first = a.query_start[walk.s];
             // Both warpgroups have read the last item's output: every product is done with Q.
             ptx::named_sync(1, 256);
-            for (int i = threadIdx.x; i < (wide ? 2 : 1) * kTile * (D / 8); i += 256) {
-                const int c = i % (D / 8), rr = i / (D / 8), half_tile = rr >> 7, lr = rr & 127;
-                const int32_t token = r.first + half_tile * p.tile_tokens + lr / p.group;
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (lr < p.tile_tokens * p.group && token < r.end) {
-                    const int head = walk.head * p.group + lr % p.group;
-                    x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + static_cast<int64_t>(q_first + token) * a.q_tok + head * a.q_head + c * 8);
-                    x.x ^= p.negate, x.y ^= p.negate, x.z ^= p.negate, x.w ^= p.negate;
+            {
+                // A thread's vector column is fixed; its rows come eight at a time, all loads in flight together.
+                constexpr int kCols = D / 8, kRowStep = 256 / kCols, kBatch = 8;
+                const int c = threadIdx.x % kCols;
+                const uint32_t at0 = q_smem + (c >> 3) * (kTile * 128);
+#pragma unroll 1
+                for (int r0 = threadIdx.x / kCols; r0 < (wide ? 2 : 1) * kTile; r0 += kRowStep * kBatch) {
+                    uint4 x[kBatch];
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        const int rr = r0 + j * kRowStep, lr = rr & 127, tok = lr * p.group_inv >> 16;
+                        const int32_t token = r.first + (rr >> 7) * p.tile_tokens + tok;
+                        x[j] = make_uint4(0, 0, 0, 0);
+                        if (rr < (wide ? 2 : 1) * kTile && tok < p.tile_tokens && token < r.end)
+                            x[j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + static_cast<int64_t>(q_first + token) * a.q_tok +
+                                                                   (walk.head * p.group + lr - tok * p.group) * a.q_head + c * 8);
+                    }
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        const int rr = r0 + j * kRowStep, lr = rr & 127;
+                        if (rr >= (wide ? 2 : 1) * kTile) break;
+                        const uint32_t at = at0 + (rr >> 7) * L::kTileBytes + lr * 128 + (((c & 7) ^ (lr & 7)) << 4);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[j].x ^ p.negate), "r"(x[j].y ^ p.negate), "r"(x[j].z ^ p.negate), "r"(x[j].w ^ p.negate) : "memory");
+                    }
                 }
-                const uint32_t at = q_smem + half_tile * L::kTileBytes + (c >> 3) * (kTile * 128) + lr * 128 + (((c & 7) ^ (lr & 7)) << 4);
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
             }
+            if (threadIdx.x == 0) ctl.item_tiles[item & 1] = n, ctl.item_wide[item & 1] = wide;
             fence_async_smem();
             fence_before();
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&ctl.q_full));
 
-            const int32_t token = r.first + (wide ? wg * p.tile_tokens : 0) + row / p.group;
-            const bool live = row < p.tile_tokens * p.group && token < r.end;
+            const int32_t row_token = row * p.group_inv >> 16;
+            const int32_t token = r.first + (wide ? wg * p.tile_tokens : 0) + row_token;
+            const bool live = row_token < p.tile_tokens && token < r.end;
             const bool warp_live = __any_sync(0xffffffffu, live);
             const int32_t pos = live ? walk.shape.past + token : -1;
             // Positions of this warpgroup's rows: a tile they all see needs no mask.
@@ -542,35 +600,45 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 wait_bar(ctl, &ctl.s_full[wg], s_round & 1);
                 ++s_round;
                 fence_after();
+                if (!seen_by_item) {
+                    const uint32_t v_at = seq + (wide ? 2 * t + 1 : min(n, 2) + t + min(t, max(n - 2, 0)));
+                    wait_bar(ctl, &ctl.full[v_at % kStages], (v_at / kStages) & 1);
+                    if (clean_values<T, D>(ring + (v_at % kStages) * L::kTileBytes, key0, r, a.window, a.sinks, row)) ctl.poison = 1;
+                    fence_async_smem();
+                }
+                uint32_t x[kTile];
+                float shift = 0.f;
                 if (warp_live) {
-                    uint32_t x[kTile];
 #pragma unroll
                     for (int c = 0; c < kTile; c += 32) tmem_ld32(s_addr + c, x + c);
                     wait_ld();
                     if (!seen) {
-                        const int32_t hi = pos - key0;  // columns up to hi
+                        // Visible columns, 32 to a word: up to the row's position, and behind its window's start or among the sinks.
+                        auto upto = [](int32_t last) { return last < 0 ? 0u : last >= 31 ? 0xffffffffu : (2u << last) - 1u; };
+                        const int32_t hi = pos - key0;
                         const int32_t lo = a.window > 0 ? static_cast<int32_t>(max(static_cast<int64_t>(-1), pos - a.window - key0)) : -1;
                         const int32_t sk = a.window > 0 ? static_cast<int32_t>(min(max(a.sinks - key0, static_cast<int64_t>(0)), static_cast<int64_t>(kTile))) : 0;
 #pragma unroll
-                        for (int c = 0; c < kTile; ++c)
-                            if (!(c <= hi && (c > lo || c < sk))) x[c] = 0xff800000u;
-                    }
-                    float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+                        for (int g = 0; g < kTile; g += 32) {
+                            const uint32_t visible = upto(hi - g) & (~upto(lo - g) | upto(sk - 1 - g));
 #pragma unroll
-                    for (int c = 0; c < kTile; c += 4) {
-                        m0 = fmaxf(m0, __uint_as_float(x[c]));
-                        m1 = fmaxf(m1, __uint_as_float(x[c + 1]));
-                        m2 = fmaxf(m2, __uint_as_float(x[c + 2]));
-                        m3 = fmaxf(m3, __uint_as_float(x[c + 3]));
+                            for (int c = 0; c < 32; ++c)
+                                if (!((visible >> c) & 1)) x[g + c] = 0xff800000u;
+                        }
                     }
-                    const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * p.scale2 - Kind<T>::bias;
+                    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int c = 0; c < kTile; c += 8)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) m[j] = fmaxf(fmaxf(m[j], __uint_as_float(x[c + 2 * j])), __uint_as_float(x[c + 2 * j + 1]));
+                    const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * p.scale2 - Kind<T>::bias;
                     const bool raise = top > ref + Kind<T>::grow || (ref == -INFINITY && top > -INFINITY);
                     if (__any_sync(0xffffffffu, raise)) {
                         const float factor = raise ? (ref == -INFINITY ? 0.f : ptx::ex2(ref - top)) : 1.f;
                         if (raise) ref = top;
                         sum *= factor;
                         if (i > 0) {
-#pragma unroll
+#pragma unroll 1
                             for (int c = 0; c < D; c += 32) {
                                 uint32_t o[32];
                                 tmem_ld32(o_addr + c, o);
@@ -581,29 +649,34 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                             }
                         }
                     }
-                    const float shift = ref == -INFINITY ? 0.f : -ref;
-                    float s0 = 0.f, s1 = 0.f;
+                    shift = ref == -INFINITY ? 0.f : -ref;
+                }
+                // Weights, half a tile at a time: the second product starts on the first half.
+                const uint64_t scale_2 = ptx::pack2(p.scale2, p.scale2), shift_2 = ptx::pack2(shift, shift);
 #pragma unroll
-                    for (int c = 0; c < kTile; c += 2) {
-                        const float e0 = ptx::ex2(fmaf(__uint_as_float(x[c]), p.scale2, shift));
-                        const float e1 = ptx::ex2(fmaf(__uint_as_float(x[c + 1]), p.scale2, shift));
-                        s0 += e0, s1 += e1;
-                        x[c / 2] = pack_pair(e0, e1, T{});
+                for (int half = 0; half < 2; ++half) {
+                    if (warp_live) {
+                        uint64_t s0 = 0, s1 = 0;
+                        uint32_t w[32];
+#pragma unroll
+                        for (int c = 0; c < 64; c += 4) {
+                            float e0, e1, e2, e3;
+                            ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(x[64 * half + c]), __uint_as_float(x[64 * half + c + 1])), scale_2, shift_2), e0, e1);
+                            ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(x[64 * half + c + 2]), __uint_as_float(x[64 * half + c + 3])), scale_2, shift_2), e2, e3);
+                            e0 = ptx::ex2(e0), e1 = ptx::ex2(e1), e2 = ptx::ex2(e2), e3 = ptx::ex2(e3);
+                            s0 = ptx::add2(s0, ptx::pack2(e0, e1)), s1 = ptx::add2(s1, ptx::pack2(e2, e3));
+                            w[c / 2] = pack_pair(e0, e1, T{}), w[c / 2 + 1] = pack_pair(e2, e3, T{});
+                        }
+                        tmem_st32(s_addr + 32 * half, w);
+                        float a0, a1;
+                        ptx::unpack2(ptx::add2(s0, s1), a0, a1);
+                        sum += a0 + a1;
+                        wait_st();
                     }
-                    sum += s0 + s1;
-                    tmem_st32(s_addr, x);
-                    tmem_st32(s_addr + 32, x + 32);
-                    wait_st();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&ctl.p_full[wg][half]));
                 }
-                if (!seen_by_item) {
-                    const uint32_t v_at = seq + (wide ? 2 * t + 1 : min(n, 2) + t + min(t, max(n - 2, 0)));
-                    wait_bar(ctl, &ctl.full[v_at % kStages], (v_at / kStages) & 1);
-                    if (clean_values<T, D>(ring + (v_at % kStages) * L::kTileBytes, key0, r, a.window, a.sinks, row)) ctl.poison = 1;
-                    fence_async_smem();
-                }
-                fence_before();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&ctl.p_full[wg]));
             }
             seq += 2 * n;
             if (mine > 0) {
@@ -642,7 +715,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             if (warp_live && (wide || wg == 0)) {
                 const bool whole = walk.whole();
                 const float inv = sum != 0.f ? 1.f / sum : 0.f;
-                const int head = walk.head * p.group + row % p.group;
+                const int head = walk.head * p.group + row - row_token * p.group;
                 const int64_t out_row = static_cast<int64_t>(q_first + token) * a.heads + head;
                 const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (walk.st0 == 0 ? 1 : 0)) * 256 + wg * kTile + row;
                 const float lse2 = sum != 0.f ? ref + log2f(sum) : -INFINITY;
@@ -679,6 +752,9 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             }
             fence_before();
         }
+        if (threadIdx.x == 0) ctl.item_tiles[item & 1] = 0;
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&ctl.q_full));
     }
     __syncthreads();
     fence_after();
@@ -692,13 +768,13 @@ constexpr int kFinishThreads = 256;
 // flagged items again row by row, writes every sequence's status and clears the rows of failed ones.
 template <typename T, int D>
 __global__ void __launch_bounds__(kFinishThreads) attend_finish_kernel(const Params p) {
-    __shared__ int64_t scan[kFinishThreads / 32];
-    __shared__ int64_t total, start_off;
-    __shared__ int32_t start_seq;
+    __shared__ LocateSpace<kFinishThreads> located;
     __shared__ float qs[kFinishThreads / 32][256];
     const AttendParams& a = p.a;
     const int c = blockIdx.x, ctas = gridDim.x, warp = threadIdx.x >> 5;
-    locate<kFinishThreads>(p, scan, total, start_off, start_seq, c, ctas);
+    locate<kFinishThreads>(p, located, c, ctas);  // of the call's inputs alone: may run before the tiles are done
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int64_t total = located.start.total;
 
     // Whether all pages that the sequence's rows see lie in the cache.  All threads of the block take part.
     auto failed = [&](int s) -> int {
@@ -721,7 +797,7 @@ __global__ void __launch_bounds__(kFinishThreads) attend_finish_kernel(const Par
     for (int i = threadIdx.x; i < ctas; i += kFinishThreads) abort |= p.flags[i] & 2;
     abort = __syncthreads_or(abort);
     Walk walk;
-    walk.start(p, start_seq, start_off, end - begin);
+    walk.start(p, located.start, end - begin);
     int64_t at = begin;
     for (bool first = true; walk.valid(); at += walk.st1 - walk.st0, walk.next(p), first = false) {
         if (!first && p.flags[c] == 0) break;                     // later items that end here are whole
@@ -737,12 +813,12 @@ __global__ void __launch_bounds__(kFinishThreads) attend_finish_kernel(const Par
         const int32_t q_first = a.query_start[walk.s];
         const int tokens = walk.range.end - walk.range.first;
         if (poison) {
-            for (int i = warp; i < tokens * p.group; i += kFinishThreads / 32)
+            for (int i = blockIdx.y * (kFinishThreads / 32) + warp; i < tokens * p.group; i += gridDim.y * (kFinishThreads / 32))
                 attend_row<T>(a, walk.s, q_first + walk.range.first + i / p.group, walk.head * p.group + i % p.group, qs[warp]);
             continue;
         }
         constexpr int kVecs = D / 4;
-        for (int i = threadIdx.x; i < tokens * p.group * kVecs; i += kFinishThreads) {
+        for (int i = blockIdx.y * kFinishThreads + threadIdx.x; i < tokens * p.group * kVecs; i += gridDim.y * kFinishThreads) {
             const int v = i % kVecs, rr = i / kVecs;
             const int tok = rr / p.group, j = rr % p.group;
             const int tile = tok / p.tile_tokens;
@@ -767,6 +843,7 @@ __global__ void __launch_bounds__(kFinishThreads) attend_finish_kernel(const Par
             if (v == 0 && a.lse != nullptr) a.lse[out_row] = (best + log2f(sum)) * 0.6931471805599453f;
         }
     }
+    if (blockIdx.y != 0) return;
     for (int s = c; s < a.seqs; s += ctas) {
         int code = failed(s);
         if (code == 0 && abort) code = BMS_STATUS_TIMEOUT;

@@ -534,9 +534,17 @@ int launch_tiles(const AttendParams& a, int dtype, int device, int sms, void* wo
     p.negate = a.scale < 0.f ? 0x80008000u : 0u;
     p.group = a.heads / a.kv_heads;
     p.tile_tokens = tc::kTile / p.group;
-    kernel<<<sms, tc::kThreads, tc::Layout<D>::kSmem, stream>>>(k_map, v_map, p);
-    tc::attend_finish_kernel<T, D><<<sms, tc::kFinishThreads, 0, stream>>>(p);
-    BMS_CUDA(cudaGetLastError(), "chunk attention launch");
+    p.group_inv = (65536 + p.group - 1) / p.group;
+    // Both launches are programmatic dependents: their prologues run while the launch before them ends.
+    cudaLaunchAttribute overlap{};
+    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    overlap.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(sms), cfg.blockDim = dim3(tc::kThreads), cfg.dynamicSmemBytes = tc::Layout<D>::kSmem, cfg.stream = stream;
+    cfg.attrs = &overlap, cfg.numAttrs = 1;
+    BMS_CUDA(cudaLaunchKernelEx(&cfg, kernel, k_map, v_map, p), "chunk attention launch");
+    cfg.gridDim = dim3(sms, 4), cfg.blockDim = dim3(tc::kFinishThreads), cfg.dynamicSmemBytes = 0;
+    BMS_CUDA(cudaLaunchKernelEx(&cfg, tc::attend_finish_kernel<T, D>, p), "chunk attention launch");
     return BMS_SUCCESS;
 }
 
