@@ -6,14 +6,14 @@
 // end; else an item is two tiles of 128 rows that read every key tile together.  Key tiles that no row of the item
 // sees (causal bound, window, sinks) are not part of it.
 //
-// Split.  All items' steps (a key tile, or a pair of them for one-tile items) form one line, cut into equal
+// Split.  All items, with their steps (a key tile, or a pair of them for one-tile items), form one line, cut into equal
 // parts, one per CTA: few long sequences fill the GPU as well as many short ones.  An item that a cut divides leaves
 // float32 partials (normalised output and log2 of the sum) in the workspace, and attend_finish_kernel joins them in
 // the order of the CTAs, so that results do not depend on timing.
 //
 // Pipeline (384 threads, one CTA per SM).  A producer warp loads pages by TMA (one box of up to 128 slots x 64
-// elements per page, 128-byte swizzle) into a ring of key and value tiles in the order the products consume them.  One
-// thread issues the products: S = Q K^T into TMEM, and O += P V with P in TMEM (over S) and V as an MN-major
+// elements per page, 128-byte swizzle) into a ring of key and value tiles in the order the products consume them, another
+// one the queries of the next item as soon as the last one's are done with.  One thread issues the products: S = Q K^T into TMEM, and O += P V with P in TMEM (over S) and V as an MN-major
 // operand, so neither P nor V is transposed or copied.  While a warpgroup turns S into P the tensor cores work for
 // the other one.  A softmax thread owns a row: no shuffles.  O is rescaled only when a row's maximum grew by more
 // than a threshold (2^8 for bfloat16); sums stay float32, weights are rounded once to the inputs' type for the
@@ -32,8 +32,8 @@ namespace bms {
 namespace tc {
 
 constexpr int kTile = 128;              // keys per tile, rows per query tile
-constexpr int kThreads = 384;           // 2 softmax warpgroups, one with the producer and the product warp
-constexpr int kProducerWarp = 8, kMmaWarp = 9;
+constexpr int kThreads = 384;           // 2 softmax warpgroups, one with the key/value, product and query warps
+constexpr int kProducerWarp = 8, kMmaWarp = 9, kQueryWarp = 10;
 constexpr uint64_t kWaitNs = 1000000000ull;
 
 template <int D>
@@ -46,7 +46,7 @@ struct Layout {
 
 struct Control {
     uint64_t full[12], empty[12];
-    uint64_t q_full, s_full[2], p_full[2][2], o_full[2];
+    uint64_t q_full, q_free, s_full[2], p_full[2][2], o_full[2];
     float ref[kTile], sum[kTile];
     int32_t item_tiles[2], item_wide[2];  // of the item whose queries are in place, by the item's parity; 0 tiles: no more
     uint32_t tmem, poison, abort;
@@ -54,18 +54,18 @@ struct Control {
 
 struct Params {
     AttendParams a;
-    float* parts;      // [ctas][2][256][D]
+    float* parts;      // [ctas][2][D / 4][256][4]: lanes (rows) side by side
     float* part_lse;   // [ctas][2][256], log2
     int32_t* flags;    // [ctas]: 1 poisoned values, 2 a wait ran out
     float scale2;      // |scale| log2(e)
-    uint32_t negate;   // sign bits for queries of a negative scale
+    uint32_t negate;   // sign bit for the scores of a negative scale
     int32_t group, tile_tokens;
     int32_t group_inv;  // 65536 / group, rounded up: r / group = r * group_inv >> 16 for rows r < 128
 };
 
 // ---- schedule ---------------------------------------------------------------------------------
 struct Shape {
-    int64_t total;  // steps of one key head over all query tiles
+    int64_t total;  // length of one key head's items over all query tiles
     int32_t n, past, tiles;
     bool wide;
 };
@@ -115,41 +115,51 @@ __device__ __forceinline__ Shape sequence_shape(const Params& p, int s) {
 
 // Where a part of the line of steps starts.
 struct Start {
-    int64_t total, off;  // all steps; the part's first step within its sequence
+    int64_t total, off;  // the line's length; the part's start within its sequence
     int32_t seq;
     Shape shape;
 };
 
-// Walks the items of a CTA's part of the line of steps.
+// Walks the items of a CTA's part of the line.  An item is kItemCost + steps long: what an item costs beside its steps
+// (queries in, result out, the pipeline's filling) counts as that many steps, so that many short items and few long
+// ones balance (64 verifying sequences of 2,048 to 24,576 keys took 432, 425 and 407 us at a cost of 0, 1 and 2 steps, 16
+// windowed ones 166, 161 and 153, four long prompt chunks 1,535, 1,506 and 1,530).  A part that ends inside an item's fixed
+// length leaves all of its steps to the next part.
+constexpr int kItemCost = 2;
 struct Walk {
     int32_t s, head, qt;
-    int64_t left;       // steps of the part not yet walked
+    int64_t left;       // length of the part not yet walked
+    int64_t at;         // where in the item the part continues
     int32_t st0, st1;   // steps of the current item that belong to the part
     Shape shape;
     Range range;
-    __device__ __forceinline__ void start(const Params& p, const Start& at, int64_t count) {
-        s = at.seq, left = count;
-        head = qt = st0 = 0;
+    __device__ __forceinline__ void start(const Params& p, const Start& from, int64_t count) {
+        s = from.seq, left = count;
+        head = qt = st0 = st1 = 0;
+        at = 0;
         if (count <= 0) return;
-        shape = at.shape;
-        const int64_t off = at.off;
-        head = static_cast<int32_t>(off / shape.total);
-        int64_t rest = off % shape.total;
+        shape = from.shape;
+        head = static_cast<int32_t>(from.off / shape.total);
+        at = from.off % shape.total;
         for (;; ++qt) {
             range = query_range(p, shape.n, shape.past, shape.wide, qt);
-            if (rest < range.steps) break;
-            rest -= range.steps;
+            if (at < kItemCost + range.steps) break;
+            at -= kItemCost + range.steps;
         }
-        st0 = static_cast<int32_t>(rest);
     }
-    __device__ __forceinline__ bool valid() {
-        if (left <= 0) return false;
-        st1 = static_cast<int32_t>(min(static_cast<int64_t>(range.steps), st0 + left));
-        return true;
+    // Moves on to the next item with steps in the part; false at the part's end.
+    __device__ __forceinline__ bool valid(const Params& p) {
+        while (left > 0) {
+            st0 = static_cast<int32_t>(max(at - kItemCost, static_cast<int64_t>(0)));
+            st1 = static_cast<int32_t>(min(static_cast<int64_t>(range.steps), at + left - kItemCost));
+            if (st1 > st0) return true;
+            next(p);
+        }
+        return false;
     }
     __device__ __forceinline__ void next(const Params& p) {
-        left -= st1 - st0;
-        st0 = 0;
+        left -= kItemCost + range.steps - at;
+        at = 0;
         if (left <= 0) return;
         if (++qt == shape.tiles) {
             qt = 0;
@@ -191,14 +201,14 @@ __device__ void locate(const Params& p, LocateSpace<kBlock>& sp, int c, int ctas
                     for (int i = warp; i < kBlock && base + i < p.a.seqs; i += kW) {
                         const Shape h = sequence_shape(p, base + i);
                         int t = 0;
-                        for (int q = lane; q < h.tiles; q += 32) t += query_range(p, h.n, h.past, h.wide, q).steps;
+                        for (int q = lane; q < h.tiles; q += 32) t += kItemCost + query_range(p, h.n, h.past, h.wide, q).steps;
                         t = __reduce_add_sync(0xffffffffu, t);
                         if (lane == 0) sp.totals[i] = t;
                     }
                 } else if (s < p.a.seqs) {
                     const Shape h = sequence_shape(p, s);
                     int64_t t = 0;
-                    for (int q = 0; q < h.tiles; ++q) t += query_range(p, h.n, h.past, h.wide, q).steps;
+                    for (int q = 0; q < h.tiles; ++q) t += kItemCost + query_range(p, h.n, h.past, h.wide, q).steps;
                     sp.totals[threadIdx.x] = t;
                 }
                 __syncthreads();
@@ -308,6 +318,13 @@ __device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, i
         : "memory");
 }
 
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int x, int head, int token, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar),
+        "r"(x), "r"(head), "r"(token)
+        : "memory");
+}
+
 // Waits at most about a second; after that the CTA's abort flag ends every wait.
 __device__ __forceinline__ void wait_bar(Control& c, uint64_t* bar, uint32_t parity) {
     const uint32_t addr = ptx::smem_addr(bar);
@@ -379,7 +396,8 @@ __device__ bool clean_values(uint32_t tile, int32_t key0, const Range& r, int64_
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
-attend_tiles_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const Params p) {
+attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                    const Params p) {
     using L = Layout<D>;
     constexpr int kStages = L::kStages;
     extern __shared__ unsigned char tiles_smem[];
@@ -391,7 +409,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) ptx::mbar_init(ptx::smem_addr(&ctl.full[i]), 1), ptx::mbar_init(ptx::smem_addr(&ctl.empty[i]), 1);
-        ptx::mbar_init(ptx::smem_addr(&ctl.q_full), 8);
+        ptx::mbar_init(ptx::smem_addr(&ctl.q_full), 1), ptx::mbar_init(ptx::smem_addr(&ctl.q_free), 8);
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(ptx::smem_addr(&ctl.s_full[i]), 1);
             ptx::mbar_init(ptx::smem_addr(&ctl.p_full[i][0]), 4), ptx::mbar_init(ptx::smem_addr(&ctl.p_full[i][1]), 4);
@@ -410,12 +428,13 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     fence_after();
     const uint32_t tmem = ctl.tmem;
     const Start start = located.start;
+    fence_async_smem();
     __syncthreads();  // everyone has it before Q comes in
     const int64_t begin = part_begin(start.total, blockIdx.x, gridDim.x), end = part_begin(start.total, blockIdx.x + 1, gridDim.x);
-    // Registers: launched with 168 a thread; 2 x 128 x 232 + 128 x 40 is exactly 384 x 168.  Each role sets its own
+    // Registers: launched with 168 a thread; 2 x 128 x 224 + 128 x 56 is exactly 384 x 168.  Each role sets its own
     // share inside its branch: after a join the compiler would have to assume the smaller one.
     if (warp >= kProducerWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == kProducerWarp) {
             Walk walk;
             walk.start(p, start, end - begin);
@@ -445,7 +464,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                     for (int half = 0; half < D / 64; ++half) tma_page(dst + half * (kTile * 128), map, half * 64, walk.head, slot, page, bar);
                 }
             };
-            for (; walk.valid(); walk.next(p)) {
+            for (; walk.valid(p); walk.next(p)) {
                 const int t0 = walk.tile0(), t1 = walk.tile1(), ahead = walk.shape.wide ? 1 : 2;
                 auto fetch = [&](int t) { return t < t1 ? page_of(t) : -1; };
                 // Pages of tiles t, t + 1, t + 2: values trail their keys by `ahead` tiles.
@@ -465,6 +484,33 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 for (uint32_t i = seq > kStages ? seq - kStages : 0; i < seq; ++i)
                     while (!ptx::mbar_try_wait(ptx::smem_addr(&ctl.full[i % kStages]), (i / kStages) & 1) && ptx::globaltimer() - t0 < kWaitNs / 5) {
                     }
+            }
+        } else if (warp == kQueryWarp) {
+            // Queries of the next item as soon as the last one's space is free: rows are (token, head of the group) pairs, and a
+            // box of the group's heads by the tile's tokens is just that.  Boxes may run into the next sequence's tokens
+            // (rows that nobody reads) and behind the last token (zeros).
+            Walk walk;
+            walk.start(p, start, end - begin);
+            uint32_t item = 0;
+            for (; walk.valid(p); walk.next(p), ++item) {
+                wait_bar(ctl, &ctl.q_free, (item & 1) ^ 1);
+                if (lane == 0) {
+                    const int tiles = walk.shape.wide ? 2 : 1;
+                    const uint32_t bar = ptx::smem_addr(&ctl.q_full);
+                    ctl.item_tiles[item & 1] = walk.tile1() - walk.tile0(), ctl.item_wide[item & 1] = walk.shape.wide;
+                    const bool go = !*static_cast<volatile uint32_t*>(&ctl.abort);
+                    ptx::mbar_arrive_expect_tx(bar, go ? tiles * p.tile_tokens * p.group * D * 2 : 0);
+                    for (int t = 0; t < tiles && go; ++t)
+                        for (int half = 0; half < D / 64; ++half)
+                            tma_rows(q_smem + t * L::kTileBytes + half * (kTile * 128), &q_map, half * 64, walk.head * p.group,
+                                     a.query_start[walk.s] + walk.range.first + t * p.tile_tokens, bar);
+                }
+                __syncwarp();
+            }
+            wait_bar(ctl, &ctl.q_free, (item & 1) ^ 1);
+            if (lane == 0) {
+                ctl.item_tiles[item & 1] = 0;
+                ptx::mbar_arrive(ptx::smem_addr(&ctl.q_full));
             }
         } else if (warp == kMmaWarp) {
             if (lane == 0) {
@@ -494,7 +540,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                     }
                     p_round ^= 1u << wg;
                 };
-                // The first softmax warpgroup says what comes: the walk stays out of this thread's registers.
+                // The query warp says what comes: the walk stays out of this thread's registers.
                 for (uint32_t item = 0;; ++item) {
                     wait_bar(ctl, &ctl.q_full, item & 1);
                     fence_after();
@@ -535,53 +581,19 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             __syncwarp();
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         Walk walk;
         walk.start(p, start, end - begin);
         // ---- softmax warpgroups -------------------------------------------------------------------
         const int wg = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t s_addr = lane_base + wg * kTile, o_addr = lane_base + 2 * kTile + wg * D;
-        uint32_t seq = 0, s_round = 0, o_round = 0, item = 0;
-        for (; walk.valid(); walk.next(p), ++item) {
+        uint32_t seq = 0, s_round = 0, o_round = 0;
+        for (; walk.valid(p); walk.next(p)) {
             const Range& r = walk.range;
             const bool wide = walk.shape.wide;
             const int t0 = walk.tile0(), n = walk.tile1() - t0;
             const int32_t q_first = a.query_start[walk.s];
-            // Both warpgroups have read the last item's output: every product is done with Q.
-            ptx::named_sync(1, 256);
-            {
-                // A thread's vector column is fixed; its rows come eight at a time, all loads in flight together.
-                constexpr int kCols = D / 8, kRowStep = 256 / kCols, kBatch = 8;
-                const int c = threadIdx.x % kCols;
-                const uint32_t at0 = q_smem + (c >> 3) * (kTile * 128);
-#pragma unroll 1
-                for (int r0 = threadIdx.x / kCols; r0 < (wide ? 2 : 1) * kTile; r0 += kRowStep * kBatch) {
-                    uint4 x[kBatch];
-#pragma unroll
-                    for (int j = 0; j < kBatch; ++j) {
-                        const int rr = r0 + j * kRowStep, lr = rr & 127, tok = lr * p.group_inv >> 16;
-                        const int32_t token = r.first + (rr >> 7) * p.tile_tokens + tok;
-                        x[j] = make_uint4(0, 0, 0, 0);
-                        if (rr < (wide ? 2 : 1) * kTile && tok < p.tile_tokens && token < r.end)
-                            x[j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + static_cast<int64_t>(q_first + token) * a.q_tok +
-                                                                   (walk.head * p.group + lr - tok * p.group) * a.q_head + c * 8);
-                    }
-#pragma unroll
-                    for (int j = 0; j < kBatch; ++j) {
-                        const int rr = r0 + j * kRowStep, lr = rr & 127;
-                        if (rr >= (wide ? 2 : 1) * kTile) break;
-                        const uint32_t at = at0 + (rr >> 7) * L::kTileBytes + lr * 128 + (((c & 7) ^ (lr & 7)) << 4);
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[j].x ^ p.negate), "r"(x[j].y ^ p.negate), "r"(x[j].z ^ p.negate), "r"(x[j].w ^ p.negate) : "memory");
-                    }
-                }
-            }
-            if (threadIdx.x == 0) ctl.item_tiles[item & 1] = n, ctl.item_wide[item & 1] = wide;
-            fence_async_smem();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&ctl.q_full));
-
             const int32_t row_token = row * p.group_inv >> 16;
             const int32_t token = r.first + (wide ? wg * p.tile_tokens : 0) + row_token;
             const bool live = row_token < p.tile_tokens && token < r.end;
@@ -612,6 +624,10 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 #pragma unroll
                     for (int c = 0; c < kTile; c += 32) tmem_ld32(s_addr + c, x + c);
                     wait_ld();
+                    if (p.negate) {
+#pragma unroll
+                        for (int c = 0; c < kTile; ++c) x[c] ^= p.negate;
+                    }
                     if (!seen) {
                         // Visible columns, 32 to a word: up to the row's position, and behind its window's start or among the sinks.
                         auto upto = [](int32_t last) { return last < 0 ? 0u : last >= 31 ? 0xffffffffu : (2u << last) - 1u; };
@@ -684,26 +700,19 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 ++o_round;
                 fence_after();
             }
-            // Merge of a one-tile item's halves through the space of Q (the second half is done with it: its output
-            // was committed after every score product).
-            float mine_w = 1.f, other_w = 0.f;
-            const bool merge = !wide && n > 1;
+            // The space of Q is free now (outputs were committed after every score product that reads it): one half takes the
+            // second half of a one-tile item, element by row in float32, half of the columns at a time, the other the
+            // finished rows on their way out, so that the stores are whole lines.
+            const bool merge = !wide && n > 1, writes = (wide || wg == 0) && warp_live, whole = walk.whole();
             float* exchange = reinterpret_cast<float*>(tiles_smem + (q_smem - ptx::smem_addr(tiles_smem)));
-            if (merge && wg == 1) {
-                if (warp_live) {
-#pragma unroll
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(o_addr + c, o);
-                        wait_ld();
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) exchange[(c + j) * kTile + row] = __uint_as_float(o[j]);
-                    }
-                    ctl.ref[row] = ref, ctl.sum[row] = sum;
-                }
+            const uint32_t stage = q_smem + (wide ? wg : 1) * L::kTileBytes;
+            const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (walk.st0 == 0 ? 1 : 0);
+            if (merge) {
+                if (wg == 1) ctl.ref[row] = ref, ctl.sum[row] = sum;
+                ptx::named_sync(1, 256);  // the other half's score products are done, too
             }
-            if (merge) ptx::named_sync(1, 256);
-            if (merge && wg == 0 && live) {
+            float mine_w = 1.f, other_w = 0.f;
+            if (merge && wg == 0) {
                 const float ref1 = ctl.ref[row], sum1 = ctl.sum[row];
                 const float best = fmaxf(ref, ref1);
                 if (best > -INFINITY) {
@@ -712,49 +721,76 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                     ref = best;
                 }
             }
-            if (warp_live && (wide || wg == 0)) {
-                const bool whole = walk.whole();
-                const float inv = sum != 0.f ? 1.f / sum : 0.f;
-                const int head = walk.head * p.group + row - row_token * p.group;
-                const int64_t out_row = static_cast<int64_t>(q_first + token) * a.heads + head;
-                const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (walk.st0 == 0 ? 1 : 0)) * 256 + wg * kTile + row;
-                const float lse2 = sum != 0.f ? ref + log2f(sum) : -INFINITY;
+            const float inv = sum != 0.f ? 1.f / sum : 0.f;
+            mine_w *= inv, other_w *= inv;
+            constexpr int kPart = D / 2;
+#pragma unroll 1
+            for (int c0 = 0; c0 < D; c0 += kPart) {
+                if (merge) {
+                    if (wg == 1 && warp_live) {
+                        uint32_t o[kPart];
 #pragma unroll
-                for (int c = 0; c < D; c += 32) {
-                    uint32_t o[32];
-                    tmem_ld32(o_addr + c, o);
+                        for (int c = 0; c < kPart; c += 32) tmem_ld32(o_addr + c0 + c, o + c);
+                        wait_ld();
+#pragma unroll
+                        for (int c = 0; c < kPart; ++c) exchange[c * kTile + row] = __uint_as_float(o[c]);
+                    }
+                    ptx::named_sync(1, 256);
+                }
+                if (writes) {
+                    uint32_t o[kPart];
+#pragma unroll
+                    for (int c = 0; c < kPart; c += 32) tmem_ld32(o_addr + c0 + c, o + c);
                     wait_ld();
-                    if (live) {
-                        float f[32];
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            float y = __uint_as_float(o[j]);
-                            if (merge) y = y * mine_w + exchange[(c + j) * kTile + row] * other_w;
-                            f[j] = y * inv;
+                    for (int c = 0; c < kPart; ++c) {
+                        if (c % 8 == 0) asm volatile("" ::: "memory");  // few loads ahead: all of them would not fit the registers
+                        o[c] = __float_as_uint(__uint_as_float(o[c]) * mine_w + (merge ? exchange[c * kTile + row] * other_w : 0.f));
+                    }
+                    if (whole) {
+#pragma unroll
+                        for (int j = 0; j < kPart / 8; ++j) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) w[i] = pack_pair(__uint_as_float(o[8 * j + 2 * i]), __uint_as_float(o[8 * j + 2 * i + 1]), T{});
+                            const int c = c0 / 8 + j;
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + row * (D * 2) + ((c ^ (row & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
                         }
-                        if (whole) {
-                            uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + out_row * D + c);
+                    } else if (live) {
+                        float4* dst = reinterpret_cast<float4*>(p.parts) + (slot * (D / 4) + c0 / 4) * 256 + wg * kTile + row;
 #pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                dst[j] = make_uint4(pack_pair(f[8 * j], f[8 * j + 1], T{}), pack_pair(f[8 * j + 2], f[8 * j + 3], T{}),
-                                                    pack_pair(f[8 * j + 4], f[8 * j + 5], T{}), pack_pair(f[8 * j + 6], f[8 * j + 7], T{}));
-                        } else {
-                            float4* dst = reinterpret_cast<float4*>(p.parts + slot * D + c);
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) dst[j] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
-                        }
+                        for (int j = 0; j < kPart / 4; ++j)
+                            dst[j * 256] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
                     }
                 }
+                if (merge) ptx::named_sync(1, 256);
+            }
+            if (writes) {
                 if (live) {
-                    if (!whole) p.part_lse[slot] = lse2;
-                    else if (a.lse != nullptr) a.lse[out_row] = lse2 * 0.6931471805599453f;
+                    const float lse2 = sum != 0.f ? ref + log2f(sum) : -INFINITY;
+                    if (!whole) p.part_lse[slot * 256 + wg * kTile + row] = lse2;
+                    else if (a.lse != nullptr) a.lse[static_cast<int64_t>(q_first + token) * a.heads + walk.head * p.group + row - row_token * p.group] = lse2 * 0.6931471805599453f;
+                }
+                if (whole) {
+                    __syncwarp();
+                    constexpr int kCols = D / 8, kRows = 32 / kCols;
+                    const int c = lane % kCols;
+#pragma unroll 4
+                    for (int r0 = lane / kCols; r0 < 32; r0 += kRows) {
+                        const int rr = (warp & 3) * 32 + r0, tok = rr * p.group_inv >> 16;
+                        const int32_t to = wg_first + tok;
+                        uint4 y;
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w) : "r"(stage + rr * (D * 2) + ((c ^ (rr & 7)) << 4)));
+                        if (tok < p.tile_tokens && to < r.end)
+                            reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (static_cast<int64_t>(q_first + to) * a.heads + walk.head * p.group + rr - tok * p.group) * D)[c] = y;
+                    }
                 }
             }
+            fence_async_smem();  // the next queries come into this space by TMA
             fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&ctl.q_free));
         }
-        if (threadIdx.x == 0) ctl.item_tiles[item & 1] = 0;
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&ctl.q_full));
     }
     __syncthreads();
     fence_after();
@@ -798,11 +834,10 @@ __global__ void __launch_bounds__(kFinishThreads) attend_finish_kernel(const Par
     abort = __syncthreads_or(abort);
     Walk walk;
     walk.start(p, located.start, end - begin);
-    int64_t at = begin;
-    for (bool first = true; walk.valid(); at += walk.st1 - walk.st0, walk.next(p), first = false) {
+    for (bool first = true; walk.valid(p); walk.next(p), first = false) {
         if (!first && p.flags[c] == 0) break;                     // later items that end here are whole
         if (walk.st1 != walk.range.steps) break;                  // ends in a later part
-        const int64_t item_begin = at - walk.st0;
+        const int64_t item_begin = end - walk.left - walk.at + kItemCost;  // of the item's first step
         if (walk.st0 == 0 && p.flags[c] == 0) continue;           // whole and clean
         int from = c;
         while (from > 0 && part_begin(total, from, ctas) > item_begin) --from;
@@ -817,29 +852,31 @@ __global__ void __launch_bounds__(kFinishThreads) attend_finish_kernel(const Par
                 attend_row<T>(a, walk.s, q_first + walk.range.first + i / p.group, walk.head * p.group + i % p.group, qs[warp]);
             continue;
         }
-        constexpr int kVecs = D / 4;
-        for (int i = blockIdx.y * kFinishThreads + threadIdx.x; i < tokens * p.group * kVecs; i += gridDim.y * kFinishThreads) {
-            const int v = i % kVecs, rr = i / kVecs;
+        const int rows = tokens * p.group;
+        for (int i = blockIdx.y * kFinishThreads + threadIdx.x; i < rows * (D / 8); i += gridDim.y * kFinishThreads) {
+            const int v = i / rows, rr = i - v * rows;
             const int tok = rr / p.group, j = rr % p.group;
             const int tile = tok / p.tile_tokens;
             const int local = tile * kTile + (tok - tile * p.tile_tokens) * p.group + j;
-            auto slot = [&](int cta) { return (static_cast<int64_t>(cta) * 2 + (cta == from ? 1 : 0)) * 256 + local; };
+            auto slot = [&](int cta) { return static_cast<int64_t>(cta) * 2 + (cta == from ? 1 : 0); };
             float best = -INFINITY;
-            for (int k = from; k <= c; ++k) best = fmaxf(best, p.part_lse[slot(k)]);
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            float sum = 0.f;
+            for (int k = from; k <= c; ++k) best = fmaxf(best, p.part_lse[slot(k) * 256 + local]);
+            float o[8] = {}, sum = 0.f;
+#pragma unroll 2
             for (int k = from; k <= c; ++k) {
-                const float lse = p.part_lse[slot(k)];
+                const float lse = p.part_lse[slot(k) * 256 + local];
                 // A part whose rows saw nothing weighs 0; NaN passes on.
                 const float w = lse == -INFINITY ? 0.f : exp2f(lse - best);
-                const float4 x = *reinterpret_cast<const float4*>(p.parts + slot(k) * D + 4 * v);
-                o.x += w * x.x, o.y += w * x.y, o.z += w * x.z, o.w += w * x.w;
+                const float4* src = reinterpret_cast<const float4*>(p.parts) + (slot(k) * (D / 4) + 2 * v) * 256 + local;
+                const float4 x = src[0], y = src[256];
+                o[0] += w * x.x, o[1] += w * x.y, o[2] += w * x.z, o[3] += w * x.w;
+                o[4] += w * y.x, o[5] += w * y.y, o[6] += w * y.z, o[7] += w * y.w;
                 sum += w;
             }
             const float inv = 1.f / sum;
             const int64_t out_row = static_cast<int64_t>(q_first + walk.range.first + tok) * a.heads + walk.head * p.group + j;
-            uint2 packed = make_uint2(pack_pair(o.x * inv, o.y * inv, T{}), pack_pair(o.z * inv, o.w * inv, T{}));
-            *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + out_row * D + 4 * v) = packed;
+            reinterpret_cast<uint4*>(static_cast<T*>(a.out) + out_row * D)[v] =
+                make_uint4(pack_pair(o[0] * inv, o[1] * inv, T{}), pack_pair(o[2] * inv, o[3] * inv, T{}), pack_pair(o[4] * inv, o[5] * inv, T{}), pack_pair(o[6] * inv, o[7] * inv, T{}));
             if (v == 0 && a.lse != nullptr) a.lse[out_row] = (best + log2f(sum)) * 0.6931471805599453f;
         }
     }

@@ -511,6 +511,18 @@ int page_map(CUtensorMap* map, const AttendParams& p, int dtype, const void* bas
     return BMS_SUCCESS;
 }
 
+int query_map(CUtensorMap* map, const AttendParams& p, int dtype, int group, int tile_tokens) {
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(p.dim), static_cast<cuuint64_t>(p.heads), static_cast<cuuint64_t>(p.tokens)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(std::max<int64_t>(p.q_head * 2, 16)), static_cast<cuuint64_t>(std::max<int64_t>(p.q_tok * 2, 16))};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(tile_tokens)};
+    const cuuint32_t steps[3] = {1, 1, 1};
+    const CUresult rc = encode_tiled()(map, dtype == BMS_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                                       const_cast<void*>(p.q), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) return fail(BMS_ERROR_CUDA, "tensor map of the queries (driver error %d)", static_cast<int>(rc));
+    return BMS_SUCCESS;
+}
+
 int64_t tiles_workspace(int64_t ctas, int64_t dim) { return 256 + ctas * 2 * 256 * (dim + 1) * 4 + ((ctas * 4 + 255) / 256) * 256; }
 
 template <typename T, int D>
@@ -521,7 +533,9 @@ int launch_tiles(const AttendParams& a, int dtype, int device, int sms, void* wo
         BMS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tc::Layout<D>::kSmem), "cudaFuncSetAttribute(smem)");
         ready[device] = true;
     }
-    CUtensorMap k_map, v_map;
+    const int group = a.heads / a.kv_heads;
+    CUtensorMap q_map, k_map, v_map;
+    BMS_CHECK(query_map(&q_map, a, dtype, group, tc::kTile / group));
     BMS_CHECK(page_map(&k_map, a, dtype, a.k, a.k_page, a.k_slot, a.k_head));
     BMS_CHECK(page_map(&v_map, a, dtype, a.v, a.v_page, a.v_slot, a.v_head));
     tc::Params p{};
@@ -531,8 +545,8 @@ int launch_tiles(const AttendParams& a, int dtype, int device, int sms, void* wo
     p.parts = reinterpret_cast<float*>(rest);
     p.part_lse = p.parts + static_cast<int64_t>(sms) * 2 * 256 * D;
     p.scale2 = std::max(std::fabs(a.scale) * 1.4426950408889634f, 1e-30f);  // a factor of 0 would turn masked scores into NaN
-    p.negate = a.scale < 0.f ? 0x80008000u : 0u;
-    p.group = a.heads / a.kv_heads;
+    p.negate = a.scale < 0.f ? 0x80000000u : 0u;
+    p.group = group;
     p.tile_tokens = tc::kTile / p.group;
     p.group_inv = (65536 + p.group - 1) / p.group;
     // Both launches are programmatic dependents: their prologues run while the launch before them ends.
@@ -542,7 +556,7 @@ int launch_tiles(const AttendParams& a, int dtype, int device, int sms, void* wo
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(sms), cfg.blockDim = dim3(tc::kThreads), cfg.dynamicSmemBytes = tc::Layout<D>::kSmem, cfg.stream = stream;
     cfg.attrs = &overlap, cfg.numAttrs = 1;
-    BMS_CUDA(cudaLaunchKernelEx(&cfg, kernel, k_map, v_map, p), "chunk attention launch");
+    BMS_CUDA(cudaLaunchKernelEx(&cfg, kernel, q_map, k_map, v_map, p), "chunk attention launch");
     cfg.gridDim = dim3(sms, 4), cfg.blockDim = dim3(tc::kFinishThreads), cfg.dynamicSmemBytes = 0;
     BMS_CUDA(cudaLaunchKernelEx(&cfg, tc::attend_finish_kernel<T, D>, p), "chunk attention launch");
     return BMS_SUCCESS;
