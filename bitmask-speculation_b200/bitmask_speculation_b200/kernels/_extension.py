@@ -28,16 +28,22 @@ def _torch():
     return torch
 
 
-def _dtype_code(t) -> int:
+@lru_cache(maxsize=1)
+def _dtype_codes() -> dict:
     torch = _torch()
-    codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-    if t.dtype not in codes:
+    return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _dtype_code(t) -> int:
+    code = _dtype_codes().get(t.dtype)
+    if code is None:
         raise RuntimeError("logits must be float32, bfloat16 or float16")
-    return codes[t.dtype]
+    return code
 
 
 def _stream(device):
-    return _torch().cuda.current_stream(device).cuda_stream
+    # The raw handle: building a torch.cuda.Stream object costs a small call about 2 us of host time.
+    return _torch()._C._cuda_getCurrentRawStream(device.index)
 
 
 def _check_mask(mask, vocab: int) -> None:
@@ -319,21 +325,16 @@ class NativeModule:
         torch = _torch()
         dev = past.device
         seqs, width = table.shape
-        # One int32 block for all small outputs; views start on multiples of 4 elements.
-        sizes = (seqs + 1, seqs, tokens, seqs, 1, seqs)
-        at, offsets = 0, []
-        for n in sizes:
-            offsets.append(at)
-            at += (n + 3) // 4 * 4
-        block = torch.empty(at, dtype=torch.int32, device=dev)
-        query_start, seq_lens, positions, held_out, count_out, status = (block[o:o + n] for o, n in zip(offsets, sizes))
+        # One int32 block for the small outputs: an allocation each would double the call's host time.
+        block = torch.empty(4 * seqs + 2 + tokens, dtype=torch.int32, device=dev)
+        query_start, seq_lens, held_out, status, count_out, positions = block.split((seqs + 1, seqs, seqs, seqs, 1, tokens))
         slots = torch.empty(tokens, dtype=torch.int64, device=dev)
         base = block.data_ptr()
-        a = [base + 4 * o for o in offsets]
         _native.check(self._lib.bms_page_plan(
             past.data_ptr(), new.data_ptr(), held.data_ptr(), seqs, table.data_ptr(), width, free_pages.data_ptr(),
-            free_pages.shape[0], free_count.data_ptr(), page_size, tokens, a[0], a[1], a[2] if tokens else None,
-            slots.data_ptr() if tokens else None, a[3], a[4], a[5], dev.index, _stream(dev)))
+            free_pages.shape[0], free_count.data_ptr(), page_size, tokens, base, base + 4 * (seqs + 1),
+            base + 4 * (4 * seqs + 2) if tokens else None, slots.data_ptr() if tokens else None, base + 4 * (2 * seqs + 1),
+            base + 4 * (4 * seqs + 1), base + 4 * (3 * seqs + 1), dev.index, _stream(dev)))
         return [query_start, seq_lens, positions, slots, held_out, count_out, status]
 
     @staticmethod
@@ -368,7 +369,7 @@ class NativeModule:
         dev = q.device
         lse = torch.empty((n, heads), dtype=torch.float32, device=dev)
         status = torch.empty(seqs, dtype=torch.int32, device=dev)
-        nbytes = int(self._lib.bms_attention_workspace_bytes(dev.index, n, heads, seqs, dim))
+        nbytes = self._lib.bms_attention_workspace_bytes(dev.index, n, heads, seqs, dim)
         if nbytes < 0:
             raise RuntimeError(f"no workspace size for device {dev}")
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)

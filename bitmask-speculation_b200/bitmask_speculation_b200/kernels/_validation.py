@@ -114,11 +114,11 @@ def device_tensor(t, name: str, *, ndim: int, dtype=None, device=None, floating:
         raise TypeError(f"{name} must be a float32, bfloat16 or float16 tensor")
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{name} must be a {str(dtype).removeprefix('torch.')} tensor")
-    if t.layout != torch.strided or t.ndim != ndim:
+    if t.ndim != ndim or t.layout != torch.strided:
         raise ValueError(f"{name} must be a strided tensor of {ndim} dimensions")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name} must be on CUDA; no implicit transfer")
-    if device is not None and t.device != device:
+    if device is not None and t.get_device() != device.index:
         raise ValueError(f"{name} must be on the same CUDA device as the other inputs")
     return t
 
