@@ -13,6 +13,11 @@ kernels:
   round is verified by ``grammar_verification.verify_with_grammar`` (one launch pair, one sync)
   instead of the reference's per-row loop.
 
+A decoder forwards its whole prefix again in every call, as the loops it stands in for do.  With
+``enable_cache`` it keeps the keys and values of each sequence's last prefix in pages (``paged``) and
+forwards only the tokens behind the part that the next call shares with it: a verification round
+then costs its K + 1 rows, and rejected drafts' pages go back to the pool.
+
 Speculative decoding with greedy verification reproduces target-only greedy decoding token for
 token; ``tests/test_gpu_decode.py`` checks that, and ``bench.py --workload decode`` measures it.
 """
@@ -76,8 +81,21 @@ def build_decoder(vocab: int, *, layers: int, dim: int, heads: int, kv_heads: in
             v = v.repeat_interleave(heads // kv_heads, 0)
             a = torch.nn.functional.scaled_dot_product_attention(q[None], k[None], v[None], is_causal=True)[0]
             x = x + self.o(a.transpose(0, 1).reshape(t, heads * head_dim))
+            return self._mlp(x)
+
+        def _mlp(self, x):
             g, u = self.up(self.n2(x)).chunk(2, -1)
             return x + self.down(torch.nn.functional.silu(g) * u)
+
+        def paged(self, x, cos, sin, plan, cache, table):
+            """The block over a step's new tokens [N, dim], its keys and values in ``cache``."""
+            from .paged import chunk_attention, rotary_append
+            t = x.shape[0]
+            h = self.n1(x)
+            k, v = self.kv(h).view(t, 2, kv_heads, head_dim).unbind(1)
+            q = rotary_append(self.q(h).view(t, heads, head_dim), k, v, cos, sin, plan.positions, plan.slots, cache)
+            a = chunk_attention(q, cache, table, plan.seq_lens, plan.query_start).out
+            return self._mlp(x + self.o(a.reshape(t, heads * head_dim)))
 
     class Decoder(nn.Module):
         def __init__(self):
@@ -91,6 +109,7 @@ def build_decoder(vocab: int, *, layers: int, dim: int, heads: int, kv_heads: in
             self.register_buffer("inv_freq", inv.float(), persistent=False)
             self._graphs = None  # padded length -> (CUDA graph, token buffer, trunk output, rotary tables)
             self._pool = None
+            self._cache = None
 
         def _rope(self, length: int):
             pos = torch.arange(length, device=self.inv_freq.device, dtype=torch.float32)
@@ -111,6 +130,13 @@ def build_decoder(vocab: int, *, layers: int, dim: int, heads: int, kv_heads: in
             if self._graphs is None:
                 self._graphs = {}
                 self._pool = torch.cuda.graph_pool_handle()
+            return self
+
+        def enable_cache(self, max_tokens: int, *, sequences: int = 1, page_size: int = 64):
+            """Keep keys and values of up to ``sequences`` sequences of at most ``max_tokens`` tokens
+            between calls: ``logits`` (sequence 0) and ``logits_batch`` then forward only the tokens
+            behind the longest prefix that a sequence shares with its last call."""
+            self._cache = _PagedForward(self, kv_heads, head_dim, sequences, max_tokens, page_size)
             return self
 
         def _captured(self, length: int):
@@ -134,7 +160,10 @@ def build_decoder(vocab: int, *, layers: int, dim: int, heads: int, kv_heads: in
         def logits(self, tokens, first: int, rows: int):
             """Logits of positions [first, first + rows) after one forward over ``tokens``.  The
             sequence is padded at the end to a multiple of 64 tokens (causal attention: padding
-            never reaches earlier positions) so that kernel shapes repeat across calls."""
+            never reaches earlier positions) so that kernel shapes repeat across calls.  With a cache
+            the forward runs over the tokens that the cache lacks, unpadded."""
+            if self._cache is not None:
+                return self.logits_batch([tokens], [first], [rows])[0]
             n = len(tokens)
             padded = list(tokens) + [0] * (-n % 64)
             host = torch.tensor(padded, dtype=torch.long)
@@ -147,6 +176,17 @@ def build_decoder(vocab: int, *, layers: int, dim: int, heads: int, kv_heads: in
                 ids = host.to(self.head.weight.device, non_blocking=True)
                 x = self._trunk(ids, *self._rope(ids.shape[0]))
             return self.head(self.norm(x[first:first + rows])).contiguous()
+
+        @torch.inference_mode()
+        def logits_batch(self, sequences, firsts, rows):
+            """Logits of positions [firsts[i], firsts[i] + rows[i]) of each sequence, after one forward of
+            all of them over the cache (``enable_cache``); sequence i keeps its pages from call to call."""
+            if self._cache is None:
+                raise ValueError("logits_batch needs enable_cache")
+            x, starts = self._cache.forward(sequences, firsts)
+            at = [i for s, n in zip(starts, rows) for i in range(s, s + n)]
+            picked = x[at[0]:at[-1] + 1] if at == list(range(at[0], at[0] + len(at))) else x[torch.tensor(at, device=x.device)]
+            return self.head(self.norm(picked)).split(list(rows))
 
     gen = torch.Generator().manual_seed(seed)
     model = Decoder()
@@ -161,6 +201,63 @@ def _rotate(x, cos, sin):
     half = x.shape[-1] // 2
     a, b = x[..., :half], x[..., half:]
     return _torch().cat((a * cos - b * sin, a * sin + b * cos), -1)
+
+
+class _PagedForward:
+    """The keys and values behind ``Decoder.enable_cache``: a paged cache per block, one block table for all
+    of them, and the tokens whose keys and values each sequence's pages hold."""
+
+    def __init__(self, model, kv_heads: int, head_dim: int, sequences: int, max_tokens: int, page_size: int):
+        torch = _torch()
+        from .paged import PagedCache
+        for value, name in ((sequences, "sequences"), (max_tokens, "max_tokens"), (page_size, "page_size")):
+            if isinstance(value, bool) or not isinstance(value, int) or value <= 0:
+                raise ValueError(f"{name} must be a positive integer")
+        dev, dtype = model.head.weight.device, model.head.weight.dtype
+        width = -(-max_tokens // page_size)
+        self.model, self.max_tokens, self.page_size = model, max_tokens, page_size
+        self.caches = [PagedCache.allocate(sequences * width, page_size, kv_heads, head_dim, dtype=dtype, device=dev) for _ in model.blocks]
+        self.table = torch.zeros((sequences, width), dtype=torch.int32, device=dev)
+        self.free_pages = torch.arange(sequences * width, dtype=torch.int32, device=dev)
+        self.free_count = torch.full((1,), sequences * width, dtype=torch.int32, device=dev)
+        self.held = torch.zeros(sequences, dtype=torch.int32, device=dev)
+        angles = torch.arange(max_tokens, device=dev, dtype=torch.float32)[:, None] * model.inv_freq.float()[None, :]
+        self.cos, self.sin = angles.cos(), angles.sin()
+        self.tokens: list[list[int]] = [[] for _ in range(sequences)]
+
+    def forward(self, sequences, firsts):
+        """The last block's rows of one packed forward, and where each sequence's position ``firsts[i]`` is among
+        them.  Sequences that are not given lose their pages."""
+        torch = _torch()
+        from .paged import plan_pages
+        if not 0 < len(sequences) <= len(self.tokens) or len(firsts) != len(sequences):
+            raise ValueError(f"the cache holds {len(self.tokens)} sequences, with one first position each")
+        wanted = [[int(t) for t in tokens] for tokens in sequences] + [[] for _ in range(len(self.tokens) - len(sequences))]
+        past, new, ids, starts = [], [], [], []
+        for i, tokens in enumerate(wanted):
+            keep = 0
+            if i < len(sequences):
+                if not 0 <= firsts[i] < len(tokens) <= self.max_tokens:
+                    raise ValueError(f"sequence {i}: its length must be at most {self.max_tokens} and its first row inside it")
+                for a, b in zip(self.tokens[i], tokens[:firsts[i]]):
+                    if a != b:
+                        break
+                    keep += 1
+                starts.append(len(ids) + firsts[i] - keep)
+            past.append(keep)
+            new.append(len(tokens) - keep)
+            ids += tokens[keep:]
+        model, dev = self.model, self.table.device
+        self.tokens = [[] for _ in wanted]  # nothing is kept if a launch below fails
+        up = torch.tensor(past + new + ids, dtype=torch.int32).to(dev, non_blocking=True)
+        past, new, ids = up.split((len(past), len(new), len(ids)))
+        plan = plan_pages(past, new, self.held, self.table, self.free_pages, self.free_count, page_size=self.page_size, tokens=ids.shape[0])
+        self.held, self.free_count = plan.held, plan.free_count
+        x = model.embed(ids)
+        for block, cache in zip(model.blocks, self.caches):
+            x = block.paged(x, self.cos, self.sin, plan, cache, self.table)
+        self.tokens = wanted
+        return x, starts
 
 
 # ---------------------------------------------------------------- selection

@@ -701,7 +701,8 @@ int bms_chunk_attention(const void* q, int32_t dtype, int64_t tokens, int64_t he
     BMS_CHECK(check_cache(cache, device, size));
     if (cache->dim > 256) return fail(BMS_ERROR_UNSUPPORTED, "dim is at most 256");
     if (heads % cache->kv_heads != 0) return fail(BMS_ERROR_INVALID_ARGUMENT, "heads must be a multiple of the cache's kv_heads");
-    if (tokens > 1073741823LL || width * cache->page_size > 2147483647LL) return fail(BMS_ERROR_UNSUPPORTED, "lengths beyond the 32-bit range");
+    if (tokens > 1073741823LL || width > 2147483391LL / cache->page_size)  // positions, rounded up to a tile, fit int32
+        return fail(BMS_ERROR_UNSUPPORTED, "lengths beyond the 32-bit range");
     BMS_CHECK(check_ptr(table, device, "table", 4));
     BMS_CHECK(check_ptr(seq_lens, device, "seq_lens", 4));
     BMS_CHECK(check_ptr(query_start, device, "query_start", 4));
