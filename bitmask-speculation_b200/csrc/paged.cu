@@ -584,12 +584,16 @@ int sm_count(int device, int& sms) {
     return BMS_SUCCESS;
 }
 
-int check_cache(const bms_paged_cache* c, int device, int size) {
+int check_cache_shape(const bms_paged_cache* c) {
     if (c == nullptr) return fail(BMS_ERROR_INVALID_ARGUMENT, "cache must not be NULL");
     if (c->pages <= 0 || c->page_size <= 0 || c->kv_heads <= 0 || c->dim <= 0 || c->pages > 2147483647LL || c->page_size > 65536 || c->kv_heads > 65535)
         return fail(BMS_ERROR_INVALID_ARGUMENT, "invalid cache shape");
     for (int i = 0; i < 3; ++i)
         if (c->k_stride[i] < 0 || c->v_stride[i] < 0) return fail(BMS_ERROR_INVALID_ARGUMENT, "cache strides must not be negative");
+    return BMS_SUCCESS;
+}
+
+int check_cache(const bms_paged_cache* c, int device, int size) {
     BMS_CHECK(check_ptr(c->k, device, "cache k", size));
     return check_ptr(c->v, device, "cache v", size);
 }
@@ -651,11 +655,12 @@ int bms_rotary_append(const void* q, const void* k, const void* v, int32_t dtype
     if (tokens < 0 || heads <= 0 || heads > 65535 || max_positions <= 0)
         return fail(BMS_ERROR_INVALID_ARGUMENT, "tokens, heads and max_positions must be positive");
     if (q_stride == nullptr || k_stride == nullptr || v_stride == nullptr) return fail(BMS_ERROR_INVALID_ARGUMENT, "strides must not be NULL");
+    BMS_CHECK(check_cache_shape(cache));
+    if (cache->dim % 2 != 0 || cache->dim > 65536) return fail(BMS_ERROR_INVALID_ARGUMENT, "dim must be even");
     const int size = dtype == BMS_FLOAT32 ? 4 : 2;
     RelaxedCapture relaxed;
     BMS_CHECK(check_device(device));
     BMS_CHECK(check_cache(cache, device, size));
-    if (cache->dim % 2 != 0 || cache->dim > 65536) return fail(BMS_ERROR_INVALID_ARGUMENT, "dim must be even");
     if (tokens == 0) return BMS_SUCCESS;
     const void* ptrs[] = {q, k, v, q_out};
     const char* names[] = {"q", "k", "v", "q_out"};
@@ -695,14 +700,15 @@ int bms_chunk_attention(const void* q, int32_t dtype, int64_t tokens, int64_t he
     if (window < 0 || sinks < 0) return fail(BMS_ERROR_INVALID_ARGUMENT, "window and sinks must not be negative");
     if (!std::isfinite(scale) || std::fabs(scale) > 1e30) return fail(BMS_ERROR_INVALID_ARGUMENT, "scale must be finite");
     if (q_stride == nullptr) return fail(BMS_ERROR_INVALID_ARGUMENT, "strides must not be NULL");
-    const int size = dtype == BMS_FLOAT32 ? 4 : 2;
-    RelaxedCapture relaxed;
-    BMS_CHECK(check_device(device));
-    BMS_CHECK(check_cache(cache, device, size));
+    BMS_CHECK(check_cache_shape(cache));
     if (cache->dim > 256) return fail(BMS_ERROR_UNSUPPORTED, "dim is at most 256");
     if (heads % cache->kv_heads != 0) return fail(BMS_ERROR_INVALID_ARGUMENT, "heads must be a multiple of the cache's kv_heads");
     if (tokens > 1073741823LL || width > 2147483391LL / cache->page_size)  // positions, rounded up to a tile, fit int32
         return fail(BMS_ERROR_UNSUPPORTED, "lengths beyond the 32-bit range");
+    const int size = dtype == BMS_FLOAT32 ? 4 : 2;
+    RelaxedCapture relaxed;
+    BMS_CHECK(check_device(device));
+    BMS_CHECK(check_cache(cache, device, size));
     BMS_CHECK(check_ptr(table, device, "table", 4));
     BMS_CHECK(check_ptr(seq_lens, device, "seq_lens", 4));
     BMS_CHECK(check_ptr(query_start, device, "query_start", 4));

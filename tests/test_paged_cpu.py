@@ -1,0 +1,181 @@
+"""Refusals of the paged-cache operators and the filtered sampler that need no GPU: the C entry points turn bad
+arguments away before they touch a device, the Python calls before they load the library."""
+
+import ctypes
+
+import pytest
+
+from bitmask_speculation_b200 import _native
+from bitmask_speculation_b200.build import build
+
+torch = pytest.importorskip("torch")
+INVALID, UNSUPPORTED = _native.ERROR_INVALID_ARGUMENT, _native.ERROR_UNSUPPORTED
+PTR = ctypes.c_void_p(256)  # never dereferenced: every call below is refused first
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build()
+    return _native.library()
+
+
+def pair(*x):
+    return (ctypes.c_int64 * 2)(*x)
+
+
+def cache(**change):
+    shape = dict(pages=4, page_size=16, kv_heads=2, dim=64)
+    shape.update({k: v for k, v in change.items() if k in shape})
+    strides = change.get("strides", (2048, 128, 64))
+    triple = ctypes.c_int64 * 3
+    return _native.Cache(256, 256, *shape.values(), triple(*strides), triple(*strides))
+
+
+# ---------------------------------------------------------------- C entry points
+def test_filtered_sample_refusals(lib):
+    def call(dtype=0, rows=1, vocab=32, temperature=1.0, top_p=1.0, min_p=0.0, top_k=0, masks=None, mask_rows=None, table=0, filt=True):
+        f = _native.Filter(temperature, top_p, min_p, top_k)
+        return lib.bms_filtered_sample_batch(PTR, dtype, masks, mask_rows, table, rows, vocab, ctypes.byref(f) if filt else None, PTR, PTR, PTR, PTR, 0, None)
+    nan, inf = float("nan"), float("inf")
+    for bad in (dict(dtype=3), dict(dtype=-1), dict(vocab=0), dict(vocab=2 ** 31), dict(rows=-1), dict(filt=False), dict(temperature=-0.5), dict(temperature=nan),
+                dict(temperature=inf), dict(top_p=0.0), dict(top_p=1.5), dict(top_p=nan), dict(min_p=-0.1), dict(min_p=1.1), dict(min_p=nan),
+                dict(top_k=-1), dict(mask_rows=PTR)):
+        assert call(**bad) == INVALID, bad
+        assert lib.bms_last_error()
+    assert call(vocab=2 ** 31 - 1) == UNSUPPORTED
+
+
+def test_page_plan_refusals(lib):
+    def call(seqs=2, width=4, pages=8, page=16, tokens=4):
+        return lib.bms_page_plan(PTR, PTR, PTR, seqs, PTR, width, PTR, pages, PTR, page, tokens, PTR, PTR, PTR, PTR, PTR, PTR, PTR, 0, None)
+    for bad in (dict(seqs=0), dict(seqs=-1), dict(width=0), dict(pages=0), dict(page=0), dict(page=-16), dict(tokens=-1)):
+        assert call(**bad) == INVALID, bad
+    for bad in (dict(seqs=8193), dict(pages=2 ** 30), dict(page=65537), dict(tokens=2 ** 30), dict(width=2 ** 30), dict(width=2 ** 28, page=16)):
+        assert call(**bad) == UNSUPPORTED, bad
+
+
+def test_rotary_append_refusals(lib):
+    def call(dtype=1, tokens=3, heads=4, qs=pair(256, 64), max_positions=32, c=cache()):
+        return lib.bms_rotary_append(PTR, PTR, PTR, dtype, tokens, heads, qs, pair(128, 64), pair(128, 64), PTR, PTR, max_positions, PTR, PTR, PTR,
+                                     None if c is None else ctypes.byref(c), None, 0, None)
+    for bad in (dict(dtype=5), dict(tokens=-1), dict(heads=0), dict(heads=65536), dict(qs=None), dict(max_positions=0), dict(c=None), dict(c=cache(dim=63)),
+                dict(c=cache(dim=0)), dict(c=cache(pages=0)), dict(c=cache(pages=2 ** 31)), dict(c=cache(page_size=0)), dict(c=cache(page_size=65537)),
+                dict(c=cache(kv_heads=0)), dict(c=cache(strides=(-1, 64, 64)))):
+        assert call(**bad) == INVALID, bad
+
+
+def test_chunk_attention_refusals(lib):
+    def call(dtype=1, tokens=3, heads=4, qs=pair(256, 64), c=cache(), seqs=2, width=4, scale=0.125, window=0, sinks=0):
+        return lib.bms_chunk_attention(PTR, dtype, tokens, heads, qs, None if c is None else ctypes.byref(c), PTR, seqs, width, PTR, PTR, scale, window, sinks,
+                                       PTR, PTR, PTR, PTR, 1 << 40, 0, None)
+    for bad in (dict(dtype=5), dict(tokens=-1), dict(heads=0), dict(heads=3), dict(heads=65536), dict(qs=None), dict(seqs=0), dict(seqs=2 ** 20 + 1),
+                dict(width=0), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=1e31), dict(window=-1), dict(sinks=-1), dict(c=None),
+                dict(c=cache(kv_heads=3)), dict(c=cache(strides=(2048, -128, 64)))):
+        assert call(**bad) == INVALID, bad
+    # Positions rounded up to a tile stay in 32 bits; the largest width passes this check (and then fails for want of a device).
+    for bad in (dict(c=cache(dim=257)), dict(tokens=2 ** 30), dict(width=2 ** 27), dict(width=(2 ** 31 - 257) // 16 + 1)):
+        assert call(**bad) == UNSUPPORTED, bad
+    for bad in ((0, -1, 1, 1, 64), (0, 1, 0, 1, 64), (0, 1, 1, 0, 64), (0, 1, 1, 1, 0), (-1, 1, 1, 1, 64), (64, 1, 1, 1, 64)):
+        assert lib.bms_attention_workspace_bytes(*bad) == -1, bad
+
+
+# ---------------------------------------------------------------- Python calls
+def fake_cuda():
+    """Tensors that claim to be on CUDA: the checks read metadata only."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    return FakeTensorMode()
+
+
+def test_cpu_tensors_are_never_transferred():
+    from bitmask_speculation_b200 import paged
+    from bitmask_speculation_b200.kernels.cuda import batched_filtered_sample
+    x = torch.zeros(2, 4, 8, 64, dtype=torch.bfloat16)
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="no implicit transfer"):
+        paged.PagedCache(x, x)
+    with pytest.raises(ValueError, match="no implicit transfer"):
+        paged.plan_pages(i, i, i, i[None], i, i[:1], page_size=4, tokens=1)
+    with pytest.raises(ValueError, match="no implicit transfer"):
+        batched_filtered_sample(torch.zeros(2, 64), None)
+    with pytest.raises(ValueError, match="CUDA"):
+        batched_filtered_sample(torch.zeros(2, 64), torch.zeros(2, 2, dtype=torch.int32))
+    for bad in (torch.zeros(2, 64, dtype=torch.float64), torch.zeros(2, 64, dtype=torch.int32), [[0.0]]):
+        with pytest.raises(TypeError):
+            batched_filtered_sample(bad, None)
+
+
+def test_cache_refusals():
+    from bitmask_speculation_b200.paged import PagedCache
+    with fake_cuda():
+        def t(*shape, dtype=torch.bfloat16, device="cuda"):
+            return torch.empty(shape, dtype=dtype, device=device)
+        ok = t(4, 16, 2, 64)
+        assert PagedCache(ok, ok).page_size == 16
+        PagedCache(t(4, 2, 16, 64).transpose(1, 2), ok)
+        for k, v, error in ((t(4, 16, 128), ok, ValueError), (ok, t(4, 16, 2, 32), ValueError), (ok, t(4, 16, 2, 64, dtype=torch.float16), ValueError),
+                            (t(4, 16, 2, 64, dtype=torch.float64), ok, TypeError), (None, ok, TypeError), (t(0, 16, 2, 64), t(0, 16, 2, 64), ValueError),
+                            (t(4, 16, 64, 2).transpose(2, 3), ok, ValueError), (t(1, 16, 2, 64).expand(4, 16, 2, 64), ok, ValueError),
+                            (t(4, 16, 2, 64, device="cpu"), ok, ValueError)):
+            with pytest.raises(error):
+                PagedCache(k, v)
+
+
+def test_plan_refusals():
+    from bitmask_speculation_b200.paged import plan_pages
+    with fake_cuda():
+        def t(*shape, dtype=torch.int32):
+            return torch.empty(shape, dtype=dtype, device="cuda")
+        good = dict(past_lens=t(3), new_lens=t(3), held=t(3), block_table=t(3, 8), free_pages=t(24), free_count=t(1), page_size=16, tokens=9)
+        for change, error in ((dict(past_lens=t(3, dtype=torch.int64)), TypeError), (dict(new_lens=t(4)), ValueError), (dict(held=t(6)[::2]), ValueError),
+                              (dict(block_table=t(2, 8)), ValueError), (dict(block_table=t(3, 0)), ValueError), (dict(block_table=t(8, 3).t()), ValueError),
+                              (dict(free_pages=t(0)), ValueError), (dict(free_count=t(2)), ValueError), (dict(page_size=0), ValueError),
+                              (dict(page_size=16.0), TypeError), (dict(page_size=True), TypeError), (dict(tokens=-1), ValueError), (dict(tokens=2.0), TypeError),
+                              (dict(past_lens=t(0), new_lens=t(0), held=t(0), block_table=t(0, 8)), ValueError)):
+            with pytest.raises(error):
+                plan_pages(**{**good, **change})
+
+
+def test_append_and_attention_refusals():
+    from bitmask_speculation_b200.paged import PagedCache, chunk_attention, rotary_append
+    with fake_cuda():
+        def t(*shape, dtype=torch.bfloat16):
+            return torch.empty(shape, dtype=dtype, device="cuda")
+        f32, i32, i64 = torch.float32, torch.int32, torch.int64
+        c = PagedCache(t(8, 16, 2, 64), t(8, 16, 2, 64))
+        good = dict(q=t(5, 4, 64), k=t(5, 2, 64), v=t(5, 2, 64), cos=t(40, 32, dtype=f32), sin=t(40, 32, dtype=f32), positions=t(5, dtype=i32),
+                    slots=t(5, dtype=i64), cache=c)
+        for change, error in ((dict(q=t(5, 4, 64, dtype=f32)), TypeError), (dict(q=t(5, 4, 32)), ValueError), (dict(q=t(5, 0, 64)), ValueError),
+                              (dict(k=t(4, 2, 64)), ValueError), (dict(v=t(5, 4, 64)), ValueError), (dict(q=t(5, 64, 4).transpose(1, 2)), ValueError),
+                              (dict(cos=t(40, 32)), TypeError), (dict(cos=t(40, 64, dtype=f32)), ValueError), (dict(sin=t(32, 40, dtype=f32).t()), ValueError),
+                              (dict(cos=t(0, 32, dtype=f32), sin=t(0, 32, dtype=f32)), ValueError), (dict(positions=t(4, dtype=i32)), ValueError),
+                              (dict(positions=t(5, dtype=i64)), TypeError), (dict(slots=t(5, dtype=i32)), TypeError), (dict(slots=t(10, dtype=i64)[::2]), ValueError),
+                              (dict(status=t(4, dtype=i32)), ValueError), (dict(out=t(5, 4, 64, dtype=f32)), TypeError),
+                              (dict(out=t(5, 8, 64)[:, ::2]), ValueError)):
+            with pytest.raises(error):
+                rotary_append(**{**good, **change})
+        good = dict(q=t(5, 4, 64), cache=c, block_table=t(3, 4, dtype=i32), seq_lens=t(3, dtype=i32), query_start=t(4, dtype=i32))
+        for change, error in ((dict(q=t(5, 3, 64)), ValueError), (dict(q=t(5, 4, 32)), ValueError), (dict(q=t(4, 64)), ValueError), (dict(block_table=t(2, 4, dtype=i32)), ValueError),
+                              (dict(block_table=t(3, 0, dtype=i32)), ValueError), (dict(seq_lens=t(3, dtype=i64)), TypeError), (dict(query_start=t(3, dtype=i32)), ValueError),
+                              (dict(window=-1), ValueError), (dict(window=1.5), TypeError), (dict(window=True), TypeError), (dict(sinks=-1), ValueError),
+                              (dict(scale="1"), TypeError), (dict(scale=float("nan")), ValueError), (dict(scale=float("inf")), ValueError), (dict(scale=True), TypeError),
+                              (dict(out=t(5, 4, 32)), ValueError)):
+            with pytest.raises(error):
+                chunk_attention(**{**good, **change})
+
+
+def test_filtered_sample_argument_refusals():
+    from bitmask_speculation_b200.kernels.cuda import batched_filtered_sample
+    with fake_cuda():
+        def t(*shape, dtype=torch.float32):
+            return torch.empty(shape, dtype=dtype, device="cuda")
+        i32 = torch.int32
+        logits, mask = t(3, 70), t(3, 3, dtype=i32)
+        for change, error in ((dict(mask=t(3, 2, dtype=i32)), ValueError), (dict(mask=t(3, 3)), TypeError), (dict(mask=None, mask_rows=t(3, dtype=i32)), ValueError),
+                              (dict(mask_rows=t(2, dtype=i32)), ValueError), (dict(mask_rows=t(3, dtype=torch.int64)), TypeError), (dict(mask=t(0, 3, dtype=i32), mask_rows=t(3, dtype=i32)), ValueError),
+                              (dict(logits=t(70, 3).t()), ValueError), (dict(logits=t(3, 0), mask=None), ValueError),
+                              (dict(temperature=-1), ValueError), (dict(temperature=float("nan")), ValueError), (dict(temperature="1"), TypeError), (dict(temperature=True), TypeError),
+                              (dict(temperature=t(2)), ValueError), (dict(temperature=t(3, dtype=torch.float64)), TypeError), (dict(top_k=-1), ValueError), (dict(top_k=1.0), TypeError),
+                              (dict(top_k=t(3)), TypeError), (dict(top_p=0.0), ValueError), (dict(top_p=1.01), ValueError), (dict(min_p=-0.01), ValueError), (dict(min_p=2), ValueError),
+                              (dict(min_p=t(6)[::2]), ValueError)):
+            with pytest.raises(error):
+                batched_filtered_sample(**{**dict(logits=logits, mask=mask), **change})
