@@ -88,8 +88,8 @@ class PagePlan:
 @dataclass(frozen=True, slots=True)
 class ChunkAttention:
     """``out`` [tokens, heads, dim], ``lse`` float32 [tokens, heads] (natural log of the sum of
-    exponentials) and a status per sequence (0; 6: lengths that do not fit; 11: a page outside the
-    cache; the rows of a failed sequence are 0 with lse -inf)."""
+    exponentials) and a status per sequence (0; 6: lengths that do not fit; 7: a wait inside the kernel gave up;
+    11: a page outside the cache; the rows of a failed sequence are 0 with lse -inf)."""
 
     out: object
     lse: object
@@ -148,7 +148,7 @@ def rotary_append(q, k, v, cos, sin, positions, slots, cache: PagedCache, *, out
     gives them.  Element i and i + dim / 2 of a head turn together; sums are float32, rounded once.  A
     token with slot -1 writes no key or value; one with position -1 nothing, its row of the result is
     left as it was (unspecified when ``out`` is not given).  ``out``: a contiguous tensor shaped like ``q`` for
-    the result.  ``status``: an int32 [N] tensor for a code per token (0; 11: a slot outside the cache;
+    the result (a contiguous ``q`` itself may be given).  ``status``: an int32 [N] tensor for a code per token (0; 11: a slot outside the cache;
     12: a position outside the tables; such tokens write nothing).
     """
     import torch
@@ -192,6 +192,7 @@ def chunk_attention(q, cache: PagedCache, block_table, seq_lens, query_start, *,
     ``scale`` is 1 / sqrt(dim) unless given.  Keys that a row does not see never reach it, whatever
     they hold.  ``block_table`` int32 [S, width], ``seq_lens`` int32 [S], ``query_start`` int32
     [S + 1].  Rows behind the last sequence are left as they were (unspecified when ``out`` is not given).
+    A row whose visible scores are all -inf is NaN with lse -inf.  ``out`` must not overlap the inputs.
     """
     import torch
     dtype, dev = cache.k.dtype, cache.k.device

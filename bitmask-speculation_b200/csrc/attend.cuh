@@ -721,7 +721,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
                     ref = best;
                 }
             }
-            const float inv = sum != 0.f ? 1.f / sum : 0.f;
+            const float inv = sum != 0.f || whole ? 1.f / sum : 0.f;  // a part may see none of a row's keys; a whole row only with scores of -inf: NaN
             mine_w *= inv, other_w *= inv;
             constexpr int kPart = D / 2;
 #pragma unroll 1

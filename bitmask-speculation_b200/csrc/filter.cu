@@ -1140,19 +1140,19 @@ __device__ __noinline__ bool find_nucleus(Shared& sh, const RowView<T>& shared_v
             int kept;
             double mass;
             const uint64_t key = list_cut(sh, static_cast<int>(n), n, sh.top_p, above, below, kept, mass);
-        const double limit = sh.top_p * (above + mass + below);
+            const double limit = sh.top_p * (above + mass + below);
             // Outside the bracket: not one of its tokens kept, or all of them with more below.
             const bool ends_inside = kept > 0 && (above + mass >= limit || b1 == kBins - 1);
             if (ends_inside) {
                 // The bracket's kept tokens join their spans as integers: the order of the additions does not matter.
-                    for (int i = threadIdx.x; i < c * kWarps; i += kThreads) sh.extra[i] = 0;
+                for (int i = threadIdx.x; i < c * kWarps; i += kThreads) sh.extra[i] = 0;
                 if (threadIdx.x == 0) sh.passed = 0;
                 __syncthreads();
                 uint32_t passed = 0;
                 for (int i = threadIdx.x; i < n; i += kThreads) {
-                const Place at = place_of(sh.list[i]);
-                if (sh.list[i] < key || at.x < sh.floor_x) continue;
-                ++passed;
+                    const Place at = place_of(sh.list[i]);
+                    if (sh.list[i] < key || at.x < sh.floor_x) continue;
+                    ++passed;
                     const int64_t g = (static_cast<int64_t>(at.t) + shared_view.skew) / RowView<T>::kVec;
                     int q = static_cast<int>(g * c / groups);  // the CTA whose slice [groups q / c, groups (q + 1) / c) holds g
                     while (g >= groups * (q + 1) / c) ++q;
@@ -1539,6 +1539,7 @@ extern "C" int bms_filtered_sample_batch(const void* logits, int32_t dtype, cons
     BMS_CHECK(check_ptr(tokens, device, "tokens", 8));
     BMS_CHECK(check_ptr(kept, device, "kept", 8));
     BMS_CHECK(check_ptr(status, device, "status", 4));
+    if (device >= kMaxDevices) return fail(BMS_ERROR_UNSUPPORTED, "device %d", device);
     DeviceGuard guard;
     BMS_CUDA(guard.enter(device), "cudaSetDevice");
     const FilterParams p{logits, masks, mask_rows, mask_table_rows, rows, vocab, (vocab + 31) / 32, f.temperature, f.top_p, f.min_p, f.top_k,

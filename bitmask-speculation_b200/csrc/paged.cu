@@ -409,7 +409,7 @@ __device__ void attend_row(const AttendParams& p, int s, int64_t token, int head
         for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
         const float mn = fmaxf(m, mx);
         const float keep = m == -INFINITY ? 0.f : exp2f(m - mn);
-        const float w = live ? exp2f(x - mn) : 0.f;
+        const float w = live && x != -INFINITY ? exp2f(x - mn) : 0.f;  // while all scores are -inf the maximum is, too
         float sum = w;
 #pragma unroll
         for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -491,8 +491,10 @@ bool tiles_fit(const AttendParams& p, int dtype) {
     if (tc::kTile / std::min(p.page_size, tc::kTile) > 16 || p.heads / p.kv_heads > tc::kTile || encode_tiled() == nullptr) return false;
     for (const void* x : {p.q, p.k, p.v, static_cast<const void*>(p.out)})
         if (reinterpret_cast<uintptr_t>(x) % 16 != 0) return false;
-    for (const int64_t s : {p.q_tok, p.q_head, p.k_page, p.k_slot, p.k_head, p.v_page, p.v_slot, p.v_head})
-        if (s % 8 != 0 || s >= (1LL << 38)) return false;
+    const int64_t strides[][2] = {{p.q_tok, p.tokens}, {p.q_head, p.heads}, {p.k_page, p.pages}, {p.k_slot, p.page_size}, {p.k_head, p.kv_heads},
+                                  {p.v_page, p.pages}, {p.v_slot, p.page_size}, {p.v_head, p.kv_heads}};
+    for (const auto& [s, n] : strides)  // a tensor map has no stride of 0: broadcast inputs go row by row
+        if (s % 8 != 0 || s >= (1LL << 38) || (s == 0 && n > 1)) return false;
     return true;
 }
 
@@ -716,6 +718,7 @@ int bms_chunk_attention(const void* q, int32_t dtype, int64_t tokens, int64_t he
     if (tokens > 0) {
         BMS_CHECK(check_ptr(q, device, "q", size));
         BMS_CHECK(check_ptr(out, device, "out", size));
+        if (out == q) return fail(BMS_ERROR_INVALID_ARGUMENT, "out must not be q");  // rows are read again after others are written
         if (lse != nullptr) BMS_CHECK(check_ptr(lse, device, "lse", 4));
     }
     const int64_t need = bms_attention_workspace_bytes(device, tokens, heads, seqs, cache->dim);

@@ -360,10 +360,10 @@ BMS_API int bms_page_plan(const int32_t *past_lens, const int32_t *new_lens, con
  * dim], k and v [tokens, kv_heads, dim] with the given token and head strides (elements; dim is
  * contiguous and even).  With half = dim / 2, element i < half and i + half of a head at position p
  * become a cos[p, i] - b sin[p, i] and a sin[p, i] + b cos[p, i]; cos and sin are float32
- * [max_positions, half].  Sums in float32, rounded once.  q_out is contiguous [tokens, heads, dim];
- * token t's key and value go to slot slots[t].  A token with slots[t] < 0 writes no key or value, one
- * with positions[t] < 0 nothing at all.  `status` (int32 [tokens], may be NULL): 11 for a slot at or
- * past the cache's end, 12 for a position at or past max_positions (such a token writes nothing).
+ * [max_positions, half].  Sums in float32, rounded once.  q_out is contiguous [tokens, heads, dim] and
+ * may be q itself where q is contiguous; token t's key and value go to slot slots[t].  A token with
+ * slots[t] < 0 writes no key or value, one with positions[t] < 0 nothing at all.  `status` (int32
+ * [tokens], may be NULL): 11 for a slot at or past the cache's end, 12 for a position at or past max_positions (such a token writes nothing).
  * Slots of one call are distinct (plan_pages gives such slots); of equal ones either may win. */
 BMS_API int bms_rotary_append(const void *q, const void *k, const void *v, int32_t dtype, int64_t tokens, int64_t heads,
                               const int64_t q_stride[2], const int64_t k_stride[2], const int64_t v_stride[2],
@@ -383,8 +383,9 @@ BMS_API int64_t bms_attention_workspace_bytes(int32_t device, int64_t tokens, in
  * [tokens, heads], may be NULL) the natural log of the sum of exp(scale q.k).  heads is a multiple of
  * kv_heads; head h reads key head h / (heads / kv_heads).  dim is at most 256.  Keys that a row does
  * not see do not reach it, whatever their bits.  Per-sequence status: 6 for query_start out of order or beyond
- * `tokens`, seq_lens below n or above the table row; 11 for a visible page outside the cache; the
- * rows of a failed sequence are 0 with lse -inf.  Rows behind query_start[seqs] are left as they
+ * `tokens`, seq_lens below n or above the table row; 11 for a visible page outside the cache; 7 where a
+ * wait inside the kernel gave up; the rows of a failed sequence are 0 with lse -inf.  A row whose visible
+ * scores are all -inf is NaN with lse -inf.  `out` must not overlap the inputs.  Rows behind query_start[seqs] are left as they
  * were. */
 BMS_API int bms_chunk_attention(const void *q, int32_t dtype, int64_t tokens, int64_t heads, const int64_t q_stride[2],
                                 const bms_paged_cache *cache, const int32_t *table, int64_t seqs, int64_t width,

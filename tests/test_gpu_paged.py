@@ -532,3 +532,42 @@ def test_rounds_of_plan_append_attend(cuda_module, dtype):
             ks, vs = (torch.stack([pair[i] for pair in kept[s]])[None] for i in range(2))
             want = definition(turned[rows], ks, vs, i32([[0]]), [(new[s], past[s])], 0, 0, dim ** -0.5)
             assert_close(type(got)(got.out[rows], got.lse[rows], got.status), want, dtype, dim)
+
+
+def test_broadcast_queries(cuda_module):
+    """Queries expanded over heads or tokens (strides of 0)."""
+    from bitmask_speculation_b200.paged import PagedCache, chunk_attention
+    lens = [(9, 200), (70, 30), (1, 5)]
+    q, k, v, table, seq_lens, starts = make_case(lens, 8, 2, 64, 16, torch.bfloat16)
+    for rows in (q[:, :1].expand(-1, 8, -1), q[:1].expand(80, -1, -1)):
+        got = chunk_attention(rows, PagedCache(k, v), table, seq_lens, starts)
+        assert_close(got, definition(rows.contiguous(), k, v, table, lens, 0, 0, 0.125), torch.bfloat16, 64)
+
+
+@pytest.mark.parametrize("dtype,dim,page", [(torch.bfloat16, 64, 16), (torch.float16, 128, 64), (torch.bfloat16, 64, 5), (torch.float32, 32, 16)])
+def test_scores_of_minus_infinity(cuda_module, dtype, dim, page):
+    """A row that sees only scores of -inf is NaN with lse -inf, in items of one CTA and in ones that several share."""
+    from bitmask_speculation_b200.paged import PagedCache, chunk_attention
+    lens = [(1, 3), (9, 5000), (150, 20)]
+    q, k, v, table, seq_lens, starts = make_case(lens, 2, 1, dim, page, dtype)
+    q.zero_()
+    q[..., 0] = -math.inf
+    k.fill_(1)
+    got = chunk_attention(q, PagedCache(k, v), table, seq_lens, starts).check()
+    assert bool(got.out.isnan().all()) and bool((got.lse == -math.inf).all())
+
+
+def test_append_in_place_and_output_that_is_the_input(cuda_module):
+    from bitmask_speculation_b200.paged import PagedCache, chunk_attention, rotary_append
+    for dtype, dim in ((torch.bfloat16, 64), (torch.float32, 6)):
+        gen = torch.Generator(device="cuda").manual_seed(2)
+        q = torch.randn((50, 4, dim), generator=gen, device="cuda").to(dtype)
+        k, v = (torch.randn((50, 2, dim), generator=gen, device="cuda").to(dtype) for _ in range(2))
+        cos, sin = (torch.randn((64, dim // 2), generator=gen, device="cuda") for _ in range(2))
+        cache = PagedCache.allocate(8, 16, 2, dim, dtype=dtype)
+        at = torch.arange(50, dtype=torch.int32, device="cuda")
+        want = rotary_append(q, k, v, cos, sin, at, at.long(), cache)
+        got = rotary_append(q, k, v, cos, sin, at, at.long(), cache, out=q)
+        assert got is q and torch.equal(got, want)
+        with pytest.raises(RuntimeError, match="must not be q"):
+            chunk_attention(q, cache, torch.arange(8, dtype=torch.int32, device="cuda")[None], i32([50]), i32([0, 50]), out=q)
