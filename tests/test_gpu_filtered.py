@@ -283,3 +283,34 @@ def test_refusals(cuda_module):
         call(x, None, mask_rows=torch.zeros(2, dtype=torch.int32, device="cuda"))
     with pytest.raises(TypeError):
         call(x.double(), mask)
+
+
+SPREADS = {
+    "tiny": lambda rng, n: rng.standard_normal(n) * 1e-3,
+    "zeros": lambda rng, n: rng.choice([0.0, -0.0, 1e-4, -1e-4, 0.5, -0.5], n),
+    "around_zero": lambda rng, n: rng.standard_normal(n) * 0.02,
+    "negative": lambda rng, n: rng.standard_normal(n) * 2 - 40,
+    "just_negative": lambda rng, n: -np.abs(rng.standard_normal(n)) * 0.3 - 0.001,
+    "high": lambda rng, n: rng.standard_normal(n) * 0.6 + 100,
+    "coarse": lambda rng, n: np.round(rng.standard_normal(n) * 2),
+    "wide": lambda rng, n: rng.standard_normal(n) * 10.0 ** rng.uniform(-6, 4, n),
+    "outlier": lambda rng, n: np.where(np.arange(n) == n // 2, 3e4, rng.standard_normal(n) * 3),
+}
+
+
+@pytest.mark.parametrize("rows", [6, 150, 700])
+@pytest.mark.parametrize("spread", list(SPREADS))
+def test_spreads_of_scores(cuda_module, spread, rows):
+    """Rows beyond the list path whose filters end near zero, far below the maximum, among equal scores, on either side of
+    zero; with one CTA per row and with several."""
+    rng = np.random.default_rng(rows + len(spread))
+    vocab = 9973 if rows > 6 else 40009
+    values = SPREADS[spread](rng, rows * vocab).reshape(rows, vocab).astype(np.float32)
+    valid = rng.random((rows, vocab)) < rng.choice([1.0, 0.85, 0.6], rows)[:, None]
+    valid[:, 5] = True
+    scale = {"wide": 3e3, "outlier": 2e4, "high": 0.5}.get(spread, 1.0)
+    cases = (dict(top_p=0.31371), dict(top_p=0.90713), dict(top_p=0.99931, temperature=7.0 * scale), dict(top_k=5003, temperature=scale),
+             dict(top_k=vocab // 2, top_p=0.70717, temperature=2 * scale), dict(top_p=0.93711, min_p=0.03, temperature=scale))
+    for i, params in enumerate(cases if rows < 700 else cases[1:5:2]):
+        for dtype in DTYPES if rows == 6 else ("bfloat16",):
+            check(values, valid, dtype, params, rng.random(rows), offset=3 * i)
