@@ -46,7 +46,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 16;
 constexpr int kCap = 4096;   // tokens that the list path holds
-constexpr int kSegment = 512;  // of them in one warp's span
+constexpr int kSegment = 480;  // of them in one warp's span (two CTAs fill an SM's shared memory)
 constexpr int kTable = 512;    // powers 2^(j / 512)
 constexpr int kBins = 4096;   // value bins of the counting pass
 // A warp's queue: 63 tokens left over and a round of one 16-byte vector per lane.
@@ -97,11 +97,12 @@ struct MassCount {
     int64_t count;
 };
 
-// A warp's rounds in flight: a vector per lane, copied without registers (cp.async); a lane reads only
-// what it copied itself, so no barrier is needed.  (Loads ahead into rotating registers stall at the first move.)
+// A warp's rounds in flight: a vector per lane and the round's mask words, copied without registers (cp.async).  (Loads
+// ahead into rotating registers stall at the first move.)
 constexpr int kAhead = 4;
 struct Ring {
     uint4 vec[kAhead][32];
+    uint32_t mask[kAhead][12];
 };
 
 struct Shared {
@@ -263,35 +264,43 @@ struct RowView {
     __device__ __forceinline__ bool valid(int32_t t) const { return mask == nullptr || (static_cast<uint32_t>(mask[t >> 5]) >> (t & 31) & 1); }
 };
 
-// The full groups of a warp's span, a round of one vector per lane at a time, kAhead - 1 rounds ahead (the mask bits one).
+// The full groups of a warp's span, a round of one vector per lane at a time, kAhead - 1 rounds ahead.  Callers pass through a
+// warp-wide vote between two rounds, so that no lane's copy overwrites mask words that another one has yet to read.
 template <typename T>
 struct Stream {
+    static constexpr int kVec = RowView<T>::kVec;
+    static constexpr int kWords = (31 + 32 * kVec - 1) / 32 + 1;  // that a round's bits can touch
     const RowView<T>& v;
     Ring& ring;
     int32_t z, lane;
     int32_t g, ahead;  // this lane's groups: of the current round, of the next one to copy
     int32_t slot = 0;
-    uint32_t word;     // mask bits of the next round
     __device__ __forceinline__ void copy(int to) {
         if (ahead < z) ptx::cp_async_16(ptx::smem_addr(&ring.vec[to][lane]), reinterpret_cast<const uint4*>(v.row - v.skew) + ahead);
+        if (v.mask != nullptr && lane < kWords && ahead - lane < z) {  // like the vectors, only what some round takes: the space has later uses
+            const uint32_t w = (static_cast<uint32_t>(v.first(ahead - lane)) >> 5) + lane;
+            if (w <= (v.vocab - 1) >> 5) ptx::cp_async_4(ptx::smem_addr(&ring.mask[to][lane]), v.mask + w);
+        }
         asm volatile("cp.async.commit_group;" ::: "memory");
         ahead += 32;
     }
-    __device__ __forceinline__ uint32_t bits_of(int32_t at) const { return at < z ? v.bits(at) : 0u; }
     __device__ __forceinline__ Stream(const RowView<T>& view, Ring& r, int32_t g0, int32_t g1) : v(view), ring(r), z(min(g1, view.full1)), lane(threadIdx.x & 31) {
         g = ahead = max(g0, view.full0) + lane;
         for (int i = 0; i < kAhead - 1; ++i) copy(i);
-        word = bits_of(g);
     }
     __device__ __forceinline__ bool more() const { return g - lane < z; }
     // The current round's vector, and its bits (0 behind the span's end); starts the copy of a later one.
     __device__ __forceinline__ uint32_t take(uint4& now) {
-        const uint32_t bits = word;
-        word = bits_of(g + 32);
         copy((slot + kAhead - 1) % kAhead);
         asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+        __syncwarp();
         now = ring.vec[slot][lane];
-        return bits;
+        if (g >= z) return 0;
+        if (v.mask == nullptr) return RowView<T>::kAll;
+        const uint32_t t = static_cast<uint32_t>(v.first(g)), w = (t >> 5) - (static_cast<uint32_t>(v.first(g - lane)) >> 5), sh = t & 31;
+        uint32_t b = ring.mask[slot][w] >> sh;
+        if (sh > 32 - kVec) b |= ring.mask[slot][w + 1] << (32 - sh);
+        return b & RowView<T>::kAll;
     }
     __device__ __forceinline__ void next() { slot = (slot + 1) % kAhead, g += 32; }
     // Element j of the current round's vector.
@@ -720,6 +729,15 @@ __device__ __noinline__ uint64_t bisect(Shared& sh, const RowView<T>& view, uint
 template <typename T>
 __device__ __forceinline__ void append(uint64_t* segment, uint32_t& fill, uint32_t in, const Stream<T>& stream, int32_t t) {
     const int lane = threadIdx.x & 31;
+    if (!__any_sync(0xffffffffu, in & (in - 1))) {  // at most one per lane
+        const uint32_t who = __ballot_sync(0xffffffffu, in != 0), to = fill + __popc(who & ((1u << lane) - 1u));
+        if (in && to < kSegment) {
+            const int j = __ffs(in) - 1;
+            segment[to] = order_key(stream.element(j), static_cast<uint32_t>(t + j));
+        }
+        fill += __popc(who);
+        return;
+    }
     uint32_t run = __popc(in);
     uint32_t at = fill - run;
 #pragma unroll
@@ -819,11 +837,12 @@ __device__ __noinline__ RowStats first_pass(Shared& sh, const RowView<T>& shared
             max_a = fmaxf(max_a, a), max_b = fmaxf(max_b, o);
             best = fmaxf(a, o);
         }
-        if (__any_sync(0xffffffffu, least == -INFINITY)) finite -= __popc(bits & ~reaching<T>(now, bits, -FLT_MAX));  // valid, never drawn
+        const bool never = __any_sync(0xffffffffu, least == -INFINITY);
+        if (never) finite -= __popc(bits & ~reaching<T>(now, bits, -FLT_MAX));  // valid, never drawn
         if (fill <= kSegment && __any_sync(0xffffffffu, best >= low)) {
             // No room for a whole round: drop what the bound has passed.  What stays full is given up.
             if (fill + 32 * kVec > kSegment && mode) fill = filter(segment, fill, low);
-            append<T>(segment, fill, reaching<T>(now, bits, low), stream, view.first(stream.g));
+            append<T>(segment, fill, mode == 0 && !never ? bits : reaching<T>(now, bits, low), stream, view.first(stream.g));
             if (mode) {
                 if constexpr (sizeof(T) == 2) max_a = Pair<T>::lo(max2), max_b = Pair<T>::hi(max2);
                 const float lane_bound = fmaxf(max_a, max_b);
