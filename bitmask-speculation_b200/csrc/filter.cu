@@ -122,6 +122,7 @@ struct Shared {
             uint32_t bins[kBins];    // this CTA's counts, until every CTA has read them
             uint32_t merged[kBins];  // the row's counts
         };
+        double score_weight[kBins];  // bfloat16: of the kept scores
         Ring first_ring[kWarps];  // of the passes that collect, which write the list at their end
     };
     union {
@@ -153,7 +154,7 @@ struct Shared {
     // The cut by exact scores: tokens above `threshold` are kept, and the first `ties` at it.
     float threshold;
     int32_t ties, tie_limit;  // of the row; of the drawn token's span
-    int32_t k_bin, k_need;
+    int32_t k_bin, k_need;    // the last kept bin, and how many of its tokens
     struct Outside {
         double mass;
         int64_t count;
@@ -269,23 +270,30 @@ struct RowView {
 template <typename T>
 struct Stream {
     static constexpr int kVec = RowView<T>::kVec;
-    static constexpr int kWords = (31 + 32 * kVec - 1) / 32 + 1;  // that a round's bits can touch
+    static constexpr int kWords = kVec + 1;  // mask words that a round's 32 kVec bits can touch; rounds are whole words apart
     const RowView<T>& v;
     Ring& ring;
+    const uint4* from;     // this lane's next vector to copy
+    const int32_t* words;  // its next mask word to copy, among the round's
+    const int32_t* words_end;
     int32_t z, lane;
-    int32_t g, ahead;  // this lane's groups: of the current round, of the next one to copy
-    int32_t slot = 0;
-    __device__ __forceinline__ void copy(int to) {
-        if (ahead < z) ptx::cp_async_16(ptx::smem_addr(&ring.vec[to][lane]), reinterpret_cast<const uint4*>(v.row - v.skew) + ahead);
-        if (v.mask != nullptr && lane < kWords && ahead - lane < z) {  // like the vectors, only what some round takes: the space has later uses
-            const uint32_t w = (static_cast<uint32_t>(v.first(ahead - lane)) >> 5) + lane;
-            if (w <= (v.vocab - 1) >> 5) ptx::cp_async_4(ptx::smem_addr(&ring.mask[to][lane]), v.mask + w);
-        }
+    int32_t g, ahead;      // this lane's groups: of the current round, of the next one to copy
+    uint32_t slot = 0;
+    uint32_t shift, word;  // where this lane's bits start in every round's words
+    __device__ __forceinline__ void copy(uint32_t to) {
+        if (ahead < z) ptx::cp_async_16(ptx::smem_addr(&ring.vec[to][lane]), from);
+        // Like the vectors, only what some round takes: the space has later uses.
+        if (words < words_end && ahead - lane < z) ptx::cp_async_4(ptx::smem_addr(&ring.mask[to][lane]), words);
         asm volatile("cp.async.commit_group;" ::: "memory");
-        ahead += 32;
+        ahead += 32, from += 32, words += kVec;
     }
     __device__ __forceinline__ Stream(const RowView<T>& view, Ring& r, int32_t g0, int32_t g1) : v(view), ring(r), z(min(g1, view.full1)), lane(threadIdx.x & 31) {
         g = ahead = max(g0, view.full0) + lane;
+        from = reinterpret_cast<const uint4*>(v.row - v.skew) + ahead;
+        const uint32_t t0 = static_cast<uint32_t>(v.first(g - lane)), t = static_cast<uint32_t>(v.first(g));
+        word = (t >> 5) - (t0 >> 5), shift = t & 31;
+        words = v.mask + (t0 >> 5) + lane;
+        words_end = v.mask != nullptr && lane < kWords ? v.mask + ((v.vocab - 1) >> 5) + 1 : words;
         for (int i = 0; i < kAhead - 1; ++i) copy(i);
     }
     __device__ __forceinline__ bool more() const { return g - lane < z; }
@@ -297,10 +305,7 @@ struct Stream {
         now = ring.vec[slot][lane];
         if (g >= z) return 0;
         if (v.mask == nullptr) return RowView<T>::kAll;
-        const uint32_t t = static_cast<uint32_t>(v.first(g)), w = (t >> 5) - (static_cast<uint32_t>(v.first(g - lane)) >> 5), sh = t & 31;
-        uint32_t b = ring.mask[slot][w] >> sh;
-        if (sh > 32 - kVec) b |= ring.mask[slot][w + 1] << (32 - sh);
-        return b & RowView<T>::kAll;
+        return __funnelshift_r(ring.mask[slot][word], ring.mask[slot][word + 1], shift) & RowView<T>::kAll;
     }
     __device__ __forceinline__ void next() { slot = (slot + 1) % kAhead, g += 32; }
     // Element j of the current round's vector.
@@ -345,10 +350,10 @@ __device__ __forceinline__ uint32_t reaching(const uint4& now, uint32_t bits, fl
 // Calls f(x, token, live) for the valid tokens of the warp's span.  Rounds (one vector per lane) in which every token is
 // valid go straight from the registers, unrolled; in others the valid tokens go through the warp's queue in shared
 // memory, two per lane at a time, so that f's cost follows their number and not the vocabulary (grammar
-// masks keep 0.1 - 60 % of it).  kLow: only tokens with x >= low.  A queue entry is 16 bits of score and 16 of offset for 16-bit types, 8 bytes
+// masks keep 0.1 - 60 % of it).  A queue entry is 16 bits of score and 16 of offset for 16-bit types, 8 bytes
 // for float32.
-template <bool kLow = false, typename T, typename F>
-__device__ __forceinline__ void each_token(Shared& sh, const RowView<T>& v, F f, float low = -INFINITY) {
+template <typename T, typename F>
+__device__ __forceinline__ void each_token(Shared& sh, const RowView<T>& v, F f) {
     constexpr bool kHalf = sizeof(T) == 2;
     constexpr int kVec = RowView<T>::kVec;
     constexpr int kGroups = 65536 / kVec;  // offsets stay within 16 bits
@@ -366,12 +371,8 @@ __device__ __forceinline__ void each_token(Shared& sh, const RowView<T>& v, F f,
         int fill = 0;
         for (Stream<T> stream(v, sh.ring[warp], base, last); stream.more(); stream.next()) {
             uint4 now;
-            uint32_t bits = stream.take(now);
+            const uint32_t bits = stream.take(now);
             const uint32_t at = (stream.g - base) * kVec;
-            if constexpr (kLow) {
-                if (bits) bits = reaching<T>(now, bits, low);
-                if (!__any_sync(0xffffffffu, bits != 0)) continue;
-            }
             if (__all_sync(0xffffffffu, bits == RowView<T>::kAll)) {
                 float x[kVec];
                 v.expand(now, x);
@@ -443,8 +444,7 @@ __device__ __forceinline__ void each_token(Shared& sh, const RowView<T>& v, F f,
     }
     const int32_t t = v.edge(g0, g1);
     if (__any_sync(0xffffffffu, t >= 0)) {
-        float x = t >= 0 && v.valid(t) ? widen(v.row[t]) : -INFINITY;
-        if (kLow && x < low) x = -INFINITY;
+        const float x = t >= 0 && v.valid(t) ? widen(v.row[t]) : -INFINITY;
         f(x, static_cast<uint32_t>(t), x > -INFINITY);
     }
 }
@@ -840,6 +840,10 @@ __device__ __noinline__ RowStats first_pass(Shared& sh, const RowView<T>& shared
         const bool never = __any_sync(0xffffffffu, least == -INFINITY);
         if (never) finite -= __popc(bits & ~reaching<T>(now, bits, -FLT_MAX));  // valid, never drawn
         if (fill <= kSegment && __any_sync(0xffffffffu, best >= low)) {
+            if (mode == 0 && fill + __reduce_add_sync(0xffffffffu, __popc(bits)) * ((stream.z - stream.g + lane) / 32) > 2 * kSegment) {
+                fill = kSegment + 1;  // as dense as this, the span would not fit
+                continue;
+            }
             // No room for a whole round: drop what the bound has passed.  What stays full is given up.
             if (fill + 32 * kVec > kSegment && mode) fill = filter(segment, fill, low);
             append<T>(segment, fill, mode == 0 && !never ? bits : reaching<T>(now, bits, low), stream, view.first(stream.g));
@@ -1417,31 +1421,79 @@ __device__ __noinline__ bool cut_scores(Shared& sh, int c, bool k_cuts) {
     }
     if (threadIdx.x == 0) {
         const float x = bin_score(sh.k_bin, top_rank);
-        sh.threshold = fmaxf(x, sh.floor_x);  // min-p keeps every token at its score
-        sh.ties = x < sh.floor_x ? kAllTies : sh.k_need;
+        sh.threshold = fmaxf(x, sh.floor_x);
+        if (x < sh.floor_x) {  // min-p keeps every token at its score: the last bin that reaches it
+            int lo = 0, hi = sh.k_bin;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if (bin_score(mid, top_rank) >= sh.floor_x) lo = mid;
+                else hi = mid - 1;
+            }
+            sh.k_bin = lo, sh.k_need = kAllTies;
+        }
+        sh.ties = sh.k_need;
     }
     __syncthreads();
     return true;
 }
 
-// Masses of the tokens above sh.threshold by spans, their number, and the tokens at it by spans, to rank 0.
+// Masses of the kept tokens by spans, less the ones at the last score where some of those are dropped, the number of
+// these by spans, and the number of the others, to rank 0.
 template <typename T>
 __device__ __noinline__ void weigh_kept(Shared& sh, const RowView<T>& shared_view) {
     cg::cluster_group cluster = cg::this_cluster();
     const RowView<T> view = shared_view;
+    constexpr int kVec = RowView<T>::kVec;
     const int rank = cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const double top = sh.top, rate = sh.rate;
+    const int32_t top_rank = sh.top_rank, g0 = sh.bounds[warp], g1 = sh.bounds[warp + 1];
+    const uint32_t whole = sh.ties == kAllTies ? sh.k_bin + 1 : sh.k_bin;  // bins below it are kept whole
+    for (int b = threadIdx.x; b <= sh.k_bin; b += kThreads) sh.score_weight[b] = weight_of(bin_score(b, top_rank), sh.top, sh.rate, sh.exp_table);
+    __syncthreads();
     const float threshold = sh.threshold;
     double mass = 0.0;
     int count = 0, ties = 0;
-    each_token<true>(sh, view, [&](float x, uint32_t, bool live) {
-        if (!live) return;
-        if (x > threshold) mass += weight_of(x, top, rate, sh.exp_table), ++count;
-        else ++ties;
-    }, threshold);
+    auto take = [&](uint32_t u) {  // true for a token near zero
+        const uint32_t bin = static_cast<uint32_t>(score_bin(u, top_rank));
+        if (bin < whole) mass += sh.score_weight[bin], ++count;
+        else ties += bin == whole;
+        return bin == 0xffffffffu;
+    };
+    auto near_zero = [&](uint32_t u) {
+        const float x = Pair<T>::lo(u);
+        if (x >= threshold) mass += weight_of(x, sh.top, sh.rate, sh.exp_table), ++count;
+    };
+#pragma unroll 1
+    for (Stream<T> stream(view, sh.ring[warp], g0, g1); stream.more(); stream.next()) {
+        uint4 now;
+        uint32_t bits = stream.take(now);
+        if (bits) bits = reaching<T>(now, bits, threshold);  // few tokens are kept of many: cheaper than their bins
+        const int most = __reduce_max_sync(0xffffffffu, __popc(bits));
+        uint32_t near = 0;
+        if (most > 3) {
+            const uint32_t w[4] = {now.x, now.y, now.z, now.w};
+#pragma unroll
+            for (int j = 0; j < kVec; ++j)
+                if ((bits >> j & 1) && take(w[j >> 1] >> (j & 1 ? 16 : 0) & 0xffffu)) near |= 1u << j;
+        } else {
+#pragma unroll 1
+            for (uint32_t rest = bits; rest; rest &= rest - 1) {
+                const int j = __ffs(rest) - 1;
+                if (take(stream.raw_element(j))) near |= 1u << j;
+            }
+        }
+        if (__any_sync(0xffffffffu, near != 0)) {
+#pragma unroll 1
+            for (; near; near &= near - 1) near_zero(stream.raw_element(__ffs(near) - 1));
+        }
+    }
+    const int32_t t = view.edge(g0, g1);
+    if (t >= 0 && view.valid(t)) {
+        const uint32_t u = __float_as_uint(widen(view.row[t])) >> 16;
+        if (take(u)) near_zero(u);
+    }
+    if (sh.ties == kAllTies) ties = 0;  // the first bin that is not kept
     mass = warp_sum(mass);
     count = __reduce_add_sync(0xffffffffu, count), ties = __reduce_add_sync(0xffffffffu, ties);
-    __syncthreads();
     if (lane == 0) {
         sh.warp_count[warp] = count;
         *cluster.map_shared_rank(&sh.spans[rank * kWarps + warp], 0) = mass;
@@ -1484,35 +1536,71 @@ __device__ __noinline__ uint32_t lowest_at(Shared& sh, const RowView<T>& shared_
     return sh.pick;
 }
 
-// Walks the span that holds the target, one token per thread and round, to the drawn token (sh.token).  Of the tokens up to
-// `end` that score as it does, the span keeps the first `ties`.
+// Finds the drawn token (sh.token) in the span that holds the target: every warp weighs a part of it, and the part that holds
+// the target is walked, one token per thread and round.  Of the tokens up to `end` that score as it does, the span keeps the
+// first `ties`.  (Walking the whole span took 94 us of the 1,152 rows' 750, this way 20.)
 template <typename T>
 __device__ __noinline__ void walk_span(Shared& sh, const RowView<T>& shared_view, int span, Place end, int32_t ties) {
     const RowView<T> view = shared_view;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const double target = sh.target;
     double before = sh.before;
-    const int32_t s0 = max(view.first(sh.bounds[span]), 0);
-    const int32_t s1 = static_cast<int32_t>(min(static_cast<int64_t>(view.vocab), static_cast<int64_t>(sh.bounds[span + 1]) * RowView<T>::kVec - view.skew));
+    int32_t s0 = max(view.first(sh.bounds[span]), 0);
+    int32_t s1 = static_cast<int32_t>(min(static_cast<int64_t>(view.vocab), static_cast<int64_t>(sh.bounds[span + 1]) * RowView<T>::kVec - view.skew));
+    auto score = [&](int32_t t) {  // of a token up to `end`, else -inf
+        const float x = t < s1 && view.valid(t) ? widen(view.row[t]) : -INFINITY;
+        return end.keeps(x, static_cast<uint32_t>(t)) ? x : -INFINITY;
+    };
+    auto weigh = [&](float x) { return weight_of(x, sh.top, sh.rate, sh.exp_table); };
     if (threadIdx.x == 0) sh.token = -1;
+    const int32_t part = ((s1 - s0 + kWarps - 1) / kWarps + 31) & ~31;
+    const int32_t stop = min(s1, s0 + (warp + 1) * part);
+    double mass = 0.0;
+    int equal = 0;
+#pragma unroll 4
+    for (int32_t t = s0 + warp * part + lane; t < stop; t += 32) {
+        const float x = score(t);
+        if (ties != kAllTies && x == end.x) ++equal;
+        else if (x > -INFINITY) mass += weigh(x);
+    }
+    mass = warp_sum(mass);
+    equal = __reduce_add_sync(0xffffffffu, equal);
+    __syncthreads();
+    if (lane == 0) sh.warp_mass[warp] = mass, sh.warp_count[warp] = equal;
+    __syncthreads();
+    // The first part whose running mass exceeds the target; without one (rounding at the very end) the last with mass.
+    double run = before, from = before;
+    int32_t left = ties, left_from = ties, owner = 0;
+    const double one = ties != kAllTies ? weigh(end.x) : 0.0;
+    for (int w = 0; w < kWarps; ++w) {
+        const int32_t keep = min(static_cast<int32_t>(sh.warp_count[w]), left);
+        const double m = sh.warp_mass[w] + keep * one;
+        if (m > 0.0) owner = w, from = run, left_from = left;
+        run += m;
+        if (ties != kAllTies) left -= keep;
+        if (m > 0.0 && run > target) break;
+    }
+    before = from, ties = left_from;
+    s0 += owner * part;
+    s1 = min(s1, s0 + part);
     for (int32_t base = s0; base < s1; base += kThreads) {
         const int32_t t = base + threadIdx.x;
-        double w = 0.0;
-        const float x = t < s1 && view.valid(t) ? widen(view.row[t]) : -INFINITY;
-        bool in = x > -INFINITY && end.keeps(x, static_cast<uint32_t>(t));
+        const float x = score(t);
+        bool in = x > -INFINITY;
         if (ties != kAllTies) {
             int64_t all;
             const int64_t ahead = block_before(static_cast<int64_t>(in && x == end.x), sh.warp_count, all);
             in = in && (x != end.x || ahead < ties);
             ties -= static_cast<int32_t>(min(all, static_cast<int64_t>(ties)));
         }
-        if (in) w = weight_of(x, sh.top, sh.rate, sh.exp_table);
+        const double w = in ? weigh(x) : 0.0;
         double all;
-        const double run = before + block_before(w, sh.warp_mass, all) + w;
-        // The first token that crosses the target; without one (rounding at the very end) the last one with mass.
+        const double run_here = before + block_before(w, sh.warp_mass, all) + w;
+        // The first token that crosses the target; without one the last one with mass.
         if (threadIdx.x == 0) sh.pick = 0xffffffffu, sh.last = 0;
         __syncthreads();
         if (w > 0.0) {
-            if (run > target) atomicMin(&sh.pick, threadIdx.x);
+            if (run_here > target) atomicMin(&sh.pick, threadIdx.x);
             atomicMax(&sh.last, threadIdx.x + 1);
         }
         __syncthreads();
