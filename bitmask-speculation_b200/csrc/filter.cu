@@ -1856,10 +1856,11 @@ int launch_filter(const FilterParams& p, int device, cudaStream_t stream) {
         BMS_CUDA(cudaDeviceGetAttribute(&sms[device], cudaDevAttrMultiProcessorCount, device), "sm count");
         ready[device] = true;
     }
-    // CTAs per row.  Few rows are split for latency (8 rows of 248,320: 74 / 41 / 30 / 26 us with 1 / 2 / 4 / 8); up to two rows per SM,
-    // 4 keep one slow row (a wide nucleus) from ending the launch alone (256 mixed rows: 342 / 243 / 231 / 294 us); many rows keep the
-    // SMs busy by themselves (1,152 rows: 1.15 / 1.17 / 1.42 ms with 1 / 2 / 4).
-    int c = p.rows * 8 <= sms[device] ? 8 : p.rows <= 2 * sms[device] ? 4 : p.rows <= 4 * sms[device] ? 2 : 1;
+    // CTAs per row.  Few rows are split for latency, as long as the parts run side by side (two CTAs per SM): with 1 / 2 / 4 / 8 CTAs,
+    // rows of 151,936 with top-p 0.9 take 107 / 66 / 46 / 37 us for 8 of them, 108 / 66 / 46 / 52 for 32, 108 / 67 / 65 / 99 for 64
+    // and 108 / 96 / 125 / 184 for 128; 64 float32 rows of 50,257 with min-p 54 / 36 / 25 with 1 / 2 / 4.  Two keep a row that takes long (a wide nucleus) from ending the launch alone: 256 rows of
+    // mixed filters and masks take 166 / 133 / 149 / 224 us.  Many rows keep the SMs busy by themselves (600: 398 / 405 / 505 / 799).
+    int c = p.rows * 16 <= sms[device] ? 8 : p.rows * 2 <= sms[device] ? 4 : p.rows <= 2 * sms[device] ? 2 : 1;
     while (c > 1 && p.vocab / c < 4096) c /= 2;
     if (p.rows * c > 2147483647LL) return fail(BMS_ERROR_UNSUPPORTED, "too many rows");
     cudaLaunchConfig_t cfg{};
