@@ -588,8 +588,11 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
         const int wg = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t s_addr = lane_base + wg * kTile, o_addr = lane_base + 2 * kTile + wg * D;
-        uint32_t seq = 0, s_round = 0, o_round = 0;
-        for (; walk.valid(p); walk.next(p)) {
+        uint32_t seq = 0, s_round = 0, o_round = 0, item = 0;
+        for (; walk.valid(p); walk.next(p), ++item) {
+            // A warpgroup without a tile in this item has nothing else to wait for: it must not release the next item's queries
+            // before the other one is done with this item's.
+            wait_bar(ctl, &ctl.q_full, item & 1);
             const Range& r = walk.range;
             const bool wide = walk.shape.wide;
             const int t0 = walk.tile0(), n = walk.tile1() - t0;

@@ -571,3 +571,15 @@ def test_append_in_place_and_output_that_is_the_input(cuda_module):
         assert got is q and torch.equal(got, want)
         with pytest.raises(RuntimeError, match="must not be q"):
             chunk_attention(q, cache, torch.arange(8, dtype=torch.int32, device="cuda")[None], i32([50]), i32([0, 50]), out=q)
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim,page", [(torch.bfloat16, 16, 8, 64, 16), (torch.float16, 8, 8, 128, 32), (torch.bfloat16, 28, 4, 128, 128)])
+@pytest.mark.parametrize("longest", [1, 120, 129, 300, 700])
+def test_many_short_sequences(cuda_module, dtype, heads, kv_heads, dim, page, longest):
+    """Several items per CTA, most of them of a single key tile, in which one half of the softmax threads has nothing to do."""
+    rng = np.random.default_rng(longest)
+    lens = [(1, int(x)) for x in rng.integers(0, longest, 260)]
+    check_attention(lens, heads, kv_heads, dim, page, dtype)
+    mixed = [(int(n), int(x)) for n, x in zip(rng.choice([0, 1, 1, 1, 9, 40, 150], 150), rng.integers(0, longest, 150))]
+    check_attention(mixed, heads, kv_heads, dim, page, dtype)
+    check_attention(mixed, heads, kv_heads, dim, page, dtype, window=50, sinks=3)
