@@ -352,12 +352,14 @@ class NativeModule:
         n, heads, _ = q.shape
         if n == 0:
             return
-        pair = ctypes.c_int64 * 2
+        (q0, q1, _), (k0, k1, _), (v0, v1, _) = q.stride(), k.stride(), v.stride()
+        strides = (ctypes.c_int64 * 6)(q0, q1, k0, k1, v0, v1)
+        at = ctypes.addressof(strides)
         dev = q.device
         _native.check(self._lib.bms_rotary_append(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), _dtype_code(q), n, heads, pair(*q.stride()[:2]), pair(*k.stride()[:2]),
-            pair(*v.stride()[:2]), cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(), slots.data_ptr(),
-            out.data_ptr(), self._cache(cache), None if status is None else status.data_ptr(), dev.index, _stream(dev)))
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), _dtype_code(q), n, heads, at, at + 16, at + 32, cos.data_ptr(),
+            sin.data_ptr(), cos.shape[0], positions.data_ptr(), slots.data_ptr(), out.data_ptr(), self._cache(cache),
+            None if status is None else status.data_ptr(), dev.index, _stream(dev)))
 
     def chunk_attention(self, q, cache, table, seq_lens, query_start, scale, window, sinks, out):
         """``bms_chunk_attention`` with scratch from the caching allocator (its own in every call and every

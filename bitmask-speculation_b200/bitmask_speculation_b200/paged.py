@@ -238,7 +238,7 @@ def _positive_int(value, name: str) -> None:
 
 
 def _row_strides(t, name: str) -> None:
-    if t.numel() and (t.stride(2) != 1 and t.shape[2] > 1 or min(t.stride()) < 0):
+    if t.stride(2) != 1 and t.shape[2] > 1 and t.numel():
         raise ValueError(f"{name}'s last dimension must be contiguous")
 
 

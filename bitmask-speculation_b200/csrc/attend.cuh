@@ -23,6 +23,15 @@
 // 0 * NaN is NaN.  In tiles that are not seen by every row, non-finite values of keys that some row does not see are
 // zeroed in shared memory before the product; if another row does see such a key the CTA flags its range, and
 // attend_finish_kernel computes those items again row by row.
+//
+// Bound.  Prompt chunks (dim 128) run at 0.87 PFLOP/s, 1.0 in the steady state: a warpgroup's step is a chain (scores 0.4 us,
+// load 0.1, maximum 0.15, exponentials 1.2, second half of the output product 0.2), and the two warpgroups' chains overlap; TMEM
+// has no room for a second score tile of each (2 x 128 columns of scores, 2 x 128 of output).  Verification windows over long
+// caches read them at 4.3 TB/s (6.5 in the steady state).  What is lost lies between items, about 14 us of it per CTA and item
+// (output, first scores), at the start (13 us to the first scores, the search for the part's start and cold code in it)
+// and in the joining kernel (18 - 27 us for the longest cases); single tokens over short caches take 24 us of that alone.
+// Tried without gain: a warp of its own for the cleaning of values, handing the first half of the weights over later, looking up
+// the joined items before the tiles are done.
 #pragma once
 #include <cuda.h>
 

@@ -5,6 +5,11 @@
 // top_k tokens; of their total mass the tokens whose preceding mass is below top_p * total; the tokens
 // with w >= min_p.  The result is the lowest kept token whose running mass in token order exceeds u * kept mass.
 //
+// Bound.  A row has to be read once (497 KB for 248,320 bfloat16 scores), which is the first pass's work: 0.21 ms of the
+// 0.66 for 1,152 rows whose bytes alone take 0.09.  All passes issue instructions at 70 % of what the schedulers can: a round
+// of 256 tokens costs a warp about 120 in the first pass, twice that where a sparse mask's tokens are kept.  Few rows are
+// bound by latency: 8 rows with top-k 20 us, 7 of them the first pass.
+//
 // A cluster of C CTAs owns a row, each CTA a contiguous slice, each warp a contiguous span of it.  The
 // row is streamed from HBM once (maximum, counts, NaN); later passes hit L2, because only the rows in
 // flight are live there.  A place in the order is a score and a token (`Place`); every filter ends at one.
@@ -21,7 +26,7 @@
 //    bracket's tokens, whose sorted prefix gives the exact end; if the estimate missed, the exact masses place
 //    the next bracket, and if a bracket overflows (runs of equal scores) the end is bisected over the
 //    64-bit order keys instead.  (bfloat16 rows whose filters end near zero go this way, too.)  By scores 1,152 rows of
-//    248,320 with top-p take 0.84 ms, by brackets 1.15.
+//    248,320 with top-p took 0.84 ms, by brackets 1.15; with the streams below 0.66.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -1538,7 +1543,7 @@ __device__ __noinline__ uint32_t lowest_at(Shared& sh, const RowView<T>& shared_
 
 // Finds the drawn token (sh.token) in the span that holds the target: every warp weighs a part of it, and the part that holds
 // the target is walked, one token per thread and round.  Of the tokens up to `end` that score as it does, the span keeps the
-// first `ties`.  (Walking the whole span took 94 us of the 1,152 rows' 750, this way 20.)
+// first `ties`.  (Walking the whole span took 40 us more of 750 for 1,152 rows.)
 template <typename T>
 __device__ __noinline__ void walk_span(Shared& sh, const RowView<T>& shared_view, int span, Place end, int32_t ties) {
     const RowView<T> view = shared_view;
