@@ -6,7 +6,7 @@
 // with w >= min_p.  The result is the lowest kept token whose running mass in token order exceeds u * kept mass.
 //
 // Bound.  A row has to be read once (497 KB for 248,320 bfloat16 scores), which is the first pass's work: 0.21 ms of the
-// 0.66 for 1,152 rows whose bytes alone take 0.09.  All passes issue instructions at 70 % of what the schedulers can: a round
+// 0.64 for 1,152 rows whose bytes alone take 0.09.  All passes issue instructions at 70 % of what the schedulers can: a round
 // of 256 tokens costs a warp about 120 in the first pass, twice that where a sparse mask's tokens are kept.  Few rows are
 // bound by latency: 8 rows with top-k 20 us, 7 of them the first pass.
 //
@@ -26,7 +26,7 @@
 //    bracket's tokens, whose sorted prefix gives the exact end; if the estimate missed, the exact masses place
 //    the next bracket, and if a bracket overflows (runs of equal scores) the end is bisected over the
 //    64-bit order keys instead.  (bfloat16 rows whose filters end near zero go this way, too.)  By scores 1,152 rows of
-//    248,320 with top-p took 0.84 ms, by brackets 1.15; with the streams below 0.66.
+//    248,320 with top-p took 0.84 ms, by brackets 1.15; with the present streams 0.64.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -602,6 +602,181 @@ __device__ __noinline__ uint64_t list_cut(Shared& sh, int n, int64_t k, double p
     return (static_cast<uint64_t>(bits) << 32) | (0xffffffffu - cut_t);
 }
 
+// bfloat16 scores.  A row's scores are few: 128 per octave.  So a bin per score holds the whole row, but for magnitudes below
+// 2^-7 (octaves without end; 0.3 % of normal logits) and for what lies 4,096 scores below the maximum.  The masses by bin
+// are then exact, count times weight, with a weight per score and not per token, and the filters' end follows from them: a
+// score, and how many of the tokens at it are kept.  One pass counts, one weighs the kept tokens by spans.
+template <typename T>
+constexpr bool kScoreBins = std::is_same_v<T, __nv_bfloat16>;
+
+// A score's rank is 0 at 2^-7, grows with the score from there on, and is -1 at -2^-7 (and for a maximum near zero); its bin
+// is how far it lies below the maximum.
+__device__ __forceinline__ int32_t score_rank(uint32_t u) {
+    const int32_t d = static_cast<int32_t>(u & 0x7fffu) - kNear;
+    return d < 0 ? -1 : d ^ -static_cast<int32_t>(u >> 15);
+}
+
+// -1: near zero; kBins and more: below the bins.
+__device__ __forceinline__ int32_t score_bin(uint32_t u, int32_t top_rank) {
+    const int32_t d = static_cast<int32_t>(u & 0x7fffu) - kNear;
+    const int32_t bin = top_rank - (d ^ -static_cast<int32_t>(u >> 15));
+    return d < 0 ? -1 : bin;
+}
+
+__device__ __forceinline__ float bin_score(int32_t bin, int32_t top_rank) {
+    const int32_t rank = top_rank - bin;
+    const uint32_t u = rank >= 0 ? rank + kNear : 0x8000u | static_cast<uint32_t>(~rank + kNear);
+    return __uint_as_float(u << 16);
+}
+
+// The end of the first k tokens and of the nucleus among them, from counts by score and c CTAs' sh.outside: sh.threshold and sh.ties; false where
+// it lies among the tokens without a bin.  Every CTA computes the same.
+__device__ __noinline__ bool cut_scores(Shared& sh, const uint32_t* counts, int c, bool k_cuts) {
+    const int32_t top_rank = sh.top_rank, near_at = max(top_rank + 1, 0);  // the tokens near zero come before this bin
+    Shared::Outside near{0.0, 0}, low{0.0, 0};
+    for (int i = 0; i < c; ++i) {
+        near.mass += sh.outside[0][i].mass, near.count += sh.outside[0][i].count;
+        low.mass += sh.outside[1][i].mass, low.count += sh.outside[1][i].count;
+    }
+    if (near_at >= kBins) low.mass += near.mass, low.count += near.count;
+    const int first = threadIdx.x * kPerThread;
+    double mass = 0.0;
+    int64_t count = 0;
+    // Calls f(bin, tokens, weight) for this thread's bins in order; the tokens near zero are bin -1 and weigh their whole mass.
+    auto each_bin = [&](auto f) {
+#pragma unroll 1
+        for (int b = first; b < first + kPerThread; ++b) {
+            if (b == near_at && near.count) f(-1, near.count, near.mass);
+            const uint32_t n = counts[b];
+            if (n) f(b, static_cast<int64_t>(n), weight_of(bin_score(b, top_rank), sh.top, sh.rate, sh.exp_table));
+        }
+    };
+    each_bin([&](int b, int64_t n, double w) { mass += b < 0 ? w : n * w, count += n; });
+    double all_mass;
+    int64_t all_count;
+    const double mass_before = block_before(mass, sh.warp_mass, all_mass);
+    const int64_t count_before = block_before(count, sh.warp_count, all_count);
+    const int64_t k = sh.k;
+    if (threadIdx.x == 0) sh.found = 1, sh.k_bin = kBins, sh.last = 0, sh.target = all_mass + low.mass;
+    __syncthreads();
+    if (k_cuts) {
+        if (k > all_count) return false;
+        if (count_before < k && k <= count_before + count) {
+            int64_t n0 = count_before;
+            double m = mass_before;
+            bool done = false;
+            each_bin([&](int b, int64_t n, double w) {
+                if (done) return;
+                if (k > n0 + n) {
+                    n0 += n, m += b < 0 ? w : n * w;
+                    return;
+                }
+                done = true;
+                if (b < 0) sh.found = 0;
+                sh.k_bin = b, sh.k_need = static_cast<int32_t>(k - n0);
+                sh.target = m + (k - n0) * w;
+            });
+        }
+        __syncthreads();
+        if (!sh.found) return false;
+    }
+    if (sh.top_p < 1.0) {
+        const double limit = sh.top_p * sh.target;
+        if (!k_cuts && low.count && all_mass < limit) return false;
+        // The last thread with tokens before which the mass is below the limit holds the end.
+        if (count && (mass_before < limit)) atomicMax(&sh.last, threadIdx.x + 1);
+        __syncthreads();
+        if (threadIdx.x + 1 == sh.last) {
+            double m = mass_before, before = 0.0, weight = 0.0;
+            int bin = -1;
+            int64_t tokens = 0;
+            each_bin([&](int b, int64_t n, double w) {
+                if (m < limit || bin < 0 && tokens == 0) bin = b, tokens = n, before = m, weight = w;
+                m += b < 0 ? w : n * w;
+            });
+            int64_t j = 1;  // tokens at the score that the nucleus keeps: (j - 1) of their weights lie below the limit
+            for (int64_t bit = 1ll << 30; bit; bit >>= 1)
+                if (j + bit <= tokens && before + (j + bit - 1) * weight < limit) j += bit;
+            if (bin < 0) sh.found = 0;
+            if (bin < sh.k_bin || (bin == sh.k_bin && j < sh.k_need)) sh.k_bin = bin, sh.k_need = j == tokens ? kAllTies : static_cast<int32_t>(j);
+        }
+        __syncthreads();
+        if (!sh.found) return false;
+    }
+    if (threadIdx.x == 0) {
+        const float x = bin_score(sh.k_bin, top_rank);
+        sh.threshold = fmaxf(x, sh.floor_x);
+        if (x < sh.floor_x) {  // min-p keeps every token at its score: the last bin that reaches it
+            int lo = 0, hi = sh.k_bin;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if (bin_score(mid, top_rank) >= sh.floor_x) lo = mid;
+                else hi = mid - 1;
+            }
+            sh.k_bin = lo, sh.k_need = kAllTies;
+        }
+        sh.ties = sh.k_need;
+    }
+    __syncthreads();
+    return true;
+}
+
+// list_cut for bfloat16 by counts of the list's scores: the order key of the last kept token, or 0 where they do not give it.
+// (256 rows of mixed filters 131 us by bisection and 126 by counts, 1,152 rows with top-p 659 and 635.)
+__device__ __noinline__ uint64_t list_cut_scores(Shared& sh, int n, bool k_cuts) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int32_t top_rank = sh.top_rank;
+    static_assert(sizeof sh.segment >= kBins * sizeof(uint32_t), "space of the counts");
+    uint32_t* counts = reinterpret_cast<uint32_t*>(sh.segment);  // their tokens are in the list
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += kThreads) counts[i] = 0;
+    __syncthreads();
+    double near_mass = 0.0, low_mass = 0.0;
+    int near_count = 0, low_count = 0;
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const float x = order_value(static_cast<uint32_t>(sh.list[i] >> 32));
+        const int32_t bin = score_bin(__float_as_uint(x) >> 16, top_rank);
+        if (static_cast<uint32_t>(bin) < kBins) {
+            atomicAdd(&counts[bin], 1u);
+            continue;
+        }
+        const double w = weight_of(x, sh.top, sh.rate, sh.exp_table);
+        if (bin < 0) near_mass += w, ++near_count;
+        else low_mass += w, ++low_count;
+    }
+    near_mass = warp_sum(near_mass), low_mass = warp_sum(low_mass);
+    near_count = __reduce_add_sync(0xffffffffu, near_count), low_count = __reduce_add_sync(0xffffffffu, low_count);
+    if (lane == 0) {
+        sh.warp_mass[warp] = near_mass, sh.warp_below[warp] = low_mass;
+        sh.warp_count[warp] = static_cast<int64_t>(low_count) << 32 | static_cast<uint32_t>(near_count);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        Shared::Outside near{0.0, 0}, low{0.0, 0};
+        for (int w = 0; w < kWarps; ++w) {
+            near.mass += sh.warp_mass[w], near.count += sh.warp_count[w] & 0xffffffff;
+            low.mass += sh.warp_below[w], low.count += sh.warp_count[w] >> 32;
+        }
+        sh.outside[0][0] = near, sh.outside[1][0] = low;
+    }
+    __syncthreads();
+    if (!cut_scores(sh, counts, 1, k_cuts)) return 0;
+    const uint32_t bits = order_bits(sh.threshold);
+    if (sh.ties == kAllTies) return static_cast<uint64_t>(bits) << 32;
+    // The list is in token order: its entry that is the last kept one of the threshold's.
+    const int per = (n + kThreads - 1) / kThreads, first = threadIdx.x * per;
+    int mine = 0, all;
+    for (int i = first; i < min(first + per, n); ++i) mine += static_cast<uint32_t>(sh.list[i] >> 32) == bits;
+    const int ahead = block_before(mine, reinterpret_cast<int*>(sh.warp_count), all);
+    if (ahead < sh.ties && sh.ties <= ahead + mine) {
+        int left = sh.ties - ahead;
+        for (int i = first; left; ++i)
+            if (static_cast<uint32_t>(sh.list[i] >> 32) == bits && --left == 0) sh.cut = sh.list[i];
+    }
+    __syncthreads();
+    return sh.cut;
+}
+
 // The list path: the tokens in play are in sh.list, in token order.  Cuts, weighs and draws.
 __device__ __noinline__ void finish_list(Shared& sh, int n, int64_t* token, int64_t* kept_out) {
     const double top = sh.top, rate = sh.rate, p = sh.top_p, u = sh.u;
@@ -635,7 +810,8 @@ __device__ __noinline__ void finish_list(Shared& sh, int n, int64_t* token, int6
     } else if (k < n || p < 1.0) {
         int kept;
         double mass;
-        cut = list_cut(sh, n, k, p, 0.0, 0.0, kept, mass);
+        if (sh.shift == 16) cut = list_cut_scores(sh, n, k < n);
+        if (cut == 0) cut = list_cut(sh, n, k, p, 0.0, 0.0, kept, mass);
     }
     cut = max(cut, static_cast<uint64_t>(order_bits(floor_x)) << 32);
     // Running masses in token order, consecutive tokens per thread.
@@ -1245,33 +1421,6 @@ __device__ __noinline__ bool find_nucleus(Shared& sh, const RowView<T>& shared_v
     return found;
 }
 
-// bfloat16 scores.  A row's scores are few: 128 per octave.  So a bin per score holds the whole row, but for magnitudes below
-// 2^-7 (octaves without end; 0.3 % of normal logits) and for what lies 4,096 scores below the maximum.  The masses by bin
-// are then exact, count times weight, with a weight per score and not per token, and the filters' end follows from them: a
-// score, and how many of the tokens at it are kept.  One pass counts, one weighs the kept tokens by spans.
-template <typename T>
-constexpr bool kScoreBins = std::is_same_v<T, __nv_bfloat16>;
-
-// A score's rank is 0 at 2^-7, grows with the score from there on, and is -1 at -2^-7 (and for a maximum near zero); its bin
-// is how far it lies below the maximum.
-__device__ __forceinline__ int32_t score_rank(uint32_t u) {
-    const int32_t d = static_cast<int32_t>(u & 0x7fffu) - kNear;
-    return d < 0 ? -1 : d ^ -static_cast<int32_t>(u >> 15);
-}
-
-// -1: near zero; kBins and more: below the bins.
-__device__ __forceinline__ int32_t score_bin(uint32_t u, int32_t top_rank) {
-    const int32_t d = static_cast<int32_t>(u & 0x7fffu) - kNear;
-    const int32_t bin = top_rank - (d ^ -static_cast<int32_t>(u >> 15));
-    return d < 0 ? -1 : bin;
-}
-
-__device__ __forceinline__ float bin_score(int32_t bin, int32_t top_rank) {
-    const int32_t rank = top_rank - bin;
-    const uint32_t u = rank >= 0 ? rank + kNear : 0x8000u | static_cast<uint32_t>(~rank + kNear);
-    return __uint_as_float(u << 16);
-}
-
 // Counts by score in sh.merged, tokens without a bin in sh.outside; the same in every CTA.
 template <typename T>
 __device__ __noinline__ void count_scores(Shared& sh, const RowView<T>& shared_view) {
@@ -1348,98 +1497,6 @@ __device__ __noinline__ void count_scores(Shared& sh, const RowView<T>& shared_v
         sh.merged[i] = n;
     }
     cluster.sync();
-}
-
-// The end of the first k tokens and of the nucleus among them, from the counts by score: sh.threshold and sh.ties; false where
-// it lies among the tokens without a bin.  Every CTA computes the same.
-__device__ __noinline__ bool cut_scores(Shared& sh, int c, bool k_cuts) {
-    const int32_t top_rank = sh.top_rank, near_at = max(top_rank + 1, 0);  // the tokens near zero come before this bin
-    Shared::Outside near{0.0, 0}, low{0.0, 0};
-    for (int i = 0; i < c; ++i) {
-        near.mass += sh.outside[0][i].mass, near.count += sh.outside[0][i].count;
-        low.mass += sh.outside[1][i].mass, low.count += sh.outside[1][i].count;
-    }
-    if (near_at >= kBins) low.mass += near.mass, low.count += near.count;
-    const int first = threadIdx.x * kPerThread;
-    double mass = 0.0;
-    int64_t count = 0;
-    // Calls f(bin, tokens, weight) for this thread's bins in order; the tokens near zero are bin -1 and weigh their whole mass.
-    auto each_bin = [&](auto f) {
-#pragma unroll 1
-        for (int b = first; b < first + kPerThread; ++b) {
-            if (b == near_at && near.count) f(-1, near.count, near.mass);
-            const uint32_t n = sh.merged[b];
-            if (n) f(b, static_cast<int64_t>(n), weight_of(bin_score(b, top_rank), sh.top, sh.rate, sh.exp_table));
-        }
-    };
-    each_bin([&](int b, int64_t n, double w) { mass += b < 0 ? w : n * w, count += n; });
-    double all_mass;
-    int64_t all_count;
-    const double mass_before = block_before(mass, sh.warp_mass, all_mass);
-    const int64_t count_before = block_before(count, sh.warp_count, all_count);
-    const int64_t k = sh.k;
-    if (threadIdx.x == 0) sh.found = 1, sh.k_bin = kBins, sh.last = 0, sh.target = all_mass + low.mass;
-    __syncthreads();
-    if (k_cuts) {
-        if (k > all_count) return false;
-        if (count_before < k && k <= count_before + count) {
-            int64_t n0 = count_before;
-            double m = mass_before;
-            bool done = false;
-            each_bin([&](int b, int64_t n, double w) {
-                if (done) return;
-                if (k > n0 + n) {
-                    n0 += n, m += b < 0 ? w : n * w;
-                    return;
-                }
-                done = true;
-                if (b < 0) sh.found = 0;
-                sh.k_bin = b, sh.k_need = static_cast<int32_t>(k - n0);
-                sh.target = m + (k - n0) * w;
-            });
-        }
-        __syncthreads();
-        if (!sh.found) return false;
-    }
-    if (sh.top_p < 1.0) {
-        const double limit = sh.top_p * sh.target;
-        if (!k_cuts && low.count && all_mass < limit) return false;
-        // The last thread with tokens before which the mass is below the limit holds the end.
-        if (count && (mass_before < limit)) atomicMax(&sh.last, threadIdx.x + 1);
-        __syncthreads();
-        if (threadIdx.x + 1 == sh.last) {
-            double m = mass_before, before = 0.0, weight = 0.0;
-            int bin = -1;
-            int64_t tokens = 0;
-            each_bin([&](int b, int64_t n, double w) {
-                if (m < limit || bin < 0 && tokens == 0) bin = b, tokens = n, before = m, weight = w;
-                m += b < 0 ? w : n * w;
-            });
-            int64_t j = 1;  // tokens at the score that the nucleus keeps: (j - 1) of their weights lie below the limit
-            for (int64_t bit = 1ll << 30; bit; bit >>= 1)
-                if (j + bit <= tokens && before + (j + bit - 1) * weight < limit) j += bit;
-            if (bin < 0) sh.found = 0;
-            if (bin < sh.k_bin || (bin == sh.k_bin && j < sh.k_need)) sh.k_bin = bin, sh.k_need = j == tokens ? kAllTies : static_cast<int32_t>(j);
-        }
-        __syncthreads();
-        if (!sh.found) return false;
-    }
-    if (threadIdx.x == 0) {
-        const float x = bin_score(sh.k_bin, top_rank);
-        sh.threshold = fmaxf(x, sh.floor_x);
-        if (x < sh.floor_x) {  // min-p keeps every token at its score: the last bin that reaches it
-            int lo = 0, hi = sh.k_bin;
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) / 2;
-                if (bin_score(mid, top_rank) >= sh.floor_x) lo = mid;
-                else hi = mid - 1;
-            }
-            sh.k_bin = lo, sh.k_need = kAllTies;
-        }
-        sh.ties = sh.k_need;
-    }
-    __syncthreads();
-    return true;
 }
 
 // Masses of the kept tokens by spans, less the ones at the last score where some of those are dropped, the number of
@@ -1730,7 +1787,7 @@ __global__ void __launch_bounds__(kThreads, 2) filter_sample_kernel(const Filter
     if constexpr (kScoreBins<T>) {
         if (k_cuts || top_p < 1.0) {
             count_scores<T>(sh, view);
-            by_score = cut_scores(sh, c, k_cuts);
+            by_score = cut_scores(sh, sh.merged, c, k_cuts);
             if (by_score) weigh_kept<T>(sh, view);
         }
     }

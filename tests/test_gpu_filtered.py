@@ -314,3 +314,18 @@ def test_spreads_of_scores(cuda_module, spread, rows):
     for i, params in enumerate(cases if rows < 700 else cases[1:5:2]):
         for dtype in DTYPES if rows == 6 else ("bfloat16",):
             check(values, valid, dtype, params, rng.random(rows), offset=3 * i)
+
+
+@pytest.mark.parametrize("spread", list(SPREADS))
+def test_spreads_of_short_rows(cuda_module, spread):
+    """The same spreads in rows, and sparse masks of longer rows, that fit the list of 4,096 tokens."""
+    rng = np.random.default_rng(len(spread))
+    scale = {"wide": 3e3, "outlier": 2e4, "high": 0.5}.get(spread, 1.0)
+    for rows, vocab, density in ((40, 3001, (1.0, 0.7, 0.3)), (9, 60013, (0.06, 0.03, 0.012))):
+        values = SPREADS[spread](rng, rows * vocab).reshape(rows, vocab).astype(np.float32)
+        valid = rng.random((rows, vocab)) < rng.choice(density, rows)[:, None]
+        valid[:, 5] = True
+        for i, params in enumerate((dict(top_p=0.31371), dict(top_p=0.99931, temperature=7.0 * scale), dict(top_k=703, temperature=scale),
+                                    dict(top_k=1511, top_p=0.70717, temperature=2 * scale), dict(top_p=0.93711, min_p=0.03, temperature=scale))):
+            for dtype in DTYPES:
+                check(values, valid, dtype, params, rng.random(rows), offset=3 * i)
