@@ -28,9 +28,10 @@ from .kernels._validation import device_tensor, index_tensor
 class PagedCache:
     """Keys and values in pages: ``k`` and ``v`` [pages, page_size, kv_heads, dim], float32, bfloat16 or
     float16, on one CUDA device, ``dim`` contiguous, any other strides (a [pages, kv_heads, page_size,
-    dim] layout is passed as its transposed view).  Slot j of page p is slot p * page_size + j."""
+    dim] layout is passed as its transposed view).  Slot j of page p is slot p * page_size + j.  A cache keeps
+    its tensors: other ones make another cache."""
 
-    __slots__ = ("k", "v", "_native")
+    __slots__ = ("_k", "_v", "_native")
 
     def __init__(self, k, v):
         device_tensor(k, "k", ndim=4, floating=True)
@@ -44,7 +45,7 @@ class PagedCache:
         for t in (k, v):
             if any(n > 1 and s <= 0 for n, s in zip(t.shape, t.stride())):
                 raise ValueError("cache strides must be positive")
-        self.k, self.v = k, v
+        self._k, self._v = k, v
         self._native = None
 
     @classmethod
@@ -54,6 +55,14 @@ class PagedCache:
         shape = (pages, page_size, kv_heads, dim)
         dtype = torch.bfloat16 if dtype is None else dtype
         return cls(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
+
+    @property
+    def k(self):
+        return self._k
+
+    @property
+    def v(self):
+        return self._v
 
     @property
     def pages(self) -> int:

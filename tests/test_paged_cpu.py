@@ -179,3 +179,14 @@ def test_filtered_sample_argument_refusals():
                               (dict(min_p=t(6)[::2]), ValueError)):
             with pytest.raises(error):
                 batched_filtered_sample(**{**dict(logits=logits, mask=mask), **change})
+
+
+def test_a_cache_keeps_its_tensors():
+    from bitmask_speculation_b200.paged import PagedCache
+    with fake_cuda():
+        x = torch.empty((4, 16, 2, 64), dtype=torch.bfloat16, device="cuda")
+        cache = PagedCache(x, x.clone())
+        assert cache.k is x and cache.pages == 4
+        for name in ("k", "v", "pages"):
+            with pytest.raises(AttributeError):
+                setattr(cache, name, x)
