@@ -1052,6 +1052,11 @@ __device__ __noinline__ RowStats first_pass(Shared& sh, const RowView<T>& shared
     }
     st.finite = finite;
     st.flags = (nan1 != nan1 ? 1u : 0u) | (some ? 2u : 0u);
+    // The other CTAs' shared memory exists once they have started: the kernel arrived at its start, the wait ends here.
+    if (c > 1) {
+        __syncwarp();
+        ptx::cluster_wait();
+    }
     float m = st.max;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -1705,6 +1710,7 @@ __global__ void __launch_bounds__(kThreads, 2) filter_sample_kernel(const Filter
         if (rank == 0 && threadIdx.x == 0) finish(-1, 0, code);
         return;
     }
+    if (c > 1) ptx::cluster_arrive();  // first_pass waits for it before it stores into other CTAs
     RowView<T>& view = *reinterpret_cast<RowView<T>*>(sh.view);
     static_assert(sizeof(RowView<T>) <= sizeof sh.view, "space of the view");
     if (threadIdx.x == 0) {

@@ -329,3 +329,29 @@ def test_spreads_of_short_rows(cuda_module, spread):
                                     dict(top_k=1511, top_p=0.70717, temperature=2 * scale), dict(top_p=0.93711, min_p=0.03, temperature=scale))):
             for dtype in DTYPES:
                 check(values, valid, dtype, params, rng.random(rows), offset=3 * i)
+
+
+@pytest.mark.parametrize("vocab", [8192, 16385, 32771])
+def test_clusters_that_start_while_others_end(cuda_module, vocab):
+    """Rows of the shortest parts that a cluster of 2, 4 or 8 CTAs takes, launched back to back on two streams: a CTA may be done
+    with its part before another one of its cluster has started."""
+    from bitmask_speculation_b200.kernels.cuda import batched_filtered_sample
+    rng = np.random.default_rng(vocab)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for rows in (3, 9, 74, 150):
+        values = (rng.standard_normal((rows, vocab)) * 2.5).astype(np.float32)
+        valid = rng.random((rows, vocab)) < rng.choice([1.0, 0.3, 0.002], rows)[:, None]
+        valid[:, rng.integers(vocab)] = True
+        u = rng.random(rows)
+        params = dict(top_k=40, top_p=0.9)
+        want = check(values, valid, "bfloat16", params, u)
+        args = torch.from_numpy(values).cuda().bfloat16(), torch.from_numpy(pack(valid)).cuda()
+        uniforms = torch.from_numpy(u).cuda()
+        torch.cuda.synchronize()
+        got = []
+        for i in range(40):
+            with torch.cuda.stream(streams[i % 2]):
+                got.append(batched_filtered_sample(*args, uniforms=uniforms, **params))
+        torch.cuda.synchronize()
+        for g in got:
+            assert torch.equal(g.token_ids, want.token_ids) and torch.equal(g.kept_counts, want.kept_counts) and int(g.status.sum()) == 0
