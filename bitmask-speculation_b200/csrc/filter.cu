@@ -706,9 +706,9 @@ __device__ __noinline__ bool cut_scores(Shared& sh, const uint32_t* counts, int 
     if (threadIdx.x == 0) {
         const float x = bin_score(sh.k_bin, top_rank);
         sh.threshold = fmaxf(x, sh.floor_x);
-        if (x < sh.floor_x) {  // min-p keeps every token at its score: the last bin that reaches it
-            int lo = 0, hi = sh.k_bin;
-            while (lo < hi) {
+        if (x < sh.floor_x) {  // min-p keeps every token at its score: the last bin that reaches it, -1 where only scores near zero do
+            int lo = bin_score(0, top_rank) >= sh.floor_x ? 0 : -1, hi = max(lo, sh.k_bin);
+            while (lo >= 0 && lo < hi) {
                 const int mid = (lo + hi + 1) / 2;
                 if (bin_score(mid, top_rank) >= sh.floor_x) lo = mid;
                 else hi = mid - 1;

@@ -355,3 +355,18 @@ def test_clusters_that_start_while_others_end(cuda_module, vocab):
         torch.cuda.synchronize()
         for g in got:
             assert torch.equal(g.token_ids, want.token_ids) and torch.equal(g.kept_counts, want.kept_counts) and int(g.status.sum()) == 0
+
+
+@pytest.mark.parametrize("vocab", [9973, 40009])
+def test_min_p_between_zero_and_the_first_bin(cuda_module, vocab):
+    """bfloat16 rows whose maximum lies within 2^-7 of zero and whose nucleus ends behind it, while min-p keeps only scores nearer
+    to zero than 2^-7: scores of exactly -2^-7 are dropped, in the middle of the row and at its ends alike."""
+    rng = np.random.default_rng(vocab)
+    u = np.array([0.0, 1e-9, 0.1, 0.5, 0.9, 0.999999])
+    for offset in range(9):
+        values = rng.choice([-2.0 ** -7, -0.010009765625, -0.0125732421875], (6, vocab)).astype(np.float32)
+        values[:, :9] = values[:, -9:] = -2.0 ** -7
+        values[np.arange(6)[:, None], rng.integers(9, vocab - 9, (6, 5))] = -0.00099945068359375
+        for params in (dict(top_p=0.93, min_p=0.999), dict(top_k=vocab * 3 // 4, min_p=0.999), dict(top_k=vocab * 3 // 4, top_p=0.93, min_p=1.0)):
+            got = check(values, np.ones((6, vocab), dtype=bool), "bfloat16", params, u, offset=offset)
+            assert max(got.kept_counts.tolist()) <= 5
