@@ -180,12 +180,19 @@ def build_decoder(vocab: int, *, layers: int, dim: int, heads: int, kv_heads: in
         @torch.inference_mode()
         def logits_batch(self, sequences, firsts, rows):
             """Logits of positions [firsts[i], firsts[i] + rows[i]) of each sequence, after one forward of
-            all of them over the cache (``enable_cache``); sequence i keeps its pages from call to call."""
+            all of them over the cache (``enable_cache``); sequence i keeps its pages from call to call.
+            The positions lie in their sequence; ``rows[i]`` may be 0."""
             if self._cache is None:
                 raise ValueError("logits_batch needs enable_cache")
+            if not len(sequences) == len(firsts) == len(rows):
+                raise ValueError("logits_batch needs a first position and a row count per sequence")
+            for i, (tokens, first, n) in enumerate(zip(sequences, firsts, rows)):
+                if first < 0 or n < 0 or first + n > len(tokens):
+                    raise ValueError(f"sequence {i}: positions [{first}, {first + n}) are not among its {len(tokens)} tokens")
             x, starts = self._cache.forward(sequences, firsts)
             at = [i for s, n in zip(starts, rows) for i in range(s, s + n)]
-            picked = x[at[0]:at[-1] + 1] if at == list(range(at[0], at[0] + len(at))) else x[torch.tensor(at, device=x.device)]
+            begin = at[0] if at else 0
+            picked = x[begin:begin + len(at)] if at == list(range(begin, begin + len(at))) else x[torch.tensor(at, device=x.device)]
             return self.head(self.norm(picked)).split(list(rows))
 
     gen = torch.Generator().manual_seed(seed)

@@ -92,3 +92,14 @@ def test_request_loops_over_the_cache_choose_the_same_tokens(cuda_module):
         spec = speculative_c4(target, draft, prompt, g0.fork(), max_new_tokens=48, eos=(0,))
         c_spec = speculative_c4(c_target, c_draft, prompt, g0.fork(), max_new_tokens=48, eos=(0,))
         assert c_spec == spec, i
+
+
+def test_sequences_without_rows(cuda_module):
+    """Row counts of 0: the forward fills the pages, and gives no logits of those sequences."""
+    cached, exact = decoder(torch.bfloat16).enable_cache(100, sequences=2, page_size=16), decoder(torch.bfloat16).double()
+    a, b = list(range(40)), list(range(100, 130))
+    none = cached.logits_batch([a, b], [39, 29], [0, 0])
+    assert [tuple(g.shape) for g in none] == [(0, VOCAB)] * 2
+    some = cached.logits_batch([a + [7], b], [40, 29], [1, 0])
+    want = exact.logits(a + [7], 40, 1)
+    assert some[1].shape == (0, VOCAB) and float((some[0].double() - want).abs().max()) <= bound(cached, want)
