@@ -97,8 +97,9 @@ class PagePlan:
 @dataclass(frozen=True, slots=True)
 class ChunkAttention:
     """``out`` [tokens, heads, dim], ``lse`` float32 [tokens, heads] (natural log of the sum of
-    exponentials) and a status per sequence (0; 6: lengths that do not fit; 7: a wait inside the kernel gave up;
-    11: a page outside the cache; the rows of a failed sequence are 0 with lse -inf)."""
+    exponentials) and a status per sequence (0; 6: lengths that do not fit, or rows that another sequence
+    claims too; 7: a wait inside the kernel gave up; 11: a page outside the cache; the rows of a failed sequence that
+    belong to no other one are 0 with lse -inf)."""
 
     out: object
     lse: object

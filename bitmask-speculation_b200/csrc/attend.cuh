@@ -105,11 +105,6 @@ __device__ __forceinline__ Range query_range(const Params& p, int32_t n, int32_t
     return r;
 }
 
-__device__ __forceinline__ bool lengths_fit(const AttendParams& a, int s) {
-    const int64_t x = a.query_start[s], y = a.query_start[s + 1], len = a.seq_lens[s];
-    return x >= 0 && y >= x && y <= a.tokens && len >= y - x && len <= static_cast<int64_t>(a.width) * a.page_size;
-}
-
 // A sequence without its total.
 __device__ __forceinline__ Shape sequence_shape(const Params& p, int s) {
     Shape h{0, 0, 0, 0, false};
@@ -817,18 +812,22 @@ constexpr int kFinishThreads = 256;
 template <typename T, int D>
 __global__ void __launch_bounds__(kFinishThreads) attend_finish_kernel(const Params p) {
     __shared__ LocateSpace<kFinishThreads> located;
-    __shared__ float qs[kFinishThreads / 32][256];
+    __shared__ float qs[kFinishThreads / 32][256];  // also clear_rows' bitmap
+    static_assert(sizeof qs >= kClaimWords * sizeof(uint32_t), "space of the bitmap");
     const AttendParams& a = p.a;
     const int c = blockIdx.x, ctas = gridDim.x, warp = threadIdx.x >> 5;
     locate<kFinishThreads>(p, located, c, ctas);  // of the call's inputs alone: may run before the tiles are done
+    const bool broken = starts_broken(a);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t total = located.start.total;
 
-    // Whether all pages that the sequence's rows see lie in the cache.  All threads of the block take part.
+    // A sequence's status but for waits that ran out: whether its lengths fit, its rows are its own, and all pages that they see
+    // lie in the cache.  All threads of the block take part.
     auto failed = [&](int s) -> int {
         if (!lengths_fit(a, s)) return BMS_STATUS_BAD_LENGTH;
         const int32_t n = a.query_start[s + 1] - a.query_start[s], len = a.seq_lens[s];
         if (n == 0) return 0;
+        if (broken && shares_rows(a, s)) return BMS_STATUS_BAD_LENGTH;
         const int64_t low = a.window > 0 ? max(static_cast<int64_t>(0), len - n + 1 - a.window) : 0;
         int bad = 0;
         for (int32_t i = threadIdx.x; i < (len + a.page_size - 1) / a.page_size; i += kFinishThreads) {
@@ -897,7 +896,7 @@ __global__ void __launch_bounds__(kFinishThreads) attend_finish_kernel(const Par
         int code = failed(s);
         if (code == 0 && abort) code = BMS_STATUS_TIMEOUT;
         if (threadIdx.x == 0) a.status[s] = code;
-        if (code != 0) clear_rows<T>(a, s);
+        if (code != 0) clear_rows<T>(a, s, broken, reinterpret_cast<uint32_t*>(qs));
     }
 }
 

@@ -356,29 +356,87 @@ struct AttendParams {
     float scale;
 };
 
-// Status of each sequence's lengths.
-__global__ void __launch_bounds__(256) attend_check_kernel(const AttendParams p) {
-    for (int s = blockIdx.x * 256 + threadIdx.x; s < p.seqs; s += gridDim.x * 256) {
-        const int64_t a = p.query_start[s], b = p.query_start[s + 1], len = p.seq_lens[s];
-        const bool bad = a < 0 || b < a || b > p.tokens || len < b - a || len > static_cast<int64_t>(p.width) * p.page_size;
-        p.status[s] = bad ? BMS_STATUS_BAD_LENGTH : BMS_STATUS_OK;
+// Whether a sequence's rows lie in the step and its tokens in its table row.
+__device__ __forceinline__ bool lengths_fit(const AttendParams& a, int s) {
+    const int64_t x = a.query_start[s], y = a.query_start[s + 1], len = a.seq_lens[s];
+    return x >= 0 && y >= x && y <= a.tokens && len >= y - x && len <= static_cast<int64_t>(a.width) * a.page_size;
+}
+
+// Starts in order give every sequence rows of its own.  Broken ones (malformed input) need not: then a row belongs to the one
+// sequence that fits and claims it; where several do, all of them fail, and the row is nobody's.
+// Whether starts are out of order or outside the step.  All threads of the block take part, here and below.
+__device__ bool starts_broken(const AttendParams& a) {
+    int bad = 0;
+    for (int s = threadIdx.x; s < a.seqs; s += blockDim.x) {
+        const int32_t x = a.query_start[s], y = a.query_start[s + 1];
+        bad |= x < 0 || y < x || y > a.tokens;
+    }
+    return __syncthreads_or(bad) != 0;
+}
+
+// Whether another sequence that fits claims rows of sequence s, which fits.
+__device__ bool shares_rows(const AttendParams& a, int s) {
+    const int32_t x = a.query_start[s], y = a.query_start[s + 1];
+    int hit = 0;
+    for (int t = threadIdx.x; t < a.seqs; t += blockDim.x)
+        hit |= t != s && max(a.query_start[t], x) < min(a.query_start[t + 1], y) && lengths_fit(a, t);
+    return __syncthreads_or(hit) != 0;
+}
+
+constexpr int kClaimWords = 2048;  // a bitmap of 65,536 rows
+
+// Zeroes the rows of a failed sequence, as far as they lie in the step.  If the starts are broken and its own lengths do not fit, it
+// may reach over rows of others: the ones that any fitting sequence claims are left to that one.
+template <typename T>
+__device__ void clear_rows(const AttendParams& p, int s, bool broken, uint32_t* claimed) {
+    const int64_t a = max(p.query_start[s], 0), b = min(static_cast<int64_t>(p.query_start[s + 1]), p.tokens);
+    const int64_t row = static_cast<int64_t>(p.heads) * p.dim;
+    const bool others = broken && !lengths_fit(p, s);
+    T* out = static_cast<T*>(p.out);
+    for (int64_t r0 = a; r0 < b; r0 += kClaimWords * 32) {
+        const int64_t r1 = min(b, r0 + kClaimWords * 32);
+        if (others) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < kClaimWords; i += blockDim.x) claimed[i] = 0;
+            __syncthreads();
+            for (int t = threadIdx.x; t < p.seqs; t += blockDim.x) {
+                if (!lengths_fit(p, t)) continue;
+                const int from = static_cast<int>(max(p.query_start[t] - r0, static_cast<int64_t>(0)));
+                const int to = static_cast<int>(min(static_cast<int64_t>(p.query_start[t + 1]), r1) - r0);
+                for (int w = from >> 5; 32 * w < to; ++w) {  // word by word
+                    const int lo = max(from - 32 * w, 0), hi = min(to - 32 * w, 32);
+                    atomicOr(&claimed[w], (0xffffffffu >> (32 - hi)) & (0xffffffffu << lo));
+                }
+            }
+            __syncthreads();
+        }
+        auto free_row = [&](int64_t r) { return !others || !(claimed[(r - r0) >> 5] >> ((r - r0) & 31) & 1); };
+        for (int64_t i = r0 * row + threadIdx.x; i < r1 * row; i += blockDim.x)
+            if (free_row(i / row)) out[i] = Convert<T>::down(0.f);
+        if (p.lse != nullptr)
+            for (int64_t i = r0 * p.heads + threadIdx.x; i < r1 * p.heads; i += blockDim.x)
+                if (free_row(i / p.heads)) p.lse[i] = -INFINITY;
     }
 }
 
-// Zeroes the rows of a failed sequence, as far as its row range is usable.
-template <typename T>
-__device__ void clear_rows(const AttendParams& p, int s) {
-    const int64_t a = max(p.query_start[s], 0), b = min(static_cast<int64_t>(p.query_start[s + 1]), p.tokens);
-    const int64_t row = static_cast<int64_t>(p.heads) * p.dim;
-    T* out = static_cast<T*>(p.out);
-    for (int64_t i = a * row + threadIdx.x; i < b * row; i += blockDim.x) out[i] = Convert<T>::down(0.f);
-    if (p.lse != nullptr)
-        for (int64_t i = a * p.heads + threadIdx.x; i < b * p.heads; i += blockDim.x) p.lse[i] = -INFINITY;
+// Status of each sequence's lengths, and through *broken whether the starts are (written by the first block).
+__global__ void __launch_bounds__(256) attend_check_kernel(const AttendParams p, int32_t* broken) {
+    for (int s = blockIdx.x * 256 + threadIdx.x; s < p.seqs; s += gridDim.x * 256) p.status[s] = lengths_fit(p, s) ? BMS_STATUS_OK : BMS_STATUS_BAD_LENGTH;
+    if (blockIdx.x != 0) return;
+    const bool bad = starts_broken(p);
+    if (threadIdx.x == 0) *broken = bad;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) attend_clear_kernel(const AttendParams p) {
-    if (p.status[blockIdx.x] != BMS_STATUS_OK) clear_rows<T>(p, blockIdx.x);
+__global__ void __launch_bounds__(256) attend_clear_kernel(const AttendParams p, const int32_t* broken) {
+    __shared__ uint32_t claimed[kClaimWords];
+    const int s = blockIdx.x;
+    int32_t code = p.status[s];
+    if (*broken && lengths_fit(p, s) && shares_rows(p, s)) code = BMS_STATUS_BAD_LENGTH;
+    __syncthreads();
+    if (code == BMS_STATUS_OK) return;
+    if (threadIdx.x == 0) p.status[s] = code;
+    clear_rows<T>(p, s, *broken, claimed);
 }
 
 // One warp computes one row (token, head) with plain arithmetic: 32 keys at a time, one per lane, for
@@ -463,18 +521,27 @@ __device__ void attend_row(const AttendParams& p, int s, int64_t token, int head
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) attend_rows_kernel(const AttendParams p) {
+__global__ void __launch_bounds__(256) attend_rows_kernel(const AttendParams p, const int32_t* broken) {
     __shared__ float qs[8][256];
     const int64_t rows = p.tokens * p.heads;
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); r < rows; r += static_cast<int64_t>(gridDim.x) * 8) {
         const int64_t token = r / p.heads;
-        int lo = 0, hi = p.seqs;  // the last s with query_start[s] <= token
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (p.query_start[mid + 1] > token) hi = mid;
-            else lo = mid + 1;
+        int lo = 0;
+        if (!*broken) {
+            int hi = p.seqs;  // the last s with query_start[s] <= token
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (p.query_start[mid + 1] > token) hi = mid;
+                else lo = mid + 1;
+            }
+            if (lo >= p.seqs || p.query_start[lo] > token || p.status[lo] == BMS_STATUS_BAD_LENGTH) continue;
+        } else {  // any that fits: of several all fail
+            int mine = p.seqs;
+            for (int s = threadIdx.x & 31; s < p.seqs && mine == p.seqs; s += 32)
+                if (p.query_start[s] <= token && token < p.query_start[s + 1] && lengths_fit(p, s)) mine = s;
+            lo = __reduce_min_sync(0xffffffffu, mine);
+            if (lo >= p.seqs) continue;
         }
-        if (lo >= p.seqs || p.query_start[lo] > token || p.status[lo] == BMS_STATUS_BAD_LENGTH) continue;
         attend_row<T>(p, lo, token, static_cast<int>(r % p.heads), qs[threadIdx.x >> 5]);
     }
 }
@@ -586,11 +653,12 @@ int launch_tiles(const AttendParams& a, int dtype, int device, int sms, void* wo
 }
 
 template <typename T>
-int launch_attend(const AttendParams& p, int sms, cudaStream_t stream) {
-    attend_check_kernel<<<(p.seqs + 255) / 256, 256, 0, stream>>>(p);
+int launch_attend(const AttendParams& p, int sms, void* workspace, cudaStream_t stream) {
+    int32_t* broken = static_cast<int32_t*>(workspace);
+    attend_check_kernel<<<(p.seqs + 255) / 256, 256, 0, stream>>>(p, broken);
     const int64_t blocks = std::min<int64_t>((p.tokens * p.heads + 7) / 8, 16LL * sms);
-    if (blocks > 0) attend_rows_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p);
-    attend_clear_kernel<T><<<p.seqs, 256, 0, stream>>>(p);
+    if (blocks > 0) attend_rows_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p, broken);
+    attend_clear_kernel<T><<<p.seqs, 256, 0, stream>>>(p, broken);
     BMS_CUDA(cudaGetLastError(), "chunk attention launch");
     return BMS_SUCCESS;
 }
@@ -754,14 +822,14 @@ int bms_chunk_attention(const void* q, int32_t dtype, int64_t tokens, int64_t he
                          cache->pages, window, sinks, static_cast<int32_t>(seqs), static_cast<int32_t>(width), static_cast<int32_t>(cache->page_size),
                          static_cast<int32_t>(heads), static_cast<int32_t>(cache->kv_heads), static_cast<int32_t>(cache->dim), static_cast<float>(scale)};
     const auto st = static_cast<cudaStream_t>(stream);
-    if (dtype == BMS_FLOAT32) return launch_attend<float>(p, sms, st);
+    if (dtype == BMS_FLOAT32) return launch_attend<float>(p, sms, workspace, st);
     const bool bf16 = dtype == BMS_BFLOAT16;
     if (tokens > 0 && tiles_fit(p, dtype)) {
         if (p.dim == 64)
             return bf16 ? launch_tiles<__nv_bfloat16, 64>(p, dtype, device, sms, workspace, st) : launch_tiles<__half, 64>(p, dtype, device, sms, workspace, st);
         return bf16 ? launch_tiles<__nv_bfloat16, 128>(p, dtype, device, sms, workspace, st) : launch_tiles<__half, 128>(p, dtype, device, sms, workspace, st);
     }
-    return bf16 ? launch_attend<__nv_bfloat16>(p, sms, st) : launch_attend<__half>(p, sms, st);
+    return bf16 ? launch_attend<__nv_bfloat16>(p, sms, workspace, st) : launch_attend<__half>(p, sms, workspace, st);
 }
 
 }  // extern "C"

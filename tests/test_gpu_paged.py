@@ -583,3 +583,69 @@ def test_many_short_sequences(cuda_module, dtype, heads, kv_heads, dim, page, lo
     mixed = [(int(n), int(x)) for n, x in zip(rng.choice([0, 1, 1, 1, 9, 40, 150], 150), rng.integers(0, longest, 150))]
     check_attention(mixed, heads, kv_heads, dim, page, dtype)
     check_attention(mixed, heads, kv_heads, dim, page, dtype, window=50, sinks=3)
+
+
+BROKEN = {  # starts, (past, rows in order of the packed step) of the sequences that own rows, statuses
+    "beyond": ([0, 3, 1000, 7, 9], [30, 100, 0, 4000], [0, 6, 6, 0]),
+    "unordered": ([5, 8, 0, 5], [3000, 10, 700], [0, 6, 0]),
+    "overlapping": ([0, 10, 5, 20, 27], [4000, 100, 3000, 500], [6, 6, 6, 0]),
+    "inside": ([0, 9, 3, 5, 12], [300, 20, 3000, 40], [6, 6, 6, 6]),
+    "negative": ([0, 4, -3, 6, 9], [300, 50, 600, 90], [0, 6, 6, 0]),
+    "nested": ([0, 2, 40, 6, 3, 5, 8], [50, 600, 70, 800, 90, 2000], [0, 6, 6, 6, 0, 0]),
+}
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 64), (torch.float16, 128), (torch.float32, 40)])
+@pytest.mark.parametrize("kind", list(BROKEN))
+def test_starts_broken_in_the_middle(cuda_module, dtype, dim, kind):
+    """Row starts out of order or beyond the step: a sequence whose rows lie in the step and are claimed by no other one is computed
+    as ever, every other row that some sequence claims is 0 with lse -inf, the rest is left as it was."""
+    from bitmask_speculation_b200.paged import PagedCache, chunk_attention
+    starts, past, status = BROKEN[kind]
+    seqs, n = len(past), max(x for x in starts if x < 30)
+    mine = [max(b - a, 0) if a >= 0 and b <= n else 0 for a, b in zip(starts, starts[1:])]
+    lens = [(m, p) for m, p in zip(mine, past)]
+    q, k, v, table, seq_lens, _ = make_case([(m, p) for m, p in lens], 4, 2, dim, 16, dtype)
+    q = torch.cat((q, q))[:n] if q.shape[0] >= n / 2 else torch.cat([q] * n)[:n]
+    out = torch.full((n + 2, 4, dim), 5.0, dtype=dtype, device="cuda")
+    got = chunk_attention(torch.cat((q, q[:2])), PagedCache(k, v), table, seq_lens, i32(starts), out=out)
+    # `n + 2` rows: a start of 1000 or 40 lies beyond the step, the last two rows behind every sequence that fits.
+    assert got.status.tolist() == status
+    claimed = torch.zeros(n + 2, dtype=torch.bool, device="cuda")
+    for s, (a, b) in enumerate(zip(starts, starts[1:])):
+        claimed[max(a, 0):max(min(b, n + 2), 0)] = True
+    for s, (a, b) in enumerate(zip(starts, starts[1:])):
+        if status[s]:
+            continue
+        want = definition(q[a:b], k, v, table[s:s + 1], [lens[s]], 0, 0, dim ** -0.5)
+        assert_close(type(got)(got.out[a:b], got.lse[a:b], got.status), want, dtype, dim)
+        claimed[a:b] = False
+        out[a:b] = 5.0
+    assert bool((out[claimed] == 0).all()) and bool((got.lse[claimed] == -math.inf).all())
+    assert bool((out[~claimed] == 5).all())
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 64), (torch.float32, 8)])
+def test_broken_starts_over_many_rows(cuda_module, dtype, dim):
+    """A failed sequence that claims more rows than one bitmap holds, around others that own some of them."""
+    from bitmask_speculation_b200.paged import PagedCache, chunk_attention
+    n = 140000
+    starts = [0, 3, n + 5, 65530, 65560, n + 9, n - 7, n]
+    lens = [(3, 20), (0, 5), (0, 5), (30, 50), (0, 5), (0, 5), (7, 40)]
+    q, k, v, table, seq_lens, _ = make_case(lens, 1, 1, dim, 16, dtype)
+    full = torch.zeros((n, 1, dim), dtype=dtype, device="cuda")
+    rows = [slice(0, 3), slice(65530, 65560), slice(n - 7, n)]
+    at = 0
+    for r in rows:
+        full[r] = q[at:at + r.stop - r.start]
+        at += r.stop - r.start
+    out = torch.full((n, 1, dim), 5.0, dtype=dtype, device="cuda")
+    got = chunk_attention(full, PagedCache(k, v), table, seq_lens, i32(starts), out=out)
+    assert got.status.tolist() == [0, 6, 6, 0, 6, 6, 0]
+    fine = [(0, 3, 0), (65530, 65560, 3), (n - 7, n, 6)]
+    rest = torch.ones(n, dtype=torch.bool, device="cuda")
+    for a, b, s in fine:
+        want = definition(full[a:b], k, v, table[s:s + 1], [lens[s]], 0, 0, dim ** -0.5)
+        assert_close(type(got)(got.out[a:b], got.lse[a:b], got.status), want, dtype, dim)
+        rest[a:b] = False
+    assert bool((out[rest] == 0).all()) and bool((got.lse[rest] == -math.inf).all())
