@@ -58,14 +58,14 @@ struct Control {
     uint64_t q_full, q_free, s_full[2], p_full[2][2], o_full[2];
     float ref[kTile], sum[kTile];
     int32_t item_tiles[2], item_wide[2];  // of the item whose queries are in place, by the item's parity; 0 tiles: no more
-    uint32_t tmem, poison, abort;
+    uint32_t tmem, poison, abort, broken;
 };
 
 struct Params {
     AttendParams a;
     float* parts;      // [ctas][2][D / 4][256][4]: lanes (rows) side by side
     float* part_lse;   // [ctas][2][256], log2
-    int32_t* flags;    // [ctas]: 1 poisoned values, 2 a wait ran out
+    int32_t* flags;    // [ctas]: 1 poisoned values, 2 a wait ran out, 4 row starts are broken
     float scale2;      // |scale| log2(e)
     uint32_t negate;   // sign bit for the scores of a negative scale
     int32_t group, tile_tokens;
@@ -181,7 +181,7 @@ struct Walk {
 };
 
 // Finds where part `c` of `ctas` starts.  All threads of the block take part; the sequences' totals come one per thread,
-// or, for prompts of many query tiles, one per warp with the tiles over its lanes.
+// or, for prompts of many query tiles, one per warp with the tiles over its lanes.  True where this thread met a broken start.
 template <int kBlock>
 struct LocateSpace {
     int64_t totals[kBlock], scan[kBlock / 32];
@@ -189,12 +189,13 @@ struct LocateSpace {
 };
 
 template <int kBlock>
-__device__ void locate(const Params& p, LocateSpace<kBlock>& sp, int c, int ctas) {
+__device__ bool locate(const Params& p, LocateSpace<kBlock>& sp, int c, int ctas) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     constexpr int kW = kBlock / 32;
     const bool by_warp = p.a.tokens > 2LL * p.tile_tokens * p.a.seqs;
     const bool once = p.a.seqs <= kBlock;  // one round: the second pass has the totals already
     int64_t target = -1, mine = 0, v = 0;
+    bool broken = false;
     for (int pass = 0; pass < 2; ++pass) {
         int64_t run = 0;
         for (int base = 0; base < p.a.seqs; base += kBlock) {
@@ -204,6 +205,7 @@ __device__ void locate(const Params& p, LocateSpace<kBlock>& sp, int c, int ctas
                 if (by_warp) {
                     for (int i = warp; i < kBlock && base + i < p.a.seqs; i += kW) {
                         const Shape h = sequence_shape(p, base + i);
+                        broken |= h.n == 0 && start_broken(p.a, base + i);
                         int t = 0;
                         for (int q = lane; q < h.tiles; q += 32) t += kItemCost + query_range(p, h.n, h.past, h.wide, q).steps;
                         t = __reduce_add_sync(0xffffffffu, t);
@@ -211,6 +213,7 @@ __device__ void locate(const Params& p, LocateSpace<kBlock>& sp, int c, int ctas
                     }
                 } else if (s < p.a.seqs) {
                     const Shape h = sequence_shape(p, s);
+                    broken |= h.n == 0 && start_broken(p.a, s);
                     int64_t t = 0;
                     for (int q = 0; q < h.tiles; ++q) t += kItemCost + query_range(p, h.n, h.past, h.wide, q).steps;
                     sp.totals[threadIdx.x] = t;
@@ -245,6 +248,7 @@ __device__ void locate(const Params& p, LocateSpace<kBlock>& sp, int c, int ctas
         }
         __syncthreads();
     }
+    return broken;
 }
 
 __device__ __forceinline__ int64_t part_begin(int64_t total, int c, int ctas) {
@@ -420,7 +424,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
             ptx::mbar_init(ptx::smem_addr(&ctl.o_full[i]), 1);
         }
         ptx::fence_mbarrier_init();
-        ctl.poison = ctl.abort = 0;
+        ctl.poison = ctl.abort = ctl.broken = 0;
     }
     if (warp == kMmaWarp) tmem_alloc(&ctl.tmem, 512);
     fence_before();
@@ -428,7 +432,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
     asm volatile("griddepcontrol.launch_dependents;");  // not before the wait: the dependent reads this call's inputs early
     // The space of Q serves the search before the first item.
     LocateSpace<kThreads>& located = *reinterpret_cast<LocateSpace<kThreads>*>(tiles_smem + (q_smem - ptx::smem_addr(tiles_smem)));
-    locate<kThreads>(p, located, blockIdx.x, gridDim.x);
+    if (locate<kThreads>(p, located, blockIdx.x, gridDim.x)) ctl.broken = 1;
     fence_after();
     const uint32_t tmem = ctl.tmem;
     const Start start = located.start;
@@ -801,7 +805,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
     }
     __syncthreads();
     fence_after();
-    if (threadIdx.x == 0) p.flags[blockIdx.x] = ctl.poison | (ctl.abort << 1);
+    if (threadIdx.x == 0) p.flags[blockIdx.x] = ctl.poison | (ctl.abort << 1) | (ctl.broken << 2);
     if (warp == kMmaWarp) tmem_free(tmem, 512);
 }
 
@@ -817,9 +821,11 @@ __global__ void __launch_bounds__(kFinishThreads) attend_finish_kernel(const Par
     const AttendParams& a = p.a;
     const int c = blockIdx.x, ctas = gridDim.x, warp = threadIdx.x >> 5;
     locate<kFinishThreads>(p, located, c, ctas);  // of the call's inputs alone: may run before the tiles are done
-    const bool broken = starts_broken(a);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t total = located.start.total;
+    int flagged = 0;
+    for (int i = threadIdx.x; i < ctas; i += kFinishThreads) flagged |= p.flags[i];
+    const bool broken = __syncthreads_or(flagged & 4) != 0;
 
     // A sequence's status but for waits that ran out: whether its lengths fit, its rows are its own, and all pages that they see
     // lie in the cache.  All threads of the block take part.
@@ -840,16 +846,14 @@ __global__ void __launch_bounds__(kFinishThreads) attend_finish_kernel(const Par
     };
 
     const int64_t begin = part_begin(total, c, ctas), end = part_begin(total, c + 1, ctas);
-    int abort = 0;
-    for (int i = threadIdx.x; i < ctas; i += kFinishThreads) abort |= p.flags[i] & 2;
-    abort = __syncthreads_or(abort);
+    const int abort = __syncthreads_or(flagged & 2);
     Walk walk;
     walk.start(p, located.start, end - begin);
     for (bool first = true; walk.valid(p); walk.next(p), first = false) {
-        if (!first && p.flags[c] == 0) break;                     // later items that end here are whole
+        if (!first && (p.flags[c] & 3) == 0) break;                     // later items that end here are whole
         if (walk.st1 != walk.range.steps) break;                  // ends in a later part
         const int64_t item_begin = end - walk.left - walk.at + kItemCost;  // of the item's first step
-        if (walk.st0 == 0 && p.flags[c] == 0) continue;           // whole and clean
+        if (walk.st0 == 0 && (p.flags[c] & 3) == 0) continue;           // whole and clean
         int from = c;
         while (from > 0 && part_begin(total, from, ctas) > item_begin) --from;
         int poison = 0;

@@ -364,17 +364,12 @@ __device__ __forceinline__ bool lengths_fit(const AttendParams& a, int s) {
 
 // Starts in order give every sequence rows of its own.  Broken ones (malformed input) need not: then a row belongs to the one
 // sequence that fits and claims it; where several do, all of them fail, and the row is nobody's.
-// Whether starts are out of order or outside the step.  All threads of the block take part, here and below.
-__device__ bool starts_broken(const AttendParams& a) {
-    int bad = 0;
-    for (int s = threadIdx.x; s < a.seqs; s += blockDim.x) {
-        const int32_t x = a.query_start[s], y = a.query_start[s + 1];
-        bad |= x < 0 || y < x || y > a.tokens;
-    }
-    return __syncthreads_or(bad) != 0;
+__device__ __forceinline__ bool start_broken(const AttendParams& a, int s) {
+    const int32_t x = a.query_start[s], y = a.query_start[s + 1];
+    return x < 0 || y < x || y > a.tokens;
 }
 
-// Whether another sequence that fits claims rows of sequence s, which fits.
+// Whether another sequence that fits claims rows of sequence s, which fits.  All threads of the block take part, here and below.
 __device__ bool shares_rows(const AttendParams& a, int s) {
     const int32_t x = a.query_start[s], y = a.query_start[s + 1];
     int hit = 0;
@@ -423,7 +418,9 @@ __device__ void clear_rows(const AttendParams& p, int s, bool broken, uint32_t* 
 __global__ void __launch_bounds__(256) attend_check_kernel(const AttendParams p, int32_t* broken) {
     for (int s = blockIdx.x * 256 + threadIdx.x; s < p.seqs; s += gridDim.x * 256) p.status[s] = lengths_fit(p, s) ? BMS_STATUS_OK : BMS_STATUS_BAD_LENGTH;
     if (blockIdx.x != 0) return;
-    const bool bad = starts_broken(p);
+    int bad = 0;
+    for (int s = threadIdx.x; s < p.seqs; s += 256) bad |= start_broken(p, s);
+    bad = __syncthreads_or(bad);
     if (threadIdx.x == 0) *broken = bad;
 }
 
