@@ -39,7 +39,7 @@ EXPORTS = (
     "bms_exchange_bytes", "bms_exchange_create", "bms_exchange_open", "bms_exchange_close", "bms_exchange_destroy",
     "bms_shard_partials_exchange", "bms_shard_merge_exchange",
     "bms_filtered_sample_batch", "bms_page_plan", "bms_rotary_append", "bms_attention_workspace_bytes",
-    "bms_chunk_attention",
+    "bms_chunk_attention", "bms_hold_pages",
 )
 
 
@@ -96,6 +96,7 @@ def _declare(lib) -> None:
         "bms_page_plan": [p, p, p, i64, p, i64, p, i64, p, i64, i64, p, p, p, p, p, p, p, i32, p],
         "bms_rotary_append": [p, p, p, i32, i64, i64, p, p, p, p, p, i64, p, p, p, p, p, i32, p],
         "bms_chunk_attention": [p, i32, i64, i64, p, p, p, i64, i64, p, p, f64, i64, i64, p, p, p, p, i64, i32, p],
+        "bms_hold_pages": [i32],
         "bms_shard_merge_exchange": [p, i32, i32, i64, ctypes.c_uint32, i64, p, p, p, i32, p],
     }
     for name, args in sig.items():

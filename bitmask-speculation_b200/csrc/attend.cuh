@@ -55,7 +55,7 @@ struct Layout {
 
 struct Control {
     uint64_t full[12], empty[12];
-    uint64_t q_full, q_free, s_full[2], p_full[2][2], o_full[2];
+    uint64_t q_full, q_free, s_full[2], p_full[2][2], o_full[2], drained;
     float ref[kTile], sum[kTile];
     int32_t item_tiles[2], item_wide[2];  // of the item whose queries are in place, by the item's parity; 0 tiles: no more
     uint32_t tmem, poison, abort, broken;
@@ -70,6 +70,7 @@ struct Params {
     uint32_t negate;   // sign bit for the scores of a negative scale
     int32_t group, tile_tokens;
     int32_t group_inv;  // 65536 / group, rounded up: r / group = r * group_inv >> 16 for rows r < 128
+    int32_t hold;       // of tests: no page is loaded, so that the waits for them run out
 };
 
 // ---- schedule ---------------------------------------------------------------------------------
@@ -333,19 +334,32 @@ __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, i
         : "memory");
 }
 
-// Waits at most about a second; after that the CTA's abort flag ends every wait.
-__device__ __forceinline__ void wait_bar(Control& c, uint64_t* bar, uint32_t parity) {
+// Waits at most about a second; after that the CTA's abort flag ends every wait.  Nothing more is loaded or multiplied then; the
+// softmax warpgroups walk on through their items without tiles, because they meet at barriers; and copies and products
+// in flight land (`drain`) before the CTA gives its memory back.
+__device__ __forceinline__ bool wait_bar(Control& c, uint64_t* bar, uint32_t parity) {
     const uint32_t addr = ptx::smem_addr(bar);
     volatile uint32_t* abort = &c.abort;
     uint64_t t0 = 0;
     for (uint32_t i = 0; !ptx::mbar_try_wait(addr, parity); ++i) {
+        if (*abort) return false;
         if ((i & 63u) != 63u) continue;
-        if (*abort) return;
         const uint64_t now = ptx::globaltimer();
         if (t0 == 0) t0 = now;
         else if (now - t0 > kWaitNs) *abort = 1;
     }
+    return true;
 }
+
+// For what is in flight already: lands in microseconds, whether the CTA gave up or not; the limit is for hardware that failed.
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
+    const uint32_t addr = ptx::smem_addr(bar);
+    const uint64_t t0 = ptx::globaltimer();
+    while (!ptx::mbar_try_wait(addr, parity) && ptx::globaltimer() - t0 < kWaitNs / 5) {
+    }
+}
+
+__device__ __forceinline__ bool aborted(const Control& c) { return *static_cast<const volatile uint32_t*>(&c.abort) != 0; }
 
 __device__ __forceinline__ uint32_t pack_pair(float lo, float hi, __nv_bfloat16) {
     uint32_t r;
@@ -423,6 +437,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
             ptx::mbar_init(ptx::smem_addr(&ctl.p_full[i][0]), 4), ptx::mbar_init(ptx::smem_addr(&ctl.p_full[i][1]), 4);
             ptx::mbar_init(ptx::smem_addr(&ctl.o_full[i]), 1);
         }
+        ptx::mbar_init(ptx::smem_addr(&ctl.drained), 1);
         ptx::fence_mbarrier_init();
         ctl.poison = ctl.abort = ctl.broken = 0;
     }
@@ -447,6 +462,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
             Walk walk;
             walk.start(p, start, end - begin);
             uint32_t seq = 0;  // tiles loaded so far
+            bool stop = p.hold != 0;
             // Lane i loads box i of a tile.  Its page index (-1: nothing to load) is fetched a tile ahead of its use.
             const int32_t box = min(a.page_size, kTile);
             auto page_of = [&](int tile) {
@@ -457,42 +473,39 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
                 return page < a.pages ? page : -1;  // attend_finish_kernel reports pages outside the cache
             };
             auto load = [&](const CUtensorMap* map, int tile, int32_t page) {
+                if (stop) return;
                 const uint32_t stage = seq % kStages, round = seq / kStages;
+                // All lanes go on or none does: a barrier expects just the boxes that are on their way.
+                stop = __any_sync(0xffffffffu, !wait_bar(ctl, &ctl.empty[stage], (round & 1) ^ 1));
+                if (stop) return;
                 ++seq;
-                wait_bar(ctl, &ctl.empty[stage], (round & 1) ^ 1);
                 const bool mine = page >= 0;
                 const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, mine));
                 const uint32_t bar = ptx::smem_addr(&ctl.full[stage]);
                 if (lane == 0) ptx::mbar_arrive_expect_tx(bar, boxes * box * D * 2);
                 __syncwarp();
-                if (mine && !*static_cast<volatile uint32_t*>(&ctl.abort)) {
+                if (mine) {
                     const int32_t slot = (walk.range.tile(tile) * kTile + lane * box) % a.page_size;
                     const uint32_t dst = ring + stage * L::kTileBytes + lane * box * 128;
 #pragma unroll
                     for (int half = 0; half < D / 64; ++half) tma_page(dst + half * (kTile * 128), map, half * 64, walk.head, slot, page, bar);
                 }
             };
-            for (; walk.valid(p); walk.next(p)) {
+            for (; !stop && walk.valid(p); walk.next(p)) {
                 const int t0 = walk.tile0(), t1 = walk.tile1(), ahead = walk.shape.wide ? 1 : 2;
                 auto fetch = [&](int t) { return t < t1 ? page_of(t) : -1; };
                 // Pages of tiles t, t + 1, t + 2: values trail their keys by `ahead` tiles.
                 int32_t pg0 = fetch(t0), pg1 = fetch(t0 + 1), pg2 = fetch(t0 + 2);
                 load(&k_map, t0, pg0);
                 if (ahead == 2 && t0 + 1 < t1) load(&k_map, t0 + 1, pg1);
-                for (int t = t0; t < t1; ++t) {
+                for (int t = t0; t < t1 && !stop; ++t) {
                     const int32_t pg3 = fetch(t + 3);
                     load(&v_map, t, pg0);
                     if (t + ahead < t1) load(&k_map, t + ahead, ahead == 1 ? pg1 : pg2);
                     pg0 = pg1, pg1 = pg2, pg2 = pg3;
                 }
             }
-            // After an abort copies may still be in flight: they land before the shared memory goes away.
-            if (*static_cast<volatile uint32_t*>(&ctl.abort)) {
-                const uint64_t t0 = ptx::globaltimer();
-                for (uint32_t i = seq > kStages ? seq - kStages : 0; i < seq; ++i)
-                    while (!ptx::mbar_try_wait(ptx::smem_addr(&ctl.full[i % kStages]), (i / kStages) & 1) && ptx::globaltimer() - t0 < kWaitNs / 5) {
-                    }
-            }
+            for (uint32_t i = seq > kStages ? seq - kStages : 0; i < seq; ++i) drain(&ctl.full[i % kStages], (i / kStages) & 1);
         } else if (warp == kQueryWarp) {
             // Queries of the next item as soon as the last one's space is free: rows are (token, head of the group) pairs, and a
             // box of the group's heads by the tile's tokens is just that.  Boxes may run into the next sequence's tokens
@@ -500,23 +513,26 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
             Walk walk;
             walk.start(p, start, end - begin);
             uint32_t item = 0;
+            bool stop = false;
             for (; walk.valid(p); walk.next(p), ++item) {
-                wait_bar(ctl, &ctl.q_free, (item & 1) ^ 1);
+                stop = __any_sync(0xffffffffu, !wait_bar(ctl, &ctl.q_free, (item & 1) ^ 1));
+                if (stop) break;
                 if (lane == 0) {
                     const int tiles = walk.shape.wide ? 2 : 1;
                     const uint32_t bar = ptx::smem_addr(&ctl.q_full);
                     ctl.item_tiles[item & 1] = walk.tile1() - walk.tile0(), ctl.item_wide[item & 1] = walk.shape.wide;
-                    const bool go = !*static_cast<volatile uint32_t*>(&ctl.abort);
-                    ptx::mbar_arrive_expect_tx(bar, go ? tiles * p.tile_tokens * p.group * D * 2 : 0);
-                    for (int t = 0; t < tiles && go; ++t)
+                    ptx::mbar_arrive_expect_tx(bar, tiles * p.tile_tokens * p.group * D * 2);
+                    for (int t = 0; t < tiles; ++t)
                         for (int half = 0; half < D / 64; ++half)
                             tma_rows(q_smem + t * L::kTileBytes + half * (kTile * 128), &q_map, half * 64, walk.head * p.group,
                                      a.query_start[walk.s] + walk.range.first + t * p.tile_tokens, bar);
                 }
                 __syncwarp();
             }
-            wait_bar(ctl, &ctl.q_free, (item & 1) ^ 1);
-            if (lane == 0) {
+            if (!stop) stop = __any_sync(0xffffffffu, !wait_bar(ctl, &ctl.q_free, (item & 1) ^ 1));
+            if (stop) {
+                if (item > 0) drain(&ctl.q_full, (item - 1) & 1);
+            } else if (lane == 0) {
                 ctl.item_tiles[item & 1] = 0;
                 ptx::mbar_arrive(ptx::smem_addr(&ctl.q_full));
             }
@@ -554,7 +570,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
                     fence_after();
                     const int n = ctl.item_tiles[item & 1];
                     const bool wide = ctl.item_wide[item & 1];
-                    if (n == 0 || *static_cast<volatile uint32_t*>(&ctl.abort)) break;
+                    if (n == 0 || aborted(ctl)) break;
                     // Scores of the first tile (two tiles) ahead of the loop.
                     for (int t = 0; t < (wide ? 2 : min(n, 2)); ++t) {
                         if (t == 0 || !wide) ready(seq);
@@ -585,6 +601,10 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
                         seq += more ? 2 : 1;
                     }
                 }
+                if (aborted(ctl)) {  // else the softmax warpgroups have waited for all of them
+                    mma_commit(&ctl.drained);
+                    drain(&ctl.drained, 0);
+                }
             }
             __syncwarp();
         }
@@ -600,7 +620,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
         for (; walk.valid(p); walk.next(p), ++item) {
             // A warpgroup without a tile in this item has nothing else to wait for: it must not release the next item's queries
             // before the other one is done with this item's.
-            wait_bar(ctl, &ctl.q_full, item & 1);
+            if (!aborted(ctl)) wait_bar(ctl, &ctl.q_full, item & 1);
             const Range& r = walk.range;
             const bool wide = walk.shape.wide;
             const int t0 = walk.tile0(), n = walk.tile1() - t0;
@@ -614,7 +634,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
             const int32_t wg_first = r.first + (wide ? wg * p.tile_tokens : 0), wg_end = min(r.end, wg_first + p.tile_tokens);
             const int32_t wg_min = walk.shape.past + wg_first, wg_max = walk.shape.past + wg_end - 1;
             float ref = -INFINITY, sum = 0.f;
-            const int mine = wide ? n : (n + 1 - wg) / 2;
+            const int mine = __any_sync(0xffffffffu, aborted(ctl)) ? 0 : wide ? n : (n + 1 - wg) / 2;
             for (int i = 0; i < mine; ++i) {
                 const int t = wide ? i : 2 * i + wg;
                 const int32_t key0 = r.tile(t0 + t) * kTile;
@@ -711,6 +731,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
                 ++o_round;
                 fence_after();
             }
+            __syncwarp();
             // The space of Q is free now (outputs were committed after every score product that reads it): one half takes the
             // second half of a one-tile item, element by row in float32, half of the columns at a time, the other the
             // finished rows on their way out, so that the stores are whole lines.

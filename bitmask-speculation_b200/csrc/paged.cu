@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "../../include/bms_b200.h"
@@ -612,6 +613,8 @@ int query_map(CUtensorMap* map, const AttendParams& p, int dtype, int group, int
 
 int64_t tiles_workspace(int64_t ctas, int64_t dim) { return 256 + ctas * 2 * 256 * (dim + 1) * 4 + ((ctas * 4 + 255) / 256) * 256; }
 
+std::atomic<int32_t> g_hold_pages{0};  // bms_hold_pages
+
 template <typename T, int D>
 int launch_tiles(const AttendParams& a, int dtype, int device, int sms, void* workspace, cudaStream_t stream) {
     static bool ready[kMaxDevices];
@@ -636,6 +639,7 @@ int launch_tiles(const AttendParams& a, int dtype, int device, int sms, void* wo
     p.group = group;
     p.tile_tokens = tc::kTile / p.group;
     p.group_inv = (65536 + p.group - 1) / p.group;
+    p.hold = g_hold_pages.load(std::memory_order_relaxed);
     // Both launches are programmatic dependents: their prologues run while the launch before them ends.
     cudaLaunchAttribute overlap{};
     overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -827,6 +831,11 @@ int bms_chunk_attention(const void* q, int32_t dtype, int64_t tokens, int64_t he
         return bf16 ? launch_tiles<__nv_bfloat16, 128>(p, dtype, device, sms, workspace, st) : launch_tiles<__half, 128>(p, dtype, device, sms, workspace, st);
     }
     return bf16 ? launch_attend<__nv_bfloat16>(p, sms, workspace, st) : launch_attend<__half>(p, sms, workspace, st);
+}
+
+int bms_hold_pages(int32_t hold) {
+    g_hold_pages.store(hold != 0, std::memory_order_relaxed);
+    return BMS_SUCCESS;
 }
 
 }  // extern "C"

@@ -394,6 +394,10 @@ BMS_API int bms_chunk_attention(const void *q, int32_t dtype, int64_t tokens, in
                                 int64_t sinks, void *out, float *lse, int32_t *status, void *workspace,
                                 int64_t workspace_bytes, int32_t device, void *stream);
 
+/* Test hook: while `hold` is not 0, chunk attention's tile kernel loads no pages, so that its waits run out (after about a
+ * second) and every sequence of a call reports status 7.  Process-wide; not for concurrent use with other calls. */
+BMS_API int bms_hold_pages(int32_t hold);
+
 /* Test hook: force the cluster size (1, 2, 4, 8 or 16) and the number of
  * clusters of the selection kernels' fixed schedule; 0 restores the automatic
  * choice.  With cluster 0 and a workspace, `clusters` caps the number of CTAs of

@@ -649,3 +649,27 @@ def test_broken_starts_over_many_rows(cuda_module, dtype, dim):
         assert_close(type(got)(got.out[a:b], got.lse[a:b], got.status), want, dtype, dim)
         rest[a:b] = False
     assert bool((out[rest] == 0).all()) and bool((got.lse[rest] == -math.inf).all())
+
+
+@pytest.mark.parametrize("dtype,dim,page", [(torch.bfloat16, 64, 16), (torch.float16, 128, 64)])
+def test_waits_that_run_out(cuda_module, dtype, dim, page):
+    """Pages that never arrive: the call ends after its limit, every sequence reports status 7, and the next call is right."""
+    from bitmask_speculation_b200 import _native
+    from bitmask_speculation_b200.paged import PagedCache, chunk_attention
+    lens = [(1, 700), (9, 5000), (300, 900), (1, 3)]
+    q, k, v, table, seq_lens, starts = make_case(lens, 8, 2, dim, page, dtype)
+    cache = PagedCache(k, v)
+    lib = _native.library()
+    _native.check(lib.bms_hold_pages(1))
+    try:
+        held = chunk_attention(q, cache, table, seq_lens, starts)
+        torch.cuda.synchronize()
+    finally:
+        _native.check(lib.bms_hold_pages(0))
+    assert held.status.tolist() == [7] * 4
+    with pytest.raises(ValueError, match=r"\(1, 7\)"):
+        held.check()
+    for _ in range(2):
+        got = chunk_attention(q, cache, table, seq_lens, starts)
+        assert got.status.tolist() == [0] * 4
+        assert_close(got, definition(q, k, v, table, lens, 0, 0, dim ** -0.5), dtype, dim)
