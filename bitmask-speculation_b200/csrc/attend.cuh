@@ -870,7 +870,8 @@ __global__ void __launch_bounds__(kFinishThreads) attend_finish_kernel(const Par
     const int abort = __syncthreads_or(flagged & 2);
     Walk walk;
     walk.start(p, located.start, end - begin);
-    for (bool first = true; walk.valid(p); walk.next(p), first = false) {
+    // After a wait that ran out every sequence fails: its rows are cleared below, by other blocks than would write them here.
+    for (bool first = true; !abort && walk.valid(p); walk.next(p), first = false) {
         if (!first && (p.flags[c] & 3) == 0) break;                     // later items that end here are whole
         if (walk.st1 != walk.range.steps) break;                  // ends in a later part
         const int64_t item_begin = end - walk.left - walk.at + kItemCost;  // of the item's first step

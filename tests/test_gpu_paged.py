@@ -673,3 +673,27 @@ def test_waits_that_run_out(cuda_module, dtype, dim, page):
         got = chunk_attention(q, cache, table, seq_lens, starts)
         assert got.status.tolist() == [0] * 4
         assert_close(got, definition(q, k, v, table, lens, 0, 0, dim ** -0.5), dtype, dim)
+
+
+@pytest.mark.parametrize("dtype,dim,page", [(torch.bfloat16, 64, 16), (torch.float16, 128, 64)])
+def test_rows_of_a_call_that_gave_up_are_cleared(cuda_module, dtype, dim, page):
+    """No block joins parts of divided items, or computes items again, while another one clears their rows."""
+    from bitmask_speculation_b200 import _native
+    from bitmask_speculation_b200.paged import PagedCache, chunk_attention
+    lens = [(2000, 300), (150, 6000), (9, 20000), (700, 0)]
+    q, k, v, table, seq_lens, starts = make_case(lens, 8, 2, dim, page, dtype)
+    k[table[0, 0]] = math.nan
+    v[table[1, :20].long()] = math.inf
+    cache = PagedCache(k, v)
+    out = torch.full((q.shape[0] + 5, 8, dim), 5.0, dtype=dtype, device="cuda")
+    padded = torch.cat((q, q[:5]))
+    lib = _native.library()
+    _native.check(lib.bms_hold_pages(1))
+    try:
+        for _ in range(3):
+            held = chunk_attention(padded, cache, table, seq_lens, starts, out=out)
+            assert held.status.tolist() == [7] * 4
+            assert bool((out[:-5] == 0).all()) and bool((held.lse[:-5] == -math.inf).all())
+            assert bool((out[-5:] == 5).all())
+    finally:
+        _native.check(lib.bms_hold_pages(0))
