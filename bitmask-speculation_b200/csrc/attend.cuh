@@ -207,9 +207,10 @@ __device__ bool locate(const Params& p, LocateSpace<kBlock>& sp, int c, int ctas
                     for (int i = warp; i < kBlock && base + i < p.a.seqs; i += kW) {
                         const Shape h = sequence_shape(p, base + i);
                         broken |= h.n == 0 && start_broken(p.a, base + i);
-                        int t = 0;
+                        int64_t t = 0;  // beyond 2^31 from 1.05 million new tokens with 128 heads per key head on
                         for (int q = lane; q < h.tiles; q += 32) t += kItemCost + query_range(p, h.n, h.past, h.wide, q).steps;
-                        t = __reduce_add_sync(0xffffffffu, t);
+#pragma unroll
+                        for (int d = 16; d; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
                         if (lane == 0) sp.totals[i] = t;
                     }
                 } else if (s < p.a.seqs) {
