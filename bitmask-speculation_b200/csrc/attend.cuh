@@ -858,7 +858,7 @@ __global__ void __launch_bounds__(kFinishThreads) attend_finish_kernel(const Par
         if (broken && shares_rows(a, s)) return BMS_STATUS_BAD_LENGTH;
         const int64_t low = a.window > 0 ? max(static_cast<int64_t>(0), len - n + 1 - a.window) : 0;
         int bad = 0;
-        for (int32_t i = threadIdx.x; i < (len + a.page_size - 1) / a.page_size; i += kFinishThreads) {
+        for (int32_t i = threadIdx.x; i <= (len - 1) / a.page_size; i += kFinishThreads) {
             const int64_t key = static_cast<int64_t>(i) * a.page_size;
             if (key + a.page_size <= low && key >= a.sinks) continue;
             const int32_t pg = a.table[static_cast<int64_t>(s) * a.width + i];

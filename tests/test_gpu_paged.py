@@ -697,3 +697,24 @@ def test_rows_of_a_call_that_gave_up_are_cleared(cuda_module, dtype, dim, page):
             assert bool((out[-5:] == 5).all())
     finally:
         _native.check(lib.bms_hold_pages(0))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_positions_near_the_32_bit_end(cuda_module, dtype):
+    """A windowed token at the largest position that a table of these pages reaches: it sees what it would see at the end of one
+    page, and a page outside the cache is noticed."""
+    from bitmask_speculation_b200.paged import PagedCache, chunk_attention
+    page = 511 * 128
+    width = (2 ** 31 - 257) // page
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    k, v = (torch.randn((2, page, 1, 64), generator=gen, device="cuda").to(dtype) for _ in range(2))
+    q = torch.randn((1, 2, 64), generator=gen, device="cuda").to(dtype)
+    cache, starts = PagedCache(k, v), i32([0, 1])
+    table = torch.zeros((1, width), dtype=torch.int32, device="cuda")
+    table[0, -1] = 1
+    want = chunk_attention(q, cache, i32([[1]]), i32([page]), starts, window=100).check()
+    got = chunk_attention(q, cache, table, i32([width * page]), starts, window=100)
+    assert got.status.tolist() == [0] and torch.equal(got.out, want.out) and torch.equal(got.lse, want.lse)
+    table[0, -1] = 2
+    assert chunk_attention(q, cache, table, i32([width * page]), starts, window=100).status.tolist() == [11]
+    assert chunk_attention(q, cache, table, i32([(width - 1) * page]), starts, window=100).status.tolist() == [0]
