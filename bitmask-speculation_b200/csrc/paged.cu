@@ -749,6 +749,7 @@ int bms_rotary_append(const void* q, const void* k, const void* v, int32_t dtype
     if (q_stride == nullptr || k_stride == nullptr || v_stride == nullptr) return fail(BMS_ERROR_INVALID_ARGUMENT, "strides must not be NULL");
     BMS_CHECK(check_cache_shape(cache));
     if (cache->dim % 2 != 0 || cache->dim > 65536) return fail(BMS_ERROR_INVALID_ARGUMENT, "dim must be even");
+    if (tokens > 2147483647LL) return fail(BMS_ERROR_UNSUPPORTED, "at most 2^31 - 1 tokens per call");  // a block each
     const int size = dtype == BMS_FLOAT32 ? 4 : 2;
     RelaxedCapture relaxed;
     BMS_CHECK(check_device(device));

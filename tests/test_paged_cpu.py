@@ -79,6 +79,13 @@ def test_chunk_attention_refusals(lib):
         assert lib.bms_attention_workspace_bytes(*bad) == -1, bad
 
 
+def test_rotary_append_tokens_beyond_a_grid(lib):
+    """A block per token: counts that a grid does not hold are refused, not cut to 32 bits."""
+    for tokens in (2 ** 31, 2 ** 32 + 5):
+        assert lib.bms_rotary_append(PTR, PTR, PTR, 1, tokens, 4, pair(256, 64), pair(128, 64), pair(128, 64), PTR, PTR, 32, PTR, PTR, PTR, ctypes.byref(cache()),
+                                     None, 0, None) == UNSUPPORTED
+
+
 # ---------------------------------------------------------------- Python calls
 def fake_cuda():
     """Tensors that claim to be on CUDA: the checks read metadata only."""
