@@ -337,16 +337,6 @@ class NativeModule:
             base + 4 * (4 * seqs + 1), base + 4 * (3 * seqs + 1), dev.index, _stream(dev)))
         return [query_start, seq_lens, positions, slots, held_out, count_out, status]
 
-    @staticmethod
-    def _cache(cache):
-        """The cache's ``bms_paged_cache`` (kept on the cache: its tensors do not change)."""
-        import ctypes
-        if cache._native is None:
-            k, v = cache.k, cache.v
-            strides = ctypes.c_int64 * 3
-            cache._native = _native.Cache(k.data_ptr(), v.data_ptr(), *k.shape, strides(*k.stride()[:3]), strides(*v.stride()[:3]))
-        return ctypes.byref(cache._native)
-
     def rotary_append(self, q, k, v, cos, sin, positions, slots, out, cache, status):
         import ctypes
         n, heads, _ = q.shape
@@ -358,7 +348,7 @@ class NativeModule:
         dev = q.device
         _native.check(self._lib.bms_rotary_append(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), _dtype_code(q), n, heads, at, at + 16, at + 32, cos.data_ptr(),
-            sin.data_ptr(), cos.shape[0], positions.data_ptr(), slots.data_ptr(), out.data_ptr(), self._cache(cache),
+            sin.data_ptr(), cos.shape[0], positions.data_ptr(), slots.data_ptr(), out.data_ptr(), cache.describe(),
             None if status is None else status.data_ptr(), dev.index, _stream(dev)))
 
     def chunk_attention(self, q, cache, table, seq_lens, query_start, scale, window, sinks, out):
@@ -376,7 +366,7 @@ class NativeModule:
             raise RuntimeError(f"no workspace size for device {dev}")
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         _native.check(self._lib.bms_chunk_attention(
-            q.data_ptr() if n else None, _dtype_code(q), n, heads, (ctypes.c_int64 * 2)(*q.stride()[:2]), self._cache(cache),
+            q.data_ptr() if n else None, _dtype_code(q), n, heads, (ctypes.c_int64 * 2)(*q.stride()[:2]), cache.describe(),
             table.data_ptr(), seqs, width, seq_lens.data_ptr(), query_start.data_ptr(), scale, window, sinks,
             out.data_ptr() if n else None, lse.data_ptr() if n else None, status.data_ptr(), ws.data_ptr(), nbytes, dev.index,
             _stream(dev)))

@@ -19,34 +19,47 @@ error, never a CPU computation.
 from __future__ import annotations
 
 import math
+import struct
 from dataclasses import dataclass
 
 from .kernels._extension import load_extension
 from .kernels._validation import device_tensor, index_tensor
 
 
+_PACK = struct.Struct("2P10q").pack  # bms_paged_cache: k, v, shape, k's strides, v's strides
+
+
+def _check_pages(k, v) -> None:
+    device_tensor(k, "k", ndim=4, floating=True)
+    device_tensor(v, "v", ndim=4, floating=True)
+    if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+        raise ValueError("k and v must share shape, dtype and device")
+    if k.numel() == 0:
+        raise ValueError("the cache must not be empty")
+    if k.stride(3) != 1 or v.stride(3) != 1:
+        raise ValueError("the head dimension must be contiguous")
+    for t in (k, v):
+        if any(n > 1 and s <= 0 for n, s in zip(t.shape, t.stride())):
+            raise ValueError("cache strides must be positive")
+
+
+def _form(k, v):
+    return k.shape, k.stride(), v.shape, v.stride(), k.dtype, v.dtype
+
+
 class PagedCache:
     """Keys and values in pages: ``k`` and ``v`` [pages, page_size, kv_heads, dim], float32, bfloat16 or
     float16, on one CUDA device, ``dim`` contiguous, any other strides (a [pages, kv_heads, page_size,
     dim] layout is passed as its transposed view).  Slot j of page p is slot p * page_size + j.  A cache keeps
-    its tensors: other ones make another cache."""
+    its tensors: other ones make another cache.  Every call reads the tensors as they are: one whose memory, shape or
+    strides were changed in place (``resize_``, ``set_``, ``.data``) is checked again."""
 
-    __slots__ = ("_k", "_v", "_native")
+    __slots__ = ("_k", "_v", "_form")
 
     def __init__(self, k, v):
-        device_tensor(k, "k", ndim=4, floating=True)
-        device_tensor(v, "v", ndim=4, floating=True)
-        if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
-            raise ValueError("k and v must share shape, dtype and device")
-        if k.numel() == 0:
-            raise ValueError("the cache must not be empty")
-        if k.stride(3) != 1 or v.stride(3) != 1:
-            raise ValueError("the head dimension must be contiguous")
-        for t in (k, v):
-            if any(n > 1 and s <= 0 for n, s in zip(t.shape, t.stride())):
-                raise ValueError("cache strides must be positive")
+        _check_pages(k, v)
         self._k, self._v = k, v
-        self._native = None
+        self._form = _form(k, v)
 
     @classmethod
     def allocate(cls, pages: int, page_size: int, kv_heads: int, dim: int, *, dtype=None, device="cuda") -> "PagedCache":
@@ -55,6 +68,15 @@ class PagedCache:
         shape = (pages, page_size, kv_heads, dim)
         dtype = torch.bfloat16 if dtype is None else dtype
         return cls(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
+
+    def describe(self):
+        """The C library's ``bms_paged_cache`` of the tensors as they are now."""
+        k, v = self._k, self._v
+        form = _form(k, v)
+        if form != self._form:
+            _check_pages(k, v)
+            self._form = form
+        return _PACK(k.data_ptr(), v.data_ptr(), *form[0], *form[1][:3], *form[3][:3])
 
     @property
     def k(self):
@@ -162,14 +184,15 @@ def rotary_append(q, k, v, cos, sin, positions, slots, cache: PagedCache, *, out
     12: a position outside the tables; such tokens write nothing).
     """
     import torch
-    dtype, dev = cache.k.dtype, cache.k.device
+    pages = cache.k
+    dtype, dev = pages.dtype, pages.device
     device_tensor(q, "q", ndim=3, dtype=dtype, device=dev)
     device_tensor(k, "k", ndim=3, dtype=dtype, device=dev)
     device_tensor(v, "v", ndim=3, dtype=dtype, device=dev)
     n, heads, dim = q.shape
-    if dim % 2 or dim != cache.k.shape[3] or heads == 0:
+    if dim % 2 or dim != pages.shape[3] or heads == 0:
         raise ValueError("q's head dimension must be even and equal the cache's")
-    if k.shape != v.shape or tuple(k.shape) != (n, cache.k.shape[2], dim):
+    if k.shape != v.shape or tuple(k.shape) != (n, pages.shape[2], dim):
         raise ValueError("k and v must be [N, kv_heads, dim] tensors")
     for t, name in ((q, "q"), (k, "k"), (v, "v")):
         _row_strides(t, name)
@@ -205,11 +228,12 @@ def chunk_attention(q, cache: PagedCache, block_table, seq_lens, query_start, *,
     A row whose visible scores are all -inf is NaN with lse -inf.  ``out`` must not overlap the inputs.
     """
     import torch
-    dtype, dev = cache.k.dtype, cache.k.device
+    pages = cache.k
+    dtype, dev = pages.dtype, pages.device
     device_tensor(q, "q", ndim=3, dtype=dtype, device=dev)
     n, heads, dim = q.shape
-    kv_heads = cache.k.shape[2]
-    if dim != cache.k.shape[3] or dim > 256:
+    kv_heads = pages.shape[2]
+    if dim != pages.shape[3] or dim > 256:
         raise ValueError("q's head dimension must equal the cache's and be at most 256")
     if heads == 0 or heads % kv_heads:
         raise ValueError("heads must be a multiple of the cache's kv_heads")

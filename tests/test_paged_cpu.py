@@ -197,3 +197,33 @@ def test_a_cache_keeps_its_tensors():
         for name in ("k", "v", "pages"):
             with pytest.raises(AttributeError):
                 setattr(cache, name, x)
+
+
+def test_a_cache_whose_tensors_moved(monkeypatch):
+    """The description follows tensors that were changed in place; ones that no longer match are refused."""
+    from bitmask_speculation_b200 import paged
+    monkeypatch.setattr(paged, "device_tensor", lambda t, *a, **kw: t)  # tensors on the host: nothing is launched
+    k, v = torch.zeros(4, 16, 2, 64), torch.zeros(4, 16, 2, 64)
+    cache = paged.PagedCache(k, v)
+
+    def check():
+        got = _native.Cache.from_buffer_copy(cache.describe())
+        assert (got.k, got.v) == (k.data_ptr(), v.data_ptr())
+        assert (got.pages, got.page_size, got.kv_heads, got.dim) == tuple(k.shape)
+        assert list(got.k_stride) == list(k.stride()[:3]) and list(got.v_stride) == list(v.stride()[:3])
+    check()
+    k.data = torch.ones(4, 16, 2, 64)
+    check()
+    v.set_(torch.ones(4, 2, 16, 64).transpose(1, 2))
+    check()
+    for t in (k, v):
+        t.resize_(9, 16, 2, 64)
+    check()
+    v.resize_(8, 16, 2, 64)
+    with pytest.raises(ValueError, match="share"):
+        cache.describe()
+    k.resize_(8, 16, 2, 64)
+    check()
+    k.data = torch.ones(8, 16, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="share"):
+        cache.describe()
