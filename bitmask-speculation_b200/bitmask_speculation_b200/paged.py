@@ -13,7 +13,8 @@ own; these operators have no reference counterpart.  A round of speculative deco
 
 Nothing synchronises with the host, every call runs on the current stream of its tensors' device, and
 each can be captured into a CUDA graph.  Inputs must already be on the GPU; a missing library is an
-error, never a CPU computation.
+error, never a CPU computation.  There is no backward pass: inputs that require gradients are refused unless gradients
+are off.
 """
 
 from __future__ import annotations
@@ -206,6 +207,8 @@ def rotary_append(q, k, v, cos, sin, positions, slots, cache: PagedCache, *, out
         raise ValueError("positions and slots must have one entry per token")
     if status is not None and index_tensor(status, "status", ndim=1, device=dev).shape[0] != n:
         raise ValueError("status must be an int32 [N] tensor")
+    if torch.is_grad_enabled():
+        _no_gradients(q, k, v, cos, sin, out, pages, cache.v)
     if out is None:
         out = torch.empty((n, heads, dim), dtype=dtype, device=dev)
     else:
@@ -256,6 +259,8 @@ def chunk_attention(q, cache: PagedCache, block_table, seq_lens, query_start, *,
         raise TypeError("scale must be numeric")
     elif not math.isfinite(scale):
         raise ValueError("scale must be finite")
+    if torch.is_grad_enabled():
+        _no_gradients(q, out, pages, cache.v)
     if out is None:
         out = torch.empty((n, heads, dim), dtype=dtype, device=dev)
     else:
@@ -269,6 +274,11 @@ def _positive_int(value, name: str) -> None:
         raise TypeError(f"{name} must be an integer")
     if value <= 0:
         raise ValueError(f"{name} must be positive")
+
+
+def _no_gradients(*tensors) -> None:
+    if any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("the cache operators have no backward pass: detach the inputs or call them under torch.no_grad()")
 
 
 def _row_strides(t, name: str) -> None:

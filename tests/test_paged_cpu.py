@@ -227,3 +227,38 @@ def test_a_cache_whose_tensors_moved(monkeypatch):
     k.data = torch.ones(8, 16, 2, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="share"):
         cache.describe()
+
+
+def test_inputs_that_require_gradients_are_refused(monkeypatch):
+    """No result is silently detached; with gradients off the same call passes the checks."""
+    from bitmask_speculation_b200 import paged
+    reached = []
+
+    class Library:
+        def rotary_append(self, *args):
+            reached.append("append")
+
+        def chunk_attention(self, *args):
+            reached.append("attention")
+            return None, None
+    monkeypatch.setattr(paged, "load_extension", Library)
+    with fake_cuda():
+        def t(*shape, dtype=torch.bfloat16):
+            return torch.empty(shape, dtype=dtype, device="cuda")
+        i32, f32 = torch.int32, torch.float32
+        append = dict(q=t(5, 4, 64), k=t(5, 2, 64), v=t(5, 2, 64), cos=t(40, 32, dtype=f32), sin=t(40, 32, dtype=f32), positions=t(5, dtype=i32),
+                      slots=t(5, dtype=torch.int64))
+        attend = dict(q=t(5, 4, 64), block_table=t(3, 4, dtype=i32), seq_lens=t(3, dtype=i32), query_start=t(4, dtype=i32))
+        for call, args, names in ((paged.rotary_append, append, ("q", "k", "v", "cos", "sin", "out", "ck", "cv")), (paged.chunk_attention, attend, ("q", "out", "ck", "cv"))):
+            for name in names:
+                pages = {"ck": t(8, 16, 2, 64), "cv": t(8, 16, 2, 64)}
+                changed = dict(args, **({"out": t(5, 4, 64)} if name == "out" else {}))
+                (pages if name in pages else changed)[name].requires_grad_()
+                cache = paged.PagedCache(pages["ck"], pages["cv"])
+                with pytest.raises(ValueError, match="backward"):
+                    call(cache=cache, **changed)
+                assert not reached
+                with torch.no_grad():
+                    call(cache=cache, **changed)
+                assert reached.pop() and not reached
+                (pages if name in pages else changed)[name].requires_grad_(False)
