@@ -144,6 +144,6 @@ def filter_value(value, name: str, batch: int, device, *, low: float, high: floa
         return value
     if isinstance(value, bool) or not isinstance(value, int if integer else (int, float)):
         raise TypeError(f"{name} must be {'an integer' if integer else 'numeric'} or a tensor")
-    if not math.isfinite(value) or value > high or value < low or (low_open and value == low):
+    if not low <= value <= high or (low_open and value == low):
         raise ValueError(f"{name} must be in {'(' if low_open else '['}{low}, {high}]")
     return value

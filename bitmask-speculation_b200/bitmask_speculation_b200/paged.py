@@ -21,12 +21,14 @@ from __future__ import annotations
 
 import math
 import struct
+import sys
 from dataclasses import dataclass
 
 from .kernels._extension import load_extension
 from .kernels._validation import device_tensor, index_tensor
 
 
+_INT64_MAX = 2 ** 63 - 1  # the C library's integers: ctypes would cut larger ones without a word
 _PACK = struct.Struct("2P10q").pack  # bms_paged_cache: k, v, shape, k's strides, v's strides
 
 
@@ -165,8 +167,8 @@ def plan_pages(past_lens, new_lens, held, block_table, free_pages, free_count, *
     _positive_int(page_size, "page_size")
     if isinstance(tokens, bool) or not isinstance(tokens, int):
         raise TypeError("tokens must be an integer")
-    if tokens < 0:
-        raise ValueError("tokens must not be negative")
+    if not 0 <= tokens <= _INT64_MAX:
+        raise ValueError("tokens must be in [0, 2^63)")
     if seqs == 0 or block_table.shape[1] == 0 or free_pages.shape[0] == 0:
         raise ValueError("the plan needs sequences, table entries and pages")
     return PagePlan(*load_extension().page_plan(past_lens, new_lens, held, block_table, free_pages, free_count, page_size, tokens))
@@ -251,13 +253,13 @@ def chunk_attention(q, cache: PagedCache, block_table, seq_lens, query_start, *,
     for value, name in ((window, "window"), (sinks, "sinks")):
         if isinstance(value, bool) or not isinstance(value, int):
             raise TypeError(f"{name} must be an integer")
-        if value < 0:
-            raise ValueError(f"{name} must not be negative")
+        if not 0 <= value <= _INT64_MAX:
+            raise ValueError(f"{name} must be in [0, 2^63)")
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
     elif isinstance(scale, bool) or not isinstance(scale, (int, float)):
         raise TypeError("scale must be numeric")
-    elif not math.isfinite(scale):
+    elif not abs(scale) <= sys.float_info.max:  # NaN, infinities and integers that no float holds
         raise ValueError("scale must be finite")
     if torch.is_grad_enabled():
         _no_gradients(q, out, pages, cache.v)
@@ -272,8 +274,8 @@ def chunk_attention(q, cache: PagedCache, block_table, seq_lens, query_start, *,
 def _positive_int(value, name: str) -> None:
     if isinstance(value, bool) or not isinstance(value, int):
         raise TypeError(f"{name} must be an integer")
-    if value <= 0:
-        raise ValueError(f"{name} must be positive")
+    if not 0 < value <= _INT64_MAX:
+        raise ValueError(f"{name} must be positive and below 2^63")
 
 
 def _no_gradients(*tensors) -> None:

@@ -262,3 +262,26 @@ def test_inputs_that_require_gradients_are_refused(monkeypatch):
                     call(cache=cache, **changed)
                 assert reached.pop() and not reached
                 (pages if name in pages else changed)[name].requires_grad_(False)
+
+
+def test_integers_beyond_64_bits_are_refused():
+    """A foreign call would cut them: a window of 2^64 + 5 would be one of 5."""
+    from bitmask_speculation_b200.kernels.cuda import batched_filtered_sample
+    from bitmask_speculation_b200.paged import PagedCache, chunk_attention, plan_pages
+    with fake_cuda():
+        def t(*shape, dtype=torch.int32):
+            return torch.empty(shape, dtype=dtype, device="cuda")
+        bf16 = torch.bfloat16
+        cache = PagedCache(t(8, 16, 2, 64, dtype=bf16), t(8, 16, 2, 64, dtype=bf16))
+        attend = dict(q=t(5, 4, 64, dtype=bf16), cache=cache, block_table=t(3, 4), seq_lens=t(3), query_start=t(4))
+        for change in (dict(window=2 ** 64 + 5), dict(window=2 ** 63), dict(sinks=2 ** 64 + 1), dict(scale=10 ** 400), dict(scale=-10 ** 400)):
+            with pytest.raises(ValueError):
+                chunk_attention(**{**attend, **change})
+        plan = dict(past_lens=t(3), new_lens=t(3), held=t(3), block_table=t(3, 8), free_pages=t(24), free_count=t(1), page_size=16, tokens=9)
+        for change in (dict(page_size=2 ** 64 + 16), dict(tokens=2 ** 64 + 9)):
+            with pytest.raises(ValueError):
+                plan_pages(**{**plan, **change})
+        logits = t(3, 70, dtype=torch.float32)
+        for change in (dict(top_k=2 ** 63), dict(top_k=10 ** 400), dict(temperature=10 ** 400), dict(top_p=10 ** 400), dict(min_p=float("nan")), dict(top_p=float("-inf"))):
+            with pytest.raises(ValueError):
+                batched_filtered_sample(logits, None, **change)
