@@ -33,6 +33,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <cmath>
 #include <cstring>
@@ -1913,22 +1914,22 @@ __global__ void __launch_bounds__(kThreads, 2) filter_sample_kernel(const Filter
 
 template <typename T>
 int launch_filter(const FilterParams& p, int device, cudaStream_t stream) {
-    static bool ready[kMaxDevices];
-    static int sms[kMaxDevices];
+    static std::atomic<int> sm_counts[kMaxDevices];  // 0: not set up; calls of several threads may set up twice, to the same end
     auto kernel = filter_sample_kernel<T>;
     constexpr size_t smem = sizeof(Shared);
     static_assert(2 * (smem + 1024) <= 228 * 1024, "two CTAs per SM");
-    if (!ready[device]) {
+    int sms = sm_counts[device].load(std::memory_order_acquire);
+    if (sms == 0) {
         BMS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)), "cudaFuncSetAttribute(smem)");
         BMS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "cudaFuncSetAttribute(cluster)");
-        BMS_CUDA(cudaDeviceGetAttribute(&sms[device], cudaDevAttrMultiProcessorCount, device), "sm count");
-        ready[device] = true;
+        BMS_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "sm count");
+        sm_counts[device].store(sms, std::memory_order_release);
     }
     // CTAs per row.  Few rows are split for latency, as long as the parts run side by side (two CTAs per SM): with 1 / 2 / 4 / 8 CTAs,
     // rows of 151,936 with top-p 0.9 take 107 / 66 / 46 / 37 us for 8 of them, 108 / 66 / 46 / 52 for 32, 108 / 67 / 65 / 99 for 64
     // and 108 / 96 / 125 / 184 for 128; 64 float32 rows of 50,257 with min-p 54 / 36 / 25 with 1 / 2 / 4.  Two keep a row that takes long (a wide nucleus) from ending the launch alone: 256 rows of
     // mixed filters and masks take 166 / 133 / 149 / 224 us.  Many rows keep the SMs busy by themselves (600: 398 / 405 / 505 / 799).
-    int c = p.rows * 16 <= sms[device] ? 8 : p.rows * 2 <= sms[device] ? 4 : p.rows <= 2 * sms[device] ? 2 : 1;
+    int c = p.rows * 16 <= sms ? 8 : p.rows * 2 <= sms ? 4 : p.rows <= 2 * sms ? 2 : 1;
     while (c > 1 && p.vocab / c < 4096) c /= 2;
     if (p.rows * c > 2147483647LL) return fail(BMS_ERROR_UNSUPPORTED, "too many rows");
     cudaLaunchConfig_t cfg{};

@@ -617,11 +617,11 @@ std::atomic<int32_t> g_hold_pages{0};  // bms_hold_pages
 
 template <typename T, int D>
 int launch_tiles(const AttendParams& a, int dtype, int device, int sms, void* workspace, cudaStream_t stream) {
-    static bool ready[kMaxDevices];
+    static std::atomic<bool> ready[kMaxDevices];  // calls of several threads may set up twice, to the same end
     auto kernel = tc::attend_tiles_kernel<T, D>;
-    if (!ready[device]) {
+    if (!ready[device].load(std::memory_order_acquire)) {
         BMS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tc::Layout<D>::kSmem), "cudaFuncSetAttribute(smem)");
-        ready[device] = true;
+        ready[device].store(true, std::memory_order_release);
     }
     const int group = a.heads / a.kv_heads;
     CUtensorMap q_map, k_map, v_map;
@@ -665,14 +665,13 @@ int launch_attend(const AttendParams& p, int sms, void* workspace, cudaStream_t 
 }
 
 int sm_count(int device, int& sms) {
-    static int table[kMaxDevices];
+    static std::atomic<int> table[kMaxDevices];
     if (device >= kMaxDevices) return fail(BMS_ERROR_UNSUPPORTED, "device %d", device);
-    if (table[device] == 0) {
-        int n = 0;
-        BMS_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device), "sm count");
-        table[device] = n;
+    sms = table[device].load(std::memory_order_relaxed);
+    if (sms == 0) {
+        BMS_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "sm count");
+        table[device].store(sms, std::memory_order_relaxed);
     }
-    sms = table[device];
     return BMS_SUCCESS;
 }
 

@@ -718,3 +718,36 @@ def test_positions_near_the_32_bit_end(cuda_module, dtype):
     table[0, -1] = 2
     assert chunk_attention(q, cache, table, i32([width * page]), starts, window=100).status.tolist() == [11]
     assert chunk_attention(q, cache, table, i32([(width - 1) * page]), starts, window=100).status.tolist() == [0]
+
+
+def test_calls_of_several_threads(cuda_module):
+    """Four threads on streams of their own run every operator at once (foreign calls release the interpreter's lock)."""
+    from concurrent.futures import ThreadPoolExecutor
+    from bitmask_speculation_b200.kernels.cuda import batched_filtered_sample
+    from bitmask_speculation_b200.paged import PagedCache, chunk_attention, plan_pages, rotary_append
+
+    def work(seed):
+        results = []
+        with torch.cuda.stream(torch.cuda.Stream()):
+            gen = torch.Generator(device="cuda").manual_seed(seed)
+            for i in range(12):
+                dtype, dim = ((torch.bfloat16, 64), (torch.float16, 128), (torch.float32, 32))[i % 3]
+                cache = PagedCache.allocate(64, 16, 2, dim, dtype=dtype)
+                table = torch.zeros((2, 30), dtype=torch.int32, device="cuda")
+                plan = plan_pages(i32([0, 0]), i32([300, 9]), i32([0, 0]), table, torch.arange(64, dtype=torch.int32, device="cuda"), i32([64]),
+                                  page_size=16, tokens=309)
+                q, k, v = (torch.randn((309, h, dim), generator=gen, device="cuda").to(dtype) for h in (4, 2, 2))
+                turned = rotary_append(q, k, v, *rope_tables(320, dim), plan.positions, plan.slots, cache)
+                out = chunk_attention(turned, cache, table, plan.seq_lens, plan.query_start).check().out
+                x = torch.randn((5, 9001), generator=gen, device="cuda").to(dtype)
+                u = torch.rand(5, dtype=torch.float64, generator=gen, device="cuda")
+                results.append((out, batched_filtered_sample(x, None, top_p=0.9, uniforms=u).check().token_ids))
+            torch.cuda.current_stream().synchronize()
+        return results
+
+    want = [work(seed) for seed in range(4)]
+    with ThreadPoolExecutor(4) as pool:
+        got = list(pool.map(work, range(4)))
+    for a, b in zip(want, got):
+        for (x, s), (y, t) in zip(a, b):
+            assert torch.equal(x, y) and torch.equal(s, t)
