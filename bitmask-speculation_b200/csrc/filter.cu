@@ -23,7 +23,7 @@
 //    the kept ones by spans; one CTA walks the span that holds u.
 //  * For the other types one counting pass over value bins estimates where the nucleus ends, one weighing pass
 //    sums the exact masses above and below a bracket of bins around that place and collects the
-//    bracket's tokens, whose sorted prefix gives the exact end; if the estimate missed, the exact masses place
+//    bracket's tokens, whose prefix gives the exact end (they are put into token order first: sums do not depend on timing); if the estimate missed, the exact masses place
 //    the next bracket, and if a bracket overflows (runs of equal scores) the end is bisected over the
 //    64-bit order keys instead.  (bfloat16 rows whose filters end near zero go this way, too.)  By scores 1,152 rows of
 //    248,320 with top-p took 0.84 ms, by brackets 1.15; with the present streams 0.64.
@@ -142,7 +142,6 @@ struct Shared {
     uint32_t fills[kWarps];  // tokens in the warps' segments
     double exp_table[kTable];
     double spans[kMaxCluster * kWarps];
-    unsigned long long extra[kMaxCluster * kWarps];  // kept bracket tokens' mass by span, units of 2^-50
     uint32_t warp_counts[kMaxCluster * kWarps];
     float group_max[kMaxCluster * kWarps * 4];  // of the 8-lane groups of every warp
     MassCount part[2][kMaxCluster];
@@ -1219,6 +1218,37 @@ __device__ __noinline__ uint32_t pool(Shared& sh) {
     return all;
 }
 
+// Brings sh.list's n keys into token order, so that sums over it come out the same in every call, in whatever order the tokens
+// were collected.  Counts by up to 512 ranges of 2^s tokens, then every key's rank in its range.
+__device__ __noinline__ void order_list(Shared& sh, int n, uint32_t vocab) {
+    static_assert(kThreads == 1 << 9 && sizeof sh.segment >= kCap * sizeof(uint64_t) + (2 * kThreads + 1) * sizeof(uint32_t), "space of the order");
+    uint64_t* parted = &sh.segment[0][0];  // its tokens are in the list
+    uint32_t* first = reinterpret_cast<uint32_t*>(parted + kCap);  // [kThreads + 1] where each range starts
+    uint32_t* next = first + kThreads + 1;
+    const int s = max(32 - __clz(vocab - 1) - 9, 0);
+    auto range_of = [&](uint64_t key) { return (0xffffffffu - static_cast<uint32_t>(key)) >> s; };
+    __syncthreads();
+    next[threadIdx.x] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) atomicAdd(&next[range_of(sh.list[i])], 1u);
+    __syncthreads();
+    uint32_t all;
+    const uint32_t before = block_before(next[threadIdx.x], reinterpret_cast<uint32_t*>(sh.warp_count), all);
+    first[threadIdx.x] = next[threadIdx.x] = before;
+    if (threadIdx.x == 0) first[kThreads] = n;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) parted[atomicAdd(&next[range_of(sh.list[i])], 1u)] = sh.list[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const uint64_t key = parted[i];
+        const uint32_t r = range_of(key);
+        uint32_t at = first[r];
+        for (uint32_t j = first[r]; j < first[r + 1]; ++j) at += static_cast<uint32_t>(parted[j]) > static_cast<uint32_t>(key);  // lower tokens
+        sh.list[at] = key;
+    }
+    __syncthreads();
+}
+
 // The keys of bin b's tokens into sh.list (no order).
 template <typename T>
 __device__ __noinline__ void collect_bin(Shared& sh, const RowView<T>& shared_view, int b) {
@@ -1368,33 +1398,45 @@ __device__ __noinline__ bool find_nucleus(Shared& sh, const RowView<T>& shared_v
             for (int i = 0; i < c; ++i) above += sh.above[i], below += sh.below[i];
             int kept;
             double mass;
+            order_list(sh, static_cast<int>(n), shared_view.vocab);
             const uint64_t key = list_cut(sh, static_cast<int>(n), n, sh.top_p, above, below, kept, mass);
             const double limit = sh.top_p * (above + mass + below);
             // Outside the bracket: not one of its tokens kept, or all of them with more below.
             const bool ends_inside = kept > 0 && (above + mass >= limit || b1 == kBins - 1);
             if (ends_inside) {
-                // The bracket's kept tokens join their spans as integers: the order of the additions does not matter.
-                for (int i = threadIdx.x; i < c * kWarps; i += kThreads) sh.extra[i] = 0;
+                // The bracket's kept tokens join their spans, a warp per span: they lie side by side in the list.
                 if (threadIdx.x == 0) sh.passed = 0;
                 __syncthreads();
                 uint32_t passed = 0;
-                for (int i = threadIdx.x; i < n; i += kThreads) {
-                    const Place at = place_of(sh.list[i]);
-                    if (sh.list[i] < key || at.x < sh.floor_x) continue;
-                    ++passed;
-                    const int64_t g = (static_cast<int64_t>(at.t) + shared_view.skew) / RowView<T>::kVec;
-                    int q = static_cast<int>(g * c / groups);  // the CTA whose slice [groups q / c, groups (q + 1) / c) holds g
-                    while (g >= groups * (q + 1) / c) ++q;
-                    while (g < groups * q / c) --q;
+                int32_t* begins = reinterpret_cast<int32_t*>(sh.segment);  // of the spans in the list
+                static_assert(kMaxCluster * kWarps < kThreads, "a start per thread");
+                if (threadIdx.x <= c * kWarps) {
+                    const int q = threadIdx.x / kWarps, w = threadIdx.x % kWarps;
                     const int64_t from = groups * q / c, len = groups * (q + 1) / c - from;
-                    int w = static_cast<int>((g - from) * kWarps / len);
-                    while (g >= from + len * (w + 1) / kWarps) ++w;
-                    while (g < from + len * w / kWarps) --w;
-                    atomicAdd(&sh.extra[q * kWarps + w], static_cast<unsigned long long>(weight_of(at.x, sh.top, sh.rate, sh.exp_table) * 0x1p50));
+                    const int64_t t = (from + len * w / kWarps) * RowView<T>::kVec - shared_view.skew;  // of span c * kWarps: the row's end
+                    int lo = 0, hi = static_cast<int>(n);
+                    while (lo < hi) {
+                        const int mid = (lo + hi) >> 1;
+                        if (static_cast<int64_t>(0xffffffffu - static_cast<uint32_t>(sh.list[mid])) < t) lo = mid + 1;
+                        else hi = mid;
+                    }
+                    begins[threadIdx.x] = lo;
+                }
+                __syncthreads();
+                for (int span = threadIdx.x / 32; span < c * kWarps; span += kWarps) {
+                    const int end = begins[span + 1];
+                    double sum = 0.0;
+                    for (int i = begins[span] + lane; i < end; i += 32) {
+                        const Place at = place_of(sh.list[i]);
+                        if (sh.list[i] < key || at.x < sh.floor_x) continue;
+                        ++passed;
+                        sum += weight_of(at.x, sh.top, sh.rate, sh.exp_table);
+                    }
+                    sum = warp_sum(sum);
+                    if (lane == 0) sh.spans[span] += sum;
                 }
                 if (passed) atomicAdd(&sh.passed, passed);
                 __syncthreads();
-                for (int i = threadIdx.x; i < c * kWarps; i += kThreads) sh.spans[i] += sh.extra[i] * 0x1p-50;
                 if (threadIdx.x == 0) {
                     int64_t all_count = sh.passed;
                     for (int i = 0; i < c; ++i) all_count += sh.counts[i];

@@ -370,3 +370,40 @@ def test_min_p_between_zero_and_the_first_bin(cuda_module, vocab):
         for params in (dict(top_p=0.93, min_p=0.999), dict(top_k=vocab * 3 // 4, min_p=0.999), dict(top_k=vocab * 3 // 4, top_p=0.93, min_p=1.0)):
             got = check(values, np.ones((6, vocab), dtype=bool), "bfloat16", params, u, offset=offset)
             assert max(got.kept_counts.tolist()) <= 5
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_weights_far_below_the_maximum_are_drawn(cuda_module, dtype):
+    """A nucleus that reaches weights of 4e-16 of the largest, which lie in the lowest tokens by themselves: a uniform of 0 draws the
+    first of them.  min-p ends what is kept above 2e-16, so that the rounding of sums near 1 decides nothing."""
+    vocab = 5001
+    rng = np.random.default_rng(3)
+    values = np.empty((3, vocab), dtype=np.float32)
+    values[:, :500] = -35.5
+    values[:, 500:3500] = -36.25
+    values[:, 3500:] = np.float32(rng.uniform(-12.5, -11.5, (3, vocab - 3500))).astype(np.float16)
+    values[:, 4000] = 0.0
+    got = check(values, np.ones((3, vocab), dtype=bool), dtype, dict(top_p=1.0 - 3e-13, min_p=3e-16), np.array([0.0, 0.5, 0.9999]))
+    assert got.token_ids[0].item() == 0 and got.kept_counts[0].item() == 500 + 1501
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_row_in_batches_of_every_size(cuda_module, dtype):
+    """One row's draws in batches that give it 8, 4, 2 and 1 CTAs, twice each: the same tokens and counts."""
+    from bitmask_speculation_b200.kernels.cuda import batched_filtered_sample
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    vocab = 40009
+    others = (torch.randn((700, vocab), generator=gen, device="cuda") * 2).to(getattr(torch, dtype))
+    row = others[0].clone()
+    u = torch.rand(700, dtype=torch.float64, generator=gen, device="cuda")
+    for params in (dict(top_k=40, top_p=0.9), dict(top_p=0.8), dict(top_p=0.999, temperature=2.0), dict(min_p=0.1), dict(top_k=9000, top_p=0.95), dict()):
+        want = None
+        for rows in (1, 3, 40, 200, 700):
+            for at in {0, rows // 2, rows - 1}:
+                x, un = others[:rows].clone(), u[:rows].clone()
+                x[at], un[at] = row, 0.37123
+                for _ in range(2):
+                    got = batched_filtered_sample(x, None, uniforms=un, **params)
+                    one = int(got.token_ids[at]), int(got.kept_counts[at]), int(got.status[at])
+                    want = want or one
+                    assert one == want, (params, rows, at)
