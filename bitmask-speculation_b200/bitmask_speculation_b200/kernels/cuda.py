@@ -153,8 +153,10 @@ def batched_filtered_sample(logits, mask, *, temperature=1.0, top_k=0, top_p=1.0
 
     ``mask``: [B, ceil(V / 32)] int32 rows, or None (every token allowed); with ``mask_rows`` (int32
     [B] on the device) ``mask`` is a table [R, ceil(V / 32)] and row r uses ``mask[mask_rows[r]]`` (status 8
-    for an index outside it).  The other statuses are the sampler's.  Weights and sums are float64:
-    equal inputs give equal tokens whatever the batch around them.  No host synchronization.
+    for an index outside it).  The other statuses are the sampler's.  Weights and sums are float64, in
+    an order that the call's shapes fix: the same call gives the same results.  A row in a batch of another size may be
+    summed in another order; it could come out differently only where its uniform or a filter's limit lies within float64
+    rounding of a boundary.  No host synchronization.
     """
     import torch
     if mask is None:
