@@ -135,7 +135,10 @@ def build_decoder(vocab: int, *, layers: int, dim: int, heads: int, kv_heads: in
         def enable_cache(self, max_tokens: int, *, sequences: int = 1, page_size: int = 64):
             """Keep keys and values of up to ``sequences`` sequences of at most ``max_tokens`` tokens
             between calls: ``logits`` (sequence 0) and ``logits_batch`` then forward only the tokens
-            behind the longest prefix that a sequence shares with its last call."""
+            behind the longest prefix that a sequence shares with its last call.  The forward then runs eagerly,
+            with or without ``enable_graphs``, and drafting on the device goes on without the cache.  A weight that
+            was replaced, moved or changed in place empties the pages; changes through ``.data``, or of
+            inference tensors, are not seen (call ``enable_cache`` again after those)."""
             self._cache = _PagedForward(self, kv_heads, head_dim, sequences, max_tokens, page_size)
             return self
 
@@ -210,6 +213,33 @@ def _rotate(x, cos, sin):
     return _torch().cat((a * cos - b * sin, a * sin + b * cos), -1)
 
 
+def _parameters(module):
+    """A module tree's parameters (``Module.parameters`` without its bookkeeping, which takes five times as long)."""
+    for p in module._parameters.values():
+        if p is not None:
+            yield p
+    for child in module._modules.values():
+        if child is not None:
+            yield from _parameters(child)
+
+
+def _changes(p) -> int:
+    return 0 if p.is_inference() else p._version  # inference tensors are not counted
+
+
+def _weights_of(module) -> list:
+    """What tells this state of a module's weights from another one: the parameters (weak references: a replaced one may be
+    freed), their memory and autograd's count of changes."""
+    from weakref import ref
+    return [(ref(p), p.data_ptr(), _changes(p)) for p in _parameters(module)]
+
+
+def _same_weights(module, weights) -> bool:
+    now = list(_parameters(module))
+    return len(now) == len(weights) and all(
+        p is r() and _changes(p) == count and p.data_ptr() == memory for p, (r, memory, count) in zip(now, weights))
+
+
 class _PagedForward:
     """The keys and values behind ``Decoder.enable_cache``: a paged cache per block, one block table for all
     of them, and the tokens whose keys and values each sequence's pages hold."""
@@ -231,6 +261,7 @@ class _PagedForward:
         angles = torch.arange(max_tokens, device=dev, dtype=torch.float32)[:, None] * model.inv_freq.float()[None, :]
         self.cos, self.sin = angles.cos(), angles.sin()
         self.tokens: list[list[int]] = [[] for _ in range(sequences)]
+        self.weights = _weights_of(model)
 
     def forward(self, sequences, firsts):
         """The last block's rows of one packed forward, and where each sequence's position ``firsts[i]`` is among
@@ -240,6 +271,10 @@ class _PagedForward:
         if not 0 < len(sequences) <= len(self.tokens) or len(firsts) != len(sequences):
             raise ValueError(f"the cache holds {len(self.tokens)} sequences, with one first position each")
         wanted = [[int(t) for t in tokens] for tokens in sequences] + [[] for _ in range(len(self.tokens) - len(sequences))]
+        weights = self.weights
+        if not _same_weights(self.model, weights):  # the pages hold keys and values of other ones
+            self.tokens = [[] for _ in self.tokens]
+            weights = _weights_of(self.model)
         past, new, ids, starts = [], [], [], []
         for i, tokens in enumerate(wanted):
             keep = 0
@@ -263,7 +298,7 @@ class _PagedForward:
         x = model.embed(ids)
         for block, cache in zip(model.blocks, self.caches):
             x = block.paged(x, self.cos, self.sin, plan, cache, self.table)
-        self.tokens = wanted
+        self.tokens, self.weights = wanted, weights
         return x, starts
 
 

@@ -103,3 +103,22 @@ def test_sequences_without_rows(cuda_module):
     some = cached.logits_batch([a + [7], b], [40, 29], [1, 0])
     want = exact.logits(a + [7], 40, 1)
     assert some[1].shape == (0, VOCAB) and float((some[0].double() - want).abs().max()) <= bound(cached, want)
+
+
+def test_changed_weights_forget_the_pages(cuda_module):
+    """Keys and values of other weights are not attended to: a changed parameter makes the next call forward the whole prefix."""
+    model, cached = decoder(torch.bfloat16), decoder(torch.bfloat16).enable_cache(200, page_size=16)
+    other = decoder(torch.bfloat16, seed=9)
+    tokens = torch.randint(0, VOCAB, (120,), generator=torch.Generator().manual_seed(7)).tolist()
+    cached.logits(tokens[:100], 99, 1)
+    changes = (lambda m: m.load_state_dict(other.state_dict()), lambda m: m.blocks[0].kv.weight.mul_(-1.5),
+               lambda m: setattr(m.blocks[1].q, "weight", torch.nn.Parameter(m.blocks[1].q.weight.detach().roll(1, 0))),
+               lambda m: m.embed.weight.detach().neg_(),
+               lambda m: setattr(m.blocks[0], "o", copy.deepcopy(other.blocks[1].o)))
+    for i, change in enumerate(changes):
+        with torch.no_grad():
+            change(model), change(cached)
+        n = 101 + i
+        want = copy.deepcopy(model).double().logits(tokens[:n], n - 1, 1)
+        got = cached.logits(tokens[:n], n - 1, 1)
+        assert float((got.double() - want).abs().max()) <= bound(model, want), i
