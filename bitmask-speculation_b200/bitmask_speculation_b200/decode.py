@@ -223,21 +223,17 @@ def _parameters(module):
             yield from _parameters(child)
 
 
-def _changes(p) -> int:
-    return 0 if p.is_inference() else p._version  # inference tensors are not counted
-
-
 def _weights_of(module) -> list:
     """What tells this state of a module's weights from another one: the parameters (weak references: a replaced one may be
-    freed), their memory and autograd's count of changes."""
+    freed), their memory and autograd's count of changes (inference tensors have none)."""
     from weakref import ref
-    return [(ref(p), p.data_ptr(), _changes(p)) for p in _parameters(module)]
+    return [(ref(p), p.data_ptr(), None if p.is_inference() else p._version) for p in _parameters(module)]
 
 
 def _same_weights(module, weights) -> bool:
     now = list(_parameters(module))
     return len(now) == len(weights) and all(
-        p is r() and _changes(p) == count and p.data_ptr() == memory for p, (r, memory, count) in zip(now, weights))
+        p is r() and p.data_ptr() == memory and (count is None or p._version == count) for p, (r, memory, count) in zip(now, weights))
 
 
 class _PagedForward:
