@@ -1753,7 +1753,7 @@ __global__ void __launch_bounds__(kThreads, 2) filter_sample_kernel(const Filter
         if (rank == 0 && threadIdx.x == 0) finish(-1, 0, code);
         return;
     }
-    if (c > 1) ptx::cluster_arrive();  // first_pass waits for it before it stores into other CTAs
+    if (c > 1) ptx::cluster_arrive_relaxed();  // first_pass waits for it before it stores into other CTAs
     RowView<T>& view = *reinterpret_cast<RowView<T>*>(sh.view);
     static_assert(sizeof(RowView<T>) <= sizeof sh.view, "space of the view");
     if (threadIdx.x == 0) {
