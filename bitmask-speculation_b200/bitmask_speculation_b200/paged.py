@@ -183,7 +183,7 @@ def rotary_append(q, k, v, cos, sin, positions, slots, cache: PagedCache, *, out
     gives them.  Element i and i + dim / 2 of a head turn together; sums are float32, rounded once.  A
     token with slot -1 writes no key or value; one with position -1 nothing, its row of the result is
     left as it was (unspecified when ``out`` is not given).  ``out``: a contiguous tensor shaped like ``q`` for
-    the result (a contiguous ``q`` itself may be given).  ``status``: an int32 [N] tensor for a code per token (0; 11: a slot outside the cache;
+    the result (a contiguous ``q`` itself may be given; it overlaps nothing else).  ``status``: an int32 [N] tensor for a code per token (0; 11: a slot outside the cache;
     12: a position outside the tables; such tokens write nothing).
     """
     import torch
@@ -231,6 +231,10 @@ def chunk_attention(q, cache: PagedCache, block_table, seq_lens, query_start, *,
     they hold.  ``block_table`` int32 [S, width], ``seq_lens`` int32 [S], ``query_start`` int32
     [S + 1].  Rows behind the last sequence are left as they were (unspecified when ``out`` is not given).
     A row whose visible scores are all -inf is NaN with lse -inf.  ``out`` must not overlap the inputs.
+
+    Tensor cores take 16-bit types of dim 64 or 128 in pages that divide 128 slots or are divided by them (8 slots at
+    least), with bases and strides on 16-byte boundaries and no broadcast; every other call goes row by row, which is
+    meant for small ones (long float32 caches and prompts take longer than elementary operations do).
     """
     import torch
     pages = cache.k

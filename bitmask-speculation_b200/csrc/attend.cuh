@@ -17,17 +17,18 @@
 // operand, so neither P nor V is transposed or copied.  While a warpgroup turns S into P the tensor cores work for
 // the other one.  A softmax thread owns a row: no shuffles.  O is rescaled only when a row's maximum grew by more
 // than a threshold (2^8 for bfloat16); sums stay float32, weights are rounded once to the inputs' type for the
-// second product, because the tensor cores take both operands in that type.
+// second product, because the tensor cores take both operands in that type.  Exponentials are ex2.approx (2 ulp): 2^-22 beside
+// the weights' 2^-8 (2^-11 for float16).
 //
 // Hidden keys.  Scores of keys that a row does not see are replaced, so any bits there vanish.  Values cannot be:
 // 0 * NaN is NaN.  In tiles that are not seen by every row, non-finite values of keys that some row does not see are
 // zeroed in shared memory before the product; if another row does see such a key the CTA flags its range, and
 // attend_finish_kernel computes those items again row by row.
 //
-// Bound.  Prompt chunks (dim 128) run at 0.87 PFLOP/s, 1.0 in the steady state: a warpgroup's step is a chain (scores 0.4 us,
+// Bound.  Prompt chunks (dim 128) run at 0.86 - 0.9 PFLOP/s, 1.0 in the steady state: a warpgroup's step is a chain (scores 0.4 us,
 // load 0.1, maximum 0.15, exponentials 1.2, second half of the output product 0.2), and the two warpgroups' chains overlap; TMEM
 // has no room for a second score tile of each (2 x 128 columns of scores, 2 x 128 of output).  Verification windows over long
-// caches read them at 4.3 TB/s (6.5 in the steady state).  What is lost lies between items, about 14 us of it per CTA and item
+// caches read them at 4.2 - 4.5 TB/s (6.5 in the steady state).  What is lost lies between items, about 14 us of it per CTA and item
 // (output, first scores), at the start (13 us to the first scores, the search for the part's start and cold code in it)
 // and in the joining kernel (18 - 27 us for the longest cases); single tokens over short caches take 24 us of that alone.
 // Tried without gain: a warp of its own for the cleaning of values, handing the first half of the weights over later, looking up
