@@ -676,6 +676,12 @@ int sm_count(int device, int& sms) {
     return BMS_SUCCESS;
 }
 
+int check_row_strides(const int64_t* s) {
+    if (s == nullptr) return fail(BMS_ERROR_INVALID_ARGUMENT, "strides must not be NULL");
+    if (s[0] < 0 || s[1] < 0) return fail(BMS_ERROR_INVALID_ARGUMENT, "strides must not be negative");
+    return BMS_SUCCESS;
+}
+
 int check_cache_shape(const bms_paged_cache* c) {
     if (c == nullptr) return fail(BMS_ERROR_INVALID_ARGUMENT, "cache must not be NULL");
     if (c->pages <= 0 || c->page_size <= 0 || c->kv_heads <= 0 || c->dim <= 0 || c->pages > 2147483647LL || c->page_size > 65536 || c->kv_heads > 65535)
@@ -746,7 +752,7 @@ int bms_rotary_append(const void* q, const void* k, const void* v, int32_t dtype
     BMS_CHECK(check_kind(dtype));
     if (tokens < 0 || heads <= 0 || heads > 65535 || max_positions <= 0)
         return fail(BMS_ERROR_INVALID_ARGUMENT, "tokens, heads and max_positions must be positive");
-    if (q_stride == nullptr || k_stride == nullptr || v_stride == nullptr) return fail(BMS_ERROR_INVALID_ARGUMENT, "strides must not be NULL");
+    for (const int64_t* s : {q_stride, k_stride, v_stride}) BMS_CHECK(check_row_strides(s));
     BMS_CHECK(check_cache_shape(cache));
     if (cache->dim % 2 != 0 || cache->dim > 65536) return fail(BMS_ERROR_INVALID_ARGUMENT, "dim must be even");
     if (tokens > 2147483647LL) return fail(BMS_ERROR_UNSUPPORTED, "at most 2^31 - 1 tokens per call");  // a block each
@@ -792,7 +798,7 @@ int bms_chunk_attention(const void* q, int32_t dtype, int64_t tokens, int64_t he
         return fail(BMS_ERROR_INVALID_ARGUMENT, "tokens, heads, seqs and width must be positive");
     if (window < 0 || sinks < 0) return fail(BMS_ERROR_INVALID_ARGUMENT, "window and sinks must not be negative");
     if (!std::isfinite(scale) || std::fabs(scale) > 1e30) return fail(BMS_ERROR_INVALID_ARGUMENT, "scale must be finite");
-    if (q_stride == nullptr) return fail(BMS_ERROR_INVALID_ARGUMENT, "strides must not be NULL");
+    BMS_CHECK(check_row_strides(q_stride));
     BMS_CHECK(check_cache_shape(cache));
     if (cache->dim > 256) return fail(BMS_ERROR_UNSUPPORTED, "dim is at most 256");
     if (heads % cache->kv_heads != 0) return fail(BMS_ERROR_INVALID_ARGUMENT, "heads must be a multiple of the cache's kv_heads");

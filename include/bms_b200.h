@@ -357,8 +357,8 @@ BMS_API int bms_page_plan(const int32_t *past_lens, const int32_t *new_lens, con
                           int32_t *free_count_out, int32_t *status, int32_t device, void *stream);
 
 /* Rotates a step's queries and keys and writes keys and values into the cache.  q [tokens, heads,
- * dim], k and v [tokens, kv_heads, dim] with the given token and head strides (elements; dim is
- * contiguous and even).  With half = dim / 2, element i < half and i + half of a head at position p
+ * dim], k and v [tokens, kv_heads, dim] with the given token and head strides (elements, not
+ * negative; dim is contiguous and even).  With half = dim / 2, element i < half and i + half of a head at position p
  * become a cos[p, i] - b sin[p, i] and a sin[p, i] + b cos[p, i]; cos and sin are float32
  * [max_positions, half].  Sums in float32, rounded once.  q_out is contiguous [tokens, heads, dim] and
  * may be q itself where q is contiguous; token t's key and value go to slot slots[t].  A token with

@@ -86,6 +86,15 @@ def test_rotary_append_tokens_beyond_a_grid(lib):
                                      None, 0, None) == UNSUPPORTED
 
 
+def test_negative_row_strides(lib):
+    """They would lead in front of the tensors' memory (the cache's are refused with its shape)."""
+    good, bad, c = pair(256, 64), (pair(-256, 64), pair(256, -64)), cache()
+    for b in bad:
+        for qs, ks, vs in ((b, good, good), (good, b, good), (good, good, b)):
+            assert lib.bms_rotary_append(PTR, PTR, PTR, 1, 3, 4, qs, ks, vs, PTR, PTR, 32, PTR, PTR, PTR, ctypes.byref(c), None, 0, None) == INVALID
+        assert lib.bms_chunk_attention(PTR, 1, 3, 4, b, ctypes.byref(c), PTR, 2, 4, PTR, PTR, 0.125, 0, 0, PTR, PTR, PTR, PTR, 1 << 40, 0, None) == INVALID
+
+
 # ---------------------------------------------------------------- Python calls
 def fake_cuda():
     """Tensors that claim to be on CUDA: the checks read metadata only."""
