@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <cmath>
 
 #include "../../include/bms_b200.h"
@@ -635,7 +636,7 @@ int launch_tiles(const AttendParams& a, int dtype, int device, int sms, void* wo
     unsigned char* rest = static_cast<unsigned char*>(workspace) + ((sms * 4 + 255) / 256) * 256;
     p.parts = reinterpret_cast<float*>(rest);
     p.part_lse = p.parts + static_cast<int64_t>(sms) * 2 * 256 * D;
-    p.scale2 = std::max(std::fabs(a.scale) * 1.4426950408889634f, 1e-30f);  // a factor of 0 would turn masked scores into NaN
+    p.scale2 = std::max(std::fabs(a.scale) * 1.4426950408889634f, FLT_MIN);  // a factor of 0 would turn masked scores into NaN
     p.negate = a.scale < 0.f ? 0x80000000u : 0u;
     p.group = group;
     p.tile_tokens = tc::kTile / p.group;

@@ -751,3 +751,15 @@ def test_calls_of_several_threads(cuda_module):
     for a, b in zip(want, got):
         for (x, s), (y, t) in zip(a, b):
             assert torch.equal(x, y) and torch.equal(s, t)
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 64)])
+@pytest.mark.parametrize("scale", [0.0, 1e-33, -1e-33])
+def test_scales_near_zero_of_large_scores(cuda_module, dtype, dim, scale):
+    """A scale of 0 weighs all visible keys alike however large the products are; one of 1e-33 is not rounded up to anything."""
+    from bitmask_speculation_b200.paged import PagedCache, chunk_attention
+    lens = LENS["round"]
+    q, k, v, table, seq_lens, starts = make_case(lens, 4, 2, dim, 16, dtype)
+    q, k = q * 2.0 ** 51, k * 2.0 ** 50
+    got = chunk_attention(q, PagedCache(k, v), table, seq_lens, starts, scale=scale)
+    assert_close(got, definition(q, k, v, table, lens, 0, 0, scale), dtype, dim)
