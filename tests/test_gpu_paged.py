@@ -763,3 +763,51 @@ def test_scales_near_zero_of_large_scores(cuda_module, dtype, dim, scale):
     q, k = q * 2.0 ** 51, k * 2.0 ** 50
     got = chunk_attention(q, PagedCache(k, v), table, seq_lens, starts, scale=scale)
     assert_close(got, definition(q, k, v, table, lens, 0, 0, scale), dtype, dim)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_captured_round_follows_its_inputs(cuda_module, dtype):
+    """Plan, append, attention and sampling captured once: replays with other lengths, tables, values and uniforms equal direct
+    calls, on a second stream too."""
+    from bitmask_speculation_b200.kernels.cuda import batched_filtered_sample
+    from bitmask_speculation_b200.paged import PagedCache, chunk_attention, plan_pages, rotary_append
+    seqs, width, page, n, dim = 3, 40, 16, 420, 64
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    rand = lambda *shape: torch.randn(shape, generator=gen, device="cuda").to(dtype)  # noqa: E731
+    cos, sin = rope_tables(width * page, dim)
+    state = dict(past=i32([0, 0, 0]), new=i32([400, 9, 1]), held=i32([0] * 3), count=i32([120]), u=torch.rand(seqs, dtype=torch.float64, generator=gen, device="cuda"),
+                 q=rand(n, 4, dim), k=rand(n, 2, dim), v=rand(n, 2, dim), x=rand(seqs, 9001))
+
+    def run(s, table, free, cache):
+        plan = plan_pages(s["past"], s["new"], s["held"], table, free, s["count"], page_size=page, tokens=n)
+        turned = rotary_append(s["q"], s["k"], s["v"], cos, sin, plan.positions, plan.slots, cache)
+        out = chunk_attention(turned, cache, table, plan.seq_lens, plan.query_start, window=300, sinks=4)
+        return plan, out, batched_filtered_sample(s["x"], None, top_p=0.9, top_k=3000, uniforms=s["u"])
+
+    def fresh():
+        return torch.zeros((seqs, width), dtype=torch.int32, device="cuda"), torch.arange(120, dtype=torch.int32, device="cuda"), PagedCache.allocate(120, page, 2, dim, dtype=dtype)
+
+    mine, other = fresh(), fresh()
+    warm = fresh()
+    run(state, *warm)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = run(state, *mine)
+    stream = torch.cuda.Stream()
+    for i, (past, new) in enumerate([([0, 0, 0], [400, 9, 1]), ([391, 5, 1], [9, 300, 1]), ([0, 305, 2], [200, 0, 9]), ([200, 300, 0], [9, 9, 0])]):
+        state["past"].copy_(i32(past)), state["new"].copy_(i32(new))
+        for name in ("q", "k", "v", "x"):
+            state[name].copy_(rand(*state[name].shape))
+        state["u"].uniform_(generator=gen)
+        want = run(state, *other)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream if i % 2 else torch.cuda.current_stream()):
+            graph.replay()
+        torch.cuda.synchronize()
+        for a, b in ((held[0].check(), want[0].check()), (held[1].check(), want[1].check()), (held[2].check(), want[2].check())):
+            for name in a.__slots__:
+                x, y = getattr(a, name), getattr(b, name)
+                rows = sum(new) if name in ("out", "lse") else None  # rows behind the last sequence are unspecified
+                assert torch.equal(x[:rows], y[:rows]), (i, name)
+        assert torch.equal(mine[0], other[0]) and torch.equal(mine[1], other[1]) and torch.equal(mine[2].k, other[2].k) and torch.equal(mine[2].v, other[2].v)
+        state["held"].copy_(want[0].held), state["count"].copy_(want[0].free_count)
