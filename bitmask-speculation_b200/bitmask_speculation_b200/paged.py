@@ -230,7 +230,8 @@ def chunk_attention(q, cache: PagedCache, block_table, seq_lens, query_start, *,
     ``scale`` is 1 / sqrt(dim) unless given.  Keys that a row does not see never reach it, whatever
     they hold.  ``block_table`` int32 [S, width], ``seq_lens`` int32 [S], ``query_start`` int32
     [S + 1].  Rows behind the last sequence are left as they were (unspecified when ``out`` is not given).
-    A row whose visible scores are all -inf is NaN with lse -inf.  ``out`` must not overlap the inputs.
+    A row whose visible scores are all -inf is NaN with lse -inf; one that sees a score of +inf or NaN is NaN with
+    lse NaN.  ``out`` must not overlap the inputs.
 
     Tensor cores take 16-bit types of dim 64 or 128 in pages that divide 128 slots or are divided by them (8 slots at
     least), with bases and strides on 16-byte boundaries and no broadcast; every other call goes row by row, which is

@@ -23,8 +23,8 @@
 //    the kept ones by spans; one CTA walks the span that holds u.
 //  * For the other types one counting pass over value bins estimates where the nucleus ends, one weighing pass
 //    sums the exact masses above and below a bracket of bins around that place and collects the
-//    bracket's tokens, whose prefix gives the exact end (they are put into token order first: sums do not depend on timing); if the estimate missed, the exact masses place
-//    the next bracket, and if a bracket overflows (runs of equal scores) the end is bisected over the
+//    bracket's tokens, whose prefix gives the exact end (they are put into token order first: sums do not depend on
+//    timing); if the estimate missed, the exact masses place the next bracket, and if a bracket overflows (runs of equal scores) the end is bisected over the
 //    64-bit order keys instead.  (bfloat16 rows whose filters end near zero go this way, too.)  By scores 1,152 rows of
 //    248,320 with top-p took 0.84 ms, by brackets 1.15 (masked rows); with the present streams 0.64.  Unmasked rows take 0.85 by
 //    scores, 1.24 (float16) and 1.50 (float32) by brackets; 8 rows of 151,936 equal scores 0.69 by bisection.

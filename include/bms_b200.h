@@ -386,7 +386,7 @@ BMS_API int64_t bms_attention_workspace_bytes(int32_t device, int64_t tokens, in
  * `tokens`, rows that another sequence claims too, seq_lens below n or above the table row; 11 for a visible page
  * outside the cache; 7 where a wait inside the kernel gave up; the rows of a failed sequence are 0 with lse -inf, but for
  * those of its claim that belong to another one (only where query_start is out of order).  A row whose visible
- * scores are all -inf is NaN with lse -inf.  `out` must not overlap the inputs.  Rows behind query_start[seqs] are left as they
+ * scores are all -inf is NaN with lse -inf, one that sees a score of +inf or NaN is NaN with lse NaN.  `out` must not overlap the inputs.  Rows behind query_start[seqs] are left as they
  * were. */
 BMS_API int bms_chunk_attention(const void *q, int32_t dtype, int64_t tokens, int64_t heads, const int64_t q_stride[2],
                                 const bms_paged_cache *cache, const int32_t *table, int64_t seqs, int64_t width,

@@ -811,3 +811,46 @@ def test_a_captured_round_follows_its_inputs(cuda_module, dtype):
                 assert torch.equal(x[:rows], y[:rows]), (i, name)
         assert torch.equal(mine[0], other[0]) and torch.equal(mine[1], other[1]) and torch.equal(mine[2].k, other[2].k) and torch.equal(mine[2].v, other[2].v)
         state["held"].copy_(want[0].held), state["count"].copy_(want[0].free_count)
+
+
+@pytest.mark.parametrize("dtype,dim,page", [(torch.bfloat16, 64, 16), (torch.float16, 128, 64), (torch.float16, 64, 24), (torch.float32, 32, 16)])
+def test_scores_that_are_not_finite(cuda_module, dtype, dim, page):
+    """Keys whose scores are -inf weigh nothing; a row that sees one of +inf or NaN is NaN, and no other row is."""
+    from bitmask_speculation_b200.paged import PagedCache, chunk_attention
+    lens = [(1, 300), (9, 6000), (200, 150), (3, 2), (40, 700)]
+    for window, sinks in ((0, 0), (90, 3)):
+        q, k, v, table, seq_lens, starts = make_case(lens, 4, 2, dim, page, dtype, poison=False)
+        q[..., 0] = 1.0
+        gen = torch.Generator().manual_seed(dim)
+        bad, low = {}, {}
+        for s, (n, past) in enumerate(lens):
+            for what, count in ((low, 5), (bad, 1 if n > 3 else 0)):
+                what[s] = torch.randint(past + (n // 2 if what is bad else 0), past + n, (count,), generator=gen).tolist()
+            for i, j in enumerate(low[s] + bad[s]):
+                pg = int(table[s, j // page])
+                k[pg, j % page, :, 0] = -math.inf if j not in bad[s] else (math.inf if s % 2 else math.nan)
+        got = chunk_attention(q, PagedCache(k, v), table, seq_lens, starts, window=window, sinks=sinks).check()
+        row = 0
+        for s, (n, past) in enumerate(lens):
+            at = torch.arange(n + past, device="cuda")
+            pg = table[s].long()[at // page]
+            ks, vs = k[pg, at % page].double(), v[pg, at % page].double()
+            age = (past + torch.arange(n, device="cuda"))[:, None] - at
+            seen = age >= 0
+            if window:
+                seen &= (age < window) | (at < sinks)
+            for h in range(4):
+                score = q[row:row + n, h].double() @ torch.nan_to_num(ks[:, h // 2], nan=0, posinf=0, neginf=0).T
+                extra = torch.where(torch.isfinite(ks[:, h // 2, 0]), 0.0, ks[:, h // 2, 0])
+                score = ((score + extra) * dim ** -0.5).masked_fill(~seen, -math.inf)
+                want = torch.softmax(score, 1) @ vs[:, h // 2]
+                broken = (~(score < math.inf)).any(1)
+                mine, lse = got.out[row:row + n, h].double(), got.lse[row:row + n, h]
+                assert torch.equal(torch.isnan(mine).all(1), torch.isnan(want).all(1)) and torch.equal(torch.isnan(mine).any(1), torch.isnan(want).any(1))
+                assert torch.equal(torch.isnan(lse), broken)
+                # Weights and result rounded once each, scores of a few units good to 2^-15 (dim + 4 roundings of 2^-24 of terms below 2^2).
+                eps = EPS[dtype] / 2
+                weight = torch.softmax(score, 1) @ vs[:, h // 2].abs()
+                off = (mine - want).abs()[~broken & ~torch.isnan(want).any(1)]
+                assert bool((off <= ((2 * eps + 2.0 ** -14) * weight + 2.0 ** -20)[~broken & ~torch.isnan(want).any(1)]).all())
+            row += n
